@@ -266,6 +266,60 @@ int mmfe_patch_embed_shape(const mmfe_patch_embed* handle, int64_t* n_patches, i
 int mmfe_patch_embed_run(const mmfe_patch_embed* handle, const void* x, int64_t x_batch_stride, int64_t n_batch, void* out,
                          int64_t out_batch_stride, void* hip_stream);
 
+/* ---- rotary positions with several axes ------------------------------------------------------------------------------
+ * The tokens of mmfe_patch_embed_run sit on a grid (frequency and time of a spectrogram; height and width of an image; with a time
+ * axis in front, video).  Element pair i of every query and key head turns by position[axis(i)] * theta_i.  sections[a] pairs
+ * belong to axis a, in order; R = sum of the sections; the dim - 2 R elements behind them pass through.
+ *   ladder   MMFE_ROTARY_SHARED: theta_i = base^(-i / R), one ladder over all pairs;  MMFE_ROTARY_PER_AXIS: base^(-j / sections[a])
+ *            for the j-th pair of axis a
+ *   pairing  MMFE_ROTARY_HALVES: elements (i, i + R);  MMFE_ROTARY_ADJACENT: elements (2 i, 2 i + 1)
+ * Angles are formed in float64.  The reference adds a learned position table instead (classification/vggsound/models/vit_model.py:
+ * 384-385); nothing there corresponds.  The handle owns the frequency table and may be shared between threads and streams. */
+#define MMFE_ROTARY_SHARED    0
+#define MMFE_ROTARY_PER_AXIS  1
+#define MMFE_ROTARY_HALVES    0
+#define MMFE_ROTARY_ADJACENT  1
+typedef struct mmfe_rotary mmfe_rotary;
+typedef struct mmfe_rotary_args {
+    int32_t struct_size;    /* = sizeof(mmfe_rotary_args) */
+    int32_t dtype;          /* MMFE_OUT_F32 / _F16 / _BF16: element type of q, k and their outputs */
+    int32_t pos_64;         /* 1: positions are int64_t; 0: int32_t */
+    int32_t inverse;        /* 1: rotate by the negative angle (the gradient) */
+    int32_t heads_q, heads_k;
+    int32_t dim;            /* elements of a head, 2 R to 1024, unit stride */
+    int32_t reserved;
+    int64_t n_batch, n_tokens;
+    const void* q;          /* device, (n_batch, n_tokens, heads_q, dim) with strides q_stride (elements) */
+    void* q_out;            /* may be q itself with the same strides: in place */
+    const void* k;
+    void* k_out;
+    int64_t q_stride[3], q_out_stride[3], k_stride[3], k_out_stride[3];
+    const void* positions;  /* device, (axes, n_batch, n_tokens) with strides pos_stride (batch stride 0: shared) */
+    int64_t pos_stride[3];
+} mmfe_rotary_args;
+int mmfe_rotary_create(int32_t n_axes, const int32_t* sections, int32_t ladder, int32_t pairing, double base, int device, mmfe_rotary** out_handle);
+int mmfe_rotary_destroy(mmfe_rotary* handle);
+/* One launch for q and k; either may have no heads.  Asynchronous on hip_stream, allocates nothing. */
+int mmfe_rotary_run(const mmfe_rotary* handle, const mmfe_rotary_args* args, void* hip_stream);
+
+/* ---- global norm of many tensors, and clipping by it ------------------------------------------------------------------
+ * What a training step of the encoders does between backward and the optimizer (the reference's loops call the optimizer directly,
+ * classification/vggsound/vanilla_single.py:75-80).  norm = (sum of all squares)^(1/2) (MMFE_NORM_2) or the largest magnitude
+ * (MMFE_NORM_MAX) over all tensors, summed in float64 in a fixed order; with out != NULL every tensor times
+ * min(1, max_norm / (norm + 1e-6)) goes to out[i], as out_dtype[i]; out[i] may be x[i] with the same type (in place: nothing is
+ * written when the factor is 1).  A NaN norm makes every output NaN; an infinite one makes finite values zero.
+ *   x, numel, dtype, out, out_dtype   HOST arrays of n_tensors entries, read before the call returns; x[i] / out[i] are device
+ *                                     pointers of numel[i] contiguous elements (MMFE_OUT_* types), aligned to their elements
+ *   partials                          device, mmfe_grad_partials(n_tensors) doubles, the call's own until it has run
+ *   norm                              device, one float
+ * What is written must not overlap any other tensor of the call (MMFE_EINVAL).  Asynchronous on hip_stream, allocates nothing on
+ * the device. */
+#define MMFE_NORM_2    2
+#define MMFE_NORM_MAX  0
+int64_t mmfe_grad_partials(int64_t n_tensors);
+int mmfe_grad_clip(int64_t n_tensors, const void* const* x, const int64_t* numel, const int32_t* dtype, void* const* out, const int32_t* out_dtype,
+                   int32_t norm_kind, float max_norm, double* partials, float* norm, int device, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

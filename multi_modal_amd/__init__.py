@@ -10,16 +10,20 @@ the Python call signatures of lixinghe1999/multi_modal's dataset classes.
     stats.cal_norm                   cal_norm                                     (vggsound.py:85-107)
     resample.load_resampled          the resampling of librosa.load(sr=16000)     (vggsound.py:114; extract_audio.py:6-13)
     patch_embed.PatchEmbed           PatchEmbed.forward with the audio projection (models/vit_model.py:193-199, 435)
+    rotary.Rotary                    rotary positions with several axes for the tokens' query and key heads
+    gradients.clip_grad_norm         global gradient norm and clipping between backward and the optimizer
     loader.DevicePrefetcher          `batch[k].to(device)` of the training loop, overlapped    (vanilla_multi.py:76-77, 89-92)
     partition.*                      batch sharding over the GPUs of a node + all-gather of features
 
 All arithmetic runs in libmmfe.so (hand-written HIP for gfx950, C ABI in include/mmfe.h).
 """
-from . import _native, epic, har, kaldi, loader, logmel, melbank, partition, patch_embed, resample, stats, transforms, vggsound  # noqa: F401
+from . import _native, epic, gradients, har, kaldi, loader, logmel, melbank, partition, patch_embed, resample, rotary, stats, transforms, vggsound  # noqa: F401
 from ._native import MmfeError, library_path, load_library  # noqa: F401
 from .epic import log_specgram, log_specgram_batch, spec_to_tensor  # noqa: F401
+from .gradients import clip_grad_norm, grad_norm  # noqa: F401
 from .har import stft_mag  # noqa: F401
 from .resample import load_resampled, resample_batch  # noqa: F401
+from .rotary import Rotary, grid_positions  # noqa: F401
 from .kaldi import fbank, fbank_batch  # noqa: F401
 from .transforms import frame_signal  # noqa: F401
 from .vggsound import preprocessing_audio, preprocessing_audio_batch  # noqa: F401
@@ -27,4 +31,5 @@ from .vggsound import preprocessing_audio, preprocessing_audio_batch  # noqa: F4
 __all__ = [
     "MmfeError", "library_path", "load_library", "fbank", "fbank_batch", "preprocessing_audio",
     "preprocessing_audio_batch", "log_specgram", "log_specgram_batch", "spec_to_tensor", "stft_mag", "frame_signal", "resample_batch", "load_resampled",
+    "Rotary", "grid_positions", "clip_grad_norm", "grad_norm",
 ]

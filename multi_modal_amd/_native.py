@@ -26,12 +26,17 @@ LAYOUT_TIME_MAJOR, LAYOUT_FEAT_MAJOR = 0, 1
 OUT_F32, OUT_F16, OUT_BF16 = 0, 1, 2
 IN_F32, IN_S16, IN_F64, IN_F16, IN_BF16 = 0, 1, 2, 3, 4
 NOALLOC_MAX_ROWS = 65536
+ROTARY_SHARED, ROTARY_PER_AXIS = 0, 1
+ROTARY_HALVES, ROTARY_ADJACENT = 0, 1
+NORM_2, NORM_MAX = 2, 0
 
 EXPORTED_SYMBOLS = (
     "mmfe_abi_version", "mmfe_last_error", "mmfe_device_count", "mmfe_spec_out_shape",
     "mmfe_plan_create", "mmfe_plan_destroy", "mmfe_run", "mmfe_run_noalloc", "mmfe_run_slices", "mmfe_run_ragged", "mmfe_run_slices_ragged", "mmfe_feature_sums",
     "mmfe_plan_kernel",
     "mmfe_patch_embed_create", "mmfe_patch_embed_destroy", "mmfe_patch_embed_shape", "mmfe_patch_embed_run", "mmfe_patch_embed_update",
+    "mmfe_rotary_create", "mmfe_rotary_destroy", "mmfe_rotary_run",
+    "mmfe_grad_partials", "mmfe_grad_clip",
 )
 
 
@@ -67,6 +72,15 @@ class MmfeSpec(ctypes.Structure):
         ("out_dtype", ctypes.c_int32),
         ("in_dtype", ctypes.c_int32),
     ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """mmfe_rotary_args"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_size", "dtype", "pos_64", "inverse", "heads_q", "heads_k", "dim", "reserved")] + [
+        ("n_batch", ctypes.c_int64), ("n_tokens", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3), ("q_out_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("k_out_stride", ctypes.c_int64 * 3),
+        ("positions", ctypes.c_void_p), ("pos_stride", ctypes.c_int64 * 3)]
 
 
 def library_path() -> str:
@@ -128,6 +142,16 @@ def bind_library(path: str):
     lib.mmfe_patch_embed_update.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     lib.mmfe_patch_embed_run.restype = ctypes.c_int
     lib.mmfe_patch_embed_run.argtypes = [ctypes.c_void_p, c_f_p, c_i64, c_i64, c_f_p, c_i64, ctypes.c_void_p]
+    lib.mmfe_rotary_create.restype = ctypes.c_int
+    lib.mmfe_rotary_create.argtypes = [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_double, ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)]
+    lib.mmfe_rotary_destroy.restype = ctypes.c_int
+    lib.mmfe_rotary_destroy.argtypes = [ctypes.c_void_p]
+    lib.mmfe_rotary_run.restype = ctypes.c_int
+    lib.mmfe_rotary_run.argtypes = [ctypes.c_void_p, ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
+    lib.mmfe_grad_partials.restype = c_i64
+    lib.mmfe_grad_partials.argtypes = [c_i64]
+    lib.mmfe_grad_clip.restype = ctypes.c_int
+    lib.mmfe_grad_clip.argtypes = [c_i64] + [ctypes.c_void_p] * 5 + [ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     if lib.mmfe_abi_version() != ABI_VERSION:
         raise MmfeError(f"{path} has ABI version {lib.mmfe_abi_version()}, the Python side expects {ABI_VERSION}")
     return lib
@@ -294,3 +318,41 @@ class PatchEmbedHandle:
             self.close()
         except Exception:
             pass
+
+
+class RotaryHandle:
+    """Owns one mmfe_rotary (the frequency table of Rotary on one device)."""
+
+    def __init__(self, sections: Sequence[int], ladder: int, pairing: int, base: float, device: int):
+        self._lib = load_library()
+        self._handle = None
+        handle = ctypes.c_void_p()
+        s = (ctypes.c_int32 * len(sections))(*sections)
+        check(self._lib.mmfe_rotary_create(len(sections), s, ladder, pairing, float(base), int(device), ctypes.byref(handle)), "mmfe_rotary_create")
+        self._handle = handle
+
+    def run(self, args: RotaryArgs, stream: int) -> None:
+        check(self._lib.mmfe_rotary_run(self._handle, ctypes.byref(args), stream or None), "mmfe_rotary_run")
+
+    def close(self) -> None:
+        if getattr(self, "_handle", None):
+            self._lib.mmfe_rotary_destroy(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def grad_partials(n: int) -> int:
+    return int(load_library().mmfe_grad_partials(n))
+
+
+def grad_clip(ptrs, numels, dtypes, out_ptrs, out_dtypes, kind: int, max_norm: float, partials_ptr: int, norm_ptr: int, device: int, stream: int = 0) -> None:
+    n = len(ptrs)
+    check(load_library().mmfe_grad_clip(n, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*numels), (ctypes.c_int32 * n)(*dtypes),
+                                        None if out_ptrs is None else (ctypes.c_void_p * n)(*out_ptrs),
+                                        None if out_ptrs is None else (ctypes.c_int32 * n)(*out_dtypes),
+                                        kind, max_norm, partials_ptr, norm_ptr, device, stream or None), "mmfe_grad_clip")

@@ -220,6 +220,23 @@ __device__ __forceinline__ unsigned pack2_bits(float a, float b, int out_dtype) 
     return (unsigned)f16_bits(a) | (unsigned)f16_bits(b) << 16;
 }
 
+// Makes `device` current for the life of the object; rc says whether that worked (the message is set).
+struct OnDevice {
+    int prev = -1, rc = MMFE_OK;
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&prev) != hipSuccess || (prev != device && hipSetDevice(device) != hipSuccess)) {
+            set_error("cannot make device %d current", device);
+            rc = MMFE_EHIP;
+            prev = -1;
+        } else if (prev == device) prev = -1;
+    }
+    ~OnDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
 // Launch-geometry helpers (thread-safe, cached per kernel and device).
 //   kernel_prepare: raises the kernel's dynamic-LDS limit to the CU's 160 KB on the current device (once) and
 //   returns how many blocks of `threads` threads with `lds` bytes of dynamic LDS are resident per CU, and the CU count.
