@@ -302,6 +302,51 @@ int mmfe_rotary_destroy(mmfe_rotary* handle);
 /* One launch for q and k; either may have no heads.  Asynchronous on hip_stream, allocates nothing. */
 int mmfe_rotary_run(const mmfe_rotary* handle, const mmfe_rotary_args* args, void* hip_stream);
 
+/* ---- attention over the encoders' tokens ------------------------------------------------------------------------------------
+ * The product the encoders spend their time in (Attention.forward, classification/vggsound/models/vit_model.py:43-69, computed there as
+ * two matrix products around a softmax over a materialised score tensor), over documents of different lengths:
+ *     s = scale q k^T;   cap > 0: s = cap tanh(s / cap);   slopes: s -= slopes[head] |i + (len_k - len_q) - j|
+ *     out = softmax(s) v over the keys j of row i's document with  not causal, or j <= i + len_k - len_q, or j < prefix[document]
+ * Rows that see no key, and rows no document holds, give zeros (lse -inf).  Key head of query head h: h / (heads / kv_heads).
+ *   packed = 0   n_docs batch entries of q_rows x k_rows; q_len / k_len (device, n_docs entries, clamped to [0, rows]) or NULL = all
+ *   packed = 1   document d holds rows q_off[d] .. q_off[d + 1] - 1 of q_rows and keys k_off[d] .. of k_rows (device, n_docs + 1
+ *                nondecreasing entries each, clamped to the rows); batch strides are ignored and must be 0
+ * float16 / bfloat16, head size a multiple of 8 up to 128; strides in elements, multiples of 8, unit stride inside the heads,
+ * 16-byte aligned.  Scores, softmax and sums are float32; the softmax's values are rounded to the 16-bit type for the product with v.
+ * Values of rows outside a document never enter it; inside one, a NaN or infinity of a key that a causal mask hides may reach rows
+ * up to 63 before it.  Asynchronous on hip_stream, allocates nothing. */
+typedef struct mmfe_attention_args {
+    int32_t struct_size;      /* = sizeof(mmfe_attention_args) */
+    int32_t dtype;            /* MMFE_OUT_F16 / MMFE_OUT_BF16, of every 16-bit tensor */
+    int32_t n_docs, heads, kv_heads, dim;
+    int32_t packed, causal;
+    float   scale, cap;
+    int64_t q_rows, k_rows;
+    const void *q, *k, *v;
+    const int32_t *q_len, *k_len, *q_off, *k_off;
+    const int32_t* prefix;    /* n_docs entries or NULL; needs causal */
+    const float* slopes;      /* heads entries or NULL */
+    void* out;
+    float* lse;               /* (n_docs,) heads, q_rows by lse_stride; NULL: not wanted (backward needs it) */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* batch, row, head */
+    int64_t lse_stride[2];    /* batch, head; rows are contiguous */
+} mmfe_attention_args;
+int mmfe_attention_forward(const mmfe_attention_args* args, int device, void* hip_stream);
+
+/* Gradients of q, k and v from the forward call's arguments (with its out and lse) and the gradient of out.  Those of a shared key
+ * head are summed over its query heads; rows outside the documents get zeros.  Sums have a fixed order: the same call gives the
+ * same bits.  lse must be the dense (n_docs,) heads, q_rows array of the forward call. */
+typedef struct mmfe_attention_grads {
+    int32_t struct_size;      /* = sizeof(mmfe_attention_grads) */
+    int32_t reserved;
+    const void* grad_out;
+    void *grad_q, *grad_k, *grad_v;
+    int64_t grad_out_stride[3], grad_q_stride[3], grad_k_stride[3], grad_v_stride[3];
+    float* scratch;           /* device, 2 x the size of lse, the call's own until it has run */
+    uint32_t* norms;          /* device, 2 x n_docs x kv_heads, ZEROED by the caller; float16 only (NULL otherwise) */
+} mmfe_attention_grads;
+int mmfe_attention_backward(const mmfe_attention_args* args, const mmfe_attention_grads* grads, int device, void* hip_stream);
+
 /* ---- global norm of many tensors, and clipping by it ------------------------------------------------------------------
  * What a training step of the encoders does between backward and the optimizer (the reference's loops call the optimizer directly,
  * classification/vggsound/vanilla_single.py:75-80).  norm = (sum of all squares)^(1/2) (MMFE_NORM_2) or the largest magnitude

@@ -11,13 +11,14 @@ the Python call signatures of lixinghe1999/multi_modal's dataset classes.
     resample.load_resampled          the resampling of librosa.load(sr=16000)     (vggsound.py:114; extract_audio.py:6-13)
     patch_embed.PatchEmbed           PatchEmbed.forward with the audio projection (models/vit_model.py:193-199, 435)
     rotary.Rotary                    rotary positions with several axes for the tokens' query and key heads
+    attention.attention              the encoders' attention (models/vit_model.py:43-69) over padded or packed documents, forward and backward
     gradients.clip_grad_norm         global gradient norm and clipping between backward and the optimizer
     loader.DevicePrefetcher          `batch[k].to(device)` of the training loop, overlapped    (vanilla_multi.py:76-77, 89-92)
     partition.*                      batch sharding over the GPUs of a node + all-gather of features
 
 All arithmetic runs in libmmfe.so (hand-written HIP for gfx950, C ABI in include/mmfe.h).
 """
-from . import _native, epic, gradients, har, kaldi, loader, logmel, melbank, partition, patch_embed, resample, rotary, stats, transforms, vggsound  # noqa: F401
+from . import _native, attention, epic, gradients, har, kaldi, loader, logmel, melbank, partition, patch_embed, resample, rotary, stats, transforms, vggsound  # noqa: F401
 from ._native import MmfeError, library_path, load_library  # noqa: F401
 from .epic import log_specgram, log_specgram_batch, spec_to_tensor  # noqa: F401
 from .gradients import clip_grad_norm, grad_norm  # noqa: F401

@@ -36,6 +36,7 @@ EXPORTED_SYMBOLS = (
     "mmfe_plan_kernel",
     "mmfe_patch_embed_create", "mmfe_patch_embed_destroy", "mmfe_patch_embed_shape", "mmfe_patch_embed_run", "mmfe_patch_embed_update",
     "mmfe_rotary_create", "mmfe_rotary_destroy", "mmfe_rotary_run",
+    "mmfe_attention_forward", "mmfe_attention_backward",
     "mmfe_grad_partials", "mmfe_grad_clip",
 )
 
@@ -81,6 +82,21 @@ class RotaryArgs(ctypes.Structure):
         ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("k", ctypes.c_void_p), ("k_out", ctypes.c_void_p),
         ("q_stride", ctypes.c_int64 * 3), ("q_out_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("k_out_stride", ctypes.c_int64 * 3),
         ("positions", ctypes.c_void_p), ("pos_stride", ctypes.c_int64 * 3)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """mmfe_attention_args"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_size", "dtype", "n_docs", "heads", "kv_heads", "dim", "packed", "causal")] + [
+        ("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_rows", ctypes.c_int64), ("k_rows", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "out", "lse")] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("lse_stride", ctypes.c_int64 * 2)]
+
+
+class AttentionGrads(ctypes.Structure):
+    """mmfe_attention_grads"""
+    _fields_ = [("struct_size", ctypes.c_int32), ("reserved", ctypes.c_int32)] + [(n, ctypes.c_void_p) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + [
+        (n, ctypes.c_int64 * 3) for n in ("grad_out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride")] + [
+        ("scratch", ctypes.c_void_p), ("norms", ctypes.c_void_p)]
 
 
 def library_path() -> str:
@@ -148,6 +164,10 @@ def bind_library(path: str):
     lib.mmfe_rotary_destroy.argtypes = [ctypes.c_void_p]
     lib.mmfe_rotary_run.restype = ctypes.c_int
     lib.mmfe_rotary_run.argtypes = [ctypes.c_void_p, ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
+    lib.mmfe_attention_forward.restype = ctypes.c_int
+    lib.mmfe_attention_forward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_backward.restype = ctypes.c_int
+    lib.mmfe_attention_backward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionGrads), ctypes.c_int, ctypes.c_void_p]
     lib.mmfe_grad_partials.restype = c_i64
     lib.mmfe_grad_partials.argtypes = [c_i64]
     lib.mmfe_grad_clip.restype = ctypes.c_int
@@ -344,6 +364,14 @@ class RotaryHandle:
             self.close()
         except Exception:
             pass
+
+
+def attention_forward(args: AttentionArgs, device: int, stream: int) -> None:
+    check(load_library().mmfe_attention_forward(ctypes.byref(args), device, stream or None), "mmfe_attention_forward")
+
+
+def attention_backward(args: AttentionArgs, grads: AttentionGrads, device: int, stream: int) -> None:
+    check(load_library().mmfe_attention_backward(ctypes.byref(args), ctypes.byref(grads), device, stream or None), "mmfe_attention_backward")
 
 
 def grad_partials(n: int) -> int:

@@ -1,0 +1,194 @@
+"""Attention over the encoders' tokens on the device, forward and backward (csrc/attention.hip, csrc/attention_backward.hip).
+
+Stands where the encoders' Attention.forward (classification/vggsound/models/vit_model.py:43-69) forms its score tensor, takes a softmax
+and multiplies by the values, and adds what batches of clips need next to it: documents of different lengths (padded or packed),
+causal and prefix masks, capped scores, a bias that falls with distance, key heads shared by query heads, and one or a few new tokens over
+what a stream has kept.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _native as N
+from .plans import OUT_CODES, require_gpu
+
+_ARGS_SIZE = ctypes.sizeof(N.AttentionArgs)
+_GRADS_SIZE = ctypes.sizeof(N.AttentionGrads)
+_DTYPES = (torch.float16, torch.bfloat16)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t itself when the kernels can read it where it is (unit stride inside the heads, 16-byte pieces), else a packed copy."""
+    s = t.stride()
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and all(v % 8 == 0 for v, m in zip(s[:-1], t.shape) if m > 1) and s[-3] <= 1 << 24:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
+    """(batch, row, head) strides, 0 where there is one entry."""
+    s = tuple(v if m > 1 else 0 for v, m in zip(t.stride()[:-1], t.shape))
+    return s if len(s) == 3 else (0,) + s
+
+
+def _counts(x, name: str, n: int, device, limit: Optional[int] = None, rising: bool = False) -> Optional[torch.Tensor]:
+    """Per-document integers as the int32 device tensor the kernels read; what the host holds is checked, what the device holds is
+    clamped by the kernels."""
+    if x is None:
+        return None
+    t = torch.as_tensor(x)
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError(f"{name} must be integers")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must hold {n} entries, got {tuple(t.shape)}")
+    if not t.is_cuda and n > 0:
+        if int(t.min()) < 0 or (limit is not None and int(t.max()) > limit):
+            raise ValueError(f"{name} must lie in [0, {limit}]")
+        if rising and bool((t[1:] < t[:-1]).any()):
+            raise ValueError(f"{name} must not fall")
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        t = t.to(device=device, dtype=torch.int32).contiguous()
+    return t
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+class _Call:
+    """One checked call: what does not depend on the outputs."""
+
+    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes")
+
+    def args(self, q, k, v, out, lse) -> N.AttentionArgs:
+        return N.AttentionArgs(
+            _ARGS_SIZE, OUT_CODES[q.dtype], self.n_docs, q.shape[-2], k.shape[-2], q.shape[-1], self.packed, self.causal, self.scale, self.cap,
+            q.shape[-3], k.shape[-3], q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(self.q_len), _ptr(self.k_len), _ptr(self.q_off), _ptr(self.k_off),
+            _ptr(self.prefix), _ptr(self.slopes), out.data_ptr(), _ptr(lse), _strides(q), _strides(k), _strides(v), _strides(out),
+            (0, 0) if lse is None else (lse.stride(0), lse.stride(1)) if lse.dim() == 3 else (0, lse.stride(0)))
+
+    def forward(self, q, k, v, want_lse: bool):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = None
+        if want_lse:
+            shape = (q.shape[-2], q.shape[-3])
+            lse = torch.empty(shape if self.packed else (q.shape[0],) + shape, dtype=torch.float32, device=q.device)
+        N.attention_forward(self.args(q, k, v, out, lse), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        return out, lse
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, call):
+        out, lse = call.forward(q, k, v, True)
+        ctx.call = call
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, grad_out, _):
+        q, k, v, out, lse = ctx.saved_tensors
+        call = ctx.call
+        g = _rows(grad_out)
+        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        scratch = torch.empty((2,) + tuple(lse.shape), dtype=torch.float32, device=q.device)
+        norms = torch.zeros(2 * call.n_docs * k.shape[-2], dtype=torch.int32, device=q.device) if q.dtype == torch.float16 else None
+        grads = N.AttentionGrads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _strides(g), _strides(gq), _strides(gk),
+                                 _strides(gv), scratch.data_ptr(), _ptr(norms))
+        N.attention_backward(call.args(q, k, v, out, lse), grads, q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        need = ctx.needs_input_grad
+        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None, kv_lengths=None, offsets=None, kv_offsets=None, causal: bool = False,
+              prefix=None, slopes=None, cap: float = 0.0, scale: Optional[float] = None,
+              return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """softmax(scores) v over the tokens of each document; float16 or bfloat16, differentiable in q, k and v.
+
+    Padded: q (B, N, H, D), k and v (B, S, K, D), a document per batch entry; `lengths` (B,) valid rows of q (default: all),
+    `kv_lengths` (B,) valid rows of k and v (default: `lengths` when S == N, else all).  K divides H: query head h reads key head
+    h // (H // K).  D: a multiple of 8 up to 128.  Any strides (views of a packed projection are read where they are).
+    Packed: q (T, H, D), k and v (S, K, D) with `offsets` (documents + 1,): document d holds rows offsets[d] .. offsets[d + 1] - 1, and
+    of the keys those that `kv_offsets` (default: `offsets`) cuts out.
+
+    Scores are scale * q . k (default scale: D ** -0.5); cap > 0 makes them cap * tanh(score / cap); `slopes` (H,) subtracts
+    slopes[h] * |distance| (row i stands at key position i + len_k - len_q: the last row meets the last key).  causal=True hides the keys
+    behind a row's position, except the first `prefix[d]` keys of a document when `prefix` (one per document) is given.
+    Rows that see no key, and rows no document holds, give zeros, no gradients, and lse = -inf.
+
+    `lengths`, `offsets` and `prefix` may be integer tensors on the GPU (not read back; entries out of range are clamped) or on the
+    host (checked).  return_lse=True also returns the float32 log-sum-exp of each row's scores, (B, H, N) or (H, T), without gradient.
+    Tensors on the CPU are copied over and the result is copied back."""
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"attention takes float16 or bfloat16 tensors of one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    packed = offsets is not None
+    dims = 3 if packed else 4
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+        raise ValueError("attention takes (batch, tokens, heads, head size) tensors, or (tokens, heads, head size) with offsets")
+    if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    H, D, K = q.shape[-2], q.shape[-1], k.shape[-2]
+    if K < 1 or H < 1 or H % K != 0:
+        raise ValueError(f"{H} query heads cannot share {K} key heads")
+    if D < 8 or D > 128 or D % 8 != 0:
+        raise ValueError(f"head size {D}: a multiple of 8 up to 128")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must be on one device")
+    call = _Call()
+    call.cap = float(cap)
+    call.scale = D ** -0.5 if scale is None else float(scale)
+    if not (0.0 <= call.cap < math.inf) or not (0.0 < call.scale < math.inf):
+        raise ValueError("cap must be >= 0 and scale > 0, both finite")
+    if prefix is not None and not causal:
+        raise ValueError("prefix belongs to causal=True")
+    if packed and (lengths is not None or kv_lengths is not None):
+        raise ValueError("lengths belong to the padded form: documents that are packed have offsets")
+    if not packed and kv_offsets is not None:
+        raise ValueError("kv_offsets needs offsets")
+    n, s = q.shape[-3], k.shape[-3]
+    if packed:
+        m = len(offsets) - 1
+        if m < 0:
+            raise ValueError("offsets holds at least one entry")
+        if kv_offsets is None and s != n:
+            raise ValueError(f"{n} rows and {s} keys: kv_offsets says how the keys are cut")
+    else:
+        m = q.shape[0]
+        if kv_lengths is None and s == n:
+            kv_lengths = lengths
+    require_gpu()
+    origin = q.device
+    if not q.is_cuda:
+        q, k, v = q.cuda(), k.cuda(), v.cuda()
+    device = q.device
+    call.packed, call.causal, call.n_docs = packed, bool(causal), m
+    call.q_len = call.k_len = call.q_off = call.k_off = None
+    if packed:
+        call.q_off = _counts(offsets, "offsets", m + 1, device, n, rising=True)
+        call.k_off = call.q_off if kv_offsets is None else _counts(kv_offsets, "kv_offsets", m + 1, device, s, rising=True)
+    else:
+        call.q_len = _counts(lengths, "lengths", m, device, n)
+        call.k_len = call.q_len if kv_lengths is lengths else _counts(kv_lengths, "kv_lengths", m, device, s)
+    call.prefix = _counts(prefix, "prefix", m, device)
+    call.slopes = None
+    if slopes is not None:
+        t = torch.as_tensor(slopes)
+        if tuple(t.shape) != (H,):
+            raise ValueError(f"slopes must hold one entry per query head ({H}), got {tuple(t.shape)}")
+        if t.requires_grad:
+            raise ValueError("slopes have no gradient: detach them")
+        call.slopes = t.to(device=device, dtype=torch.float32).contiguous()
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _AttentionFn.apply(q, k, v, call)
+    else:
+        out, lse = call.forward(q, k, v, return_lse)
+    if origin.type != "cuda":
+        out, lse = out.to(origin), None if lse is None else lse.to(origin)
+    return (out, lse) if return_lse else out

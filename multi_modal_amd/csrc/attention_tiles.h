@@ -1,0 +1,271 @@
+// Shared device code of the attention kernels (attention.hip, attention_backward.hip): which rows a block works on, how tiles get
+// into LDS, and how matrix operands are read out of them.
+//
+// All products use v_mfma_f32_32x32x16 (32 x 32 results, 16 terms per instruction, float32 accumulation).  A lane (c = lane & 31,
+// h = lane >> 5) holds of the operands 8 consecutive terms k = 8 h .. 8 h + 7 of row (column) c, and of the result column c,
+// rows 8 (i / 4) + 4 h + i % 4 in register i = 0 .. 15.  Products are arranged so that a result is the next product's operand as it
+// stands: the result's registers 8 s .. 8 s + 7 hold rows {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} of its 16-row step s, and since the order of
+// terms is free as long as both operands agree, the partner operand is fetched in that order (two transposing reads of 4 rows each).
+//
+// Tiles of rows lie in LDS as they lie in memory, in 16-byte pieces, piece c of row r at position c ^ swizzle(r): the reads of 16
+// rows' pieces of one column, and the transposing reads of 4 rows x 32 bytes, then spread over all banks.  They arrive by LDS-DMA
+// (global_load_lds_dwordx4: 64 pieces per instruction to consecutive LDS addresses, each lane naming its source), so that no
+// register or vector instruction is spent on staging; the swizzle is applied to the source addresses.
+#pragma once
+
+#include "mmfe_internal.h"
+
+namespace mmfe {
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kRows = 128;            // rows of a block: 32 per wave
+constexpr int kTile = 64;             // rows of a streamed tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A tensor of (batch, row, head) vectors with unit stride inside; strides in elements, batch = 0 where documents are packed.
+struct Rows {
+    const void* p;
+    int64_t b, n, h;
+};
+
+// What forward and backward share.  Documents: batch entries of the padded form (q_len / k_len valid rows of q_rows / k_rows), or the
+// row ranges that offsets cut the packed rows into.
+struct Problem {
+    Rows q, k, v;
+    const int32_t *q_len, *k_len;     // padded: per document, or NULL = all rows
+    const int32_t *q_off, *k_off;     // packed: n_docs + 1 entries
+    const int32_t* prefix;            // per document, or NULL
+    const float* slopes;              // per query head, or NULL
+    int64_t q_rows, k_rows;           // per document (padded) or in all (packed)
+    int n_docs, heads, kv_heads, group, dim;
+    int packed, causal;
+    float scale, cap;
+    int tiles;                        // padded: row tiles per document; packed: tiles in all (an upper bound)
+};
+
+// One document's rows, and which of them a block has.
+struct Doc {
+    int64_t q0, k0;                   // first row (packed: in all rows; padded: 0, with batch set)
+    int batch;                        // batch entry (padded), 0 when packed
+    int index;                        // document, or -1: rows that belong to none
+    int nq, nk;                       // valid rows
+    int rows;                         // rows to produce, from the tiled side (padded: all of them, whatever their length)
+    int tile;                         // tile inside the document
+    int prefix;
+};
+
+__device__ __forceinline__ int clamp_int(int64_t v, int64_t lo, int64_t hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Document and tile of tile number t, on the query side (QSIDE) or the key side.  False: there is no such tile.
+// Packed rows that no document holds (before the first offset, behind the last) form tiles of their own, of a document without
+// partners: their results are zeros.  Offsets are clamped into the rows, so that no entry can lead out of the tensors.
+template <bool QSIDE>
+__device__ __forceinline__ bool find_doc(const Problem& p, int t, int tile_rows, Doc& d) {
+    if (!p.packed) {
+        const int b = t / p.tiles;
+        d.batch = d.index = b;
+        d.tile = t - b * p.tiles;
+        d.q0 = d.k0 = 0;
+        d.nq = p.q_len ? clamp_int(uniform(p.q_len[b]), 0, p.q_rows) : (int)p.q_rows;
+        d.nk = p.k_len ? clamp_int(uniform(p.k_len[b]), 0, p.k_rows) : (int)p.k_rows;
+        d.rows = QSIDE ? (int)p.q_rows : (int)p.k_rows;
+        d.prefix = p.prefix ? uniform(p.prefix[b]) : 0;
+        return true;
+    }
+    const int32_t* off = QSIDE ? p.q_off : p.k_off;
+    const int64_t all = QSIDE ? p.q_rows : p.k_rows;
+    const int lane = threadIdx.x & 63;
+    d.batch = 0;
+    d.index = -1;
+    d.nq = d.nk = 0;
+    d.q0 = d.k0 = 0;
+    d.prefix = 0;
+    const int first = clamp_int(uniform(off[0]), 0, all);
+    const int lead = (first + tile_rows - 1) / tile_rows;
+    if (t < lead) {
+        d.tile = t;
+        d.rows = first;
+        return true;
+    }
+    t -= lead;
+    int last = first;
+    for (int base = 0; base < p.n_docs; base += 64) {
+        const int i = base + lane;
+        int s = 0, e = 0;
+        if (i < p.n_docs) {
+            s = clamp_int(off[i], 0, all);
+            e = clamp_int(off[i + 1], s, all);
+        }
+        int sum = (e - s + tile_rows - 1) / tile_rows;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o);
+            if (lane >= o) sum += up;
+        }
+        const int total = uniform(__shfl(sum, 63));
+        if (t < total) {
+            const int w = uniform(__ffsll((unsigned long long)__ballot(sum > t)) - 1);
+            const int before = w ? uniform(__shfl(sum, w - 1)) : 0;
+            const int ds = uniform(__shfl(s, w)), de = uniform(__shfl(e, w));
+            d.index = base + w;
+            d.tile = t - before;
+            d.rows = de - ds;
+            const int32_t* other = QSIDE ? p.k_off : p.q_off;
+            const int64_t other_all = QSIDE ? p.k_rows : p.q_rows;
+            const int os = clamp_int(uniform(other[d.index]), 0, other_all);
+            const int oe = clamp_int(uniform(other[d.index + 1]), os, other_all);
+            if (QSIDE) { d.q0 = ds; d.nq = de - ds; d.k0 = os; d.nk = oe - os; }
+            else { d.k0 = ds; d.nk = de - ds; d.q0 = os; d.nq = oe - os; }
+            if (p.prefix) d.prefix = uniform(p.prefix[d.index]);
+            return true;
+        }
+        t -= total;
+        const int n = p.n_docs - base < 64 ? p.n_docs - base : 64;
+        last = uniform(__shfl(e, n - 1));
+    }
+    const int rest = (int)all - last;
+    if (rest <= 0 || t >= (rest + tile_rows - 1) / tile_rows) return false;
+    d.tile = t;
+    d.rows = rest;
+    if (QSIDE) d.q0 = last;
+    else d.k0 = last;
+    return true;
+}
+
+__device__ __forceinline__ const char* row_base(const Rows& r, const Doc& d, int64_t row0, int head) {
+    return static_cast<const char*>(r.p) + 2 * (d.batch * r.b + row0 * r.n + head * r.h);
+}
+
+// ---- LDS tiles ----
+
+template <int DP>
+__device__ __forceinline__ constexpr int swizzle(int row) {
+    if constexpr (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);        // 16 pieces a row
+    else if constexpr (DP == 64) return (row & 7) ^ ((row >> 3) & 1);           // 8
+    else return (row >> 2) & 3;                                                 // 4
+}
+
+// 16 bytes per lane: from base + voff to LDS byte lds_dst + 16 * lane.  M0 holds the destination for the instruction; it is the
+// compiler's register, so it is saved and restored.  The compiler does not count these; their completion is waited for by hand.
+__device__ __forceinline__ void dma16(const void* base, unsigned voff, unsigned lds_dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(base), "s"(lds_dst) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* base, unsigned voff, unsigned lds_dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(base), "s"(lds_dst) : "memory");
+}
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// Tile of ROWS rows brought in by WAVES waves.  Rows past the last valid one repeat it and pieces past the head size repeat the
+// first: their products are masked, dropped or multiplied by zeros, and they hold no other document's (or no one's) values.
+template <int DP, int ROWS, int WAVES>
+struct Loader {
+    static constexpr int kPieces = DP / 8;
+    static constexpr int kCount = ROWS * kPieces / 64 / WAVES;      // DMA instructions of a wave
+    static_assert(kCount * 64 * WAVES == ROWS * kPieces, "whole instructions");
+    unsigned off[kCount];                                           // byte offsets from the tile's first row
+    __device__ __forceinline__ static int piece(int i, int wave) { return (i * WAVES + wave) * 64 + (int)(threadIdx.x & 63); }
+    __device__ __forceinline__ static unsigned offset(int ci, int rows, int dim, unsigned stride) {
+        const int r0 = ci / kPieces;
+        const int c = (ci & (kPieces - 1)) ^ swizzle<DP>(r0);
+        const int r = r0 < rows ? r0 : rows - 1;
+        return (unsigned)r * stride + (c * 8 < dim ? c * 16 : 0);
+    }
+    __device__ __forceinline__ void init(int dim, int64_t stride, int wave) {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) off[i] = offset(piece(i, wave), ROWS, dim, (unsigned)(2 * stride));
+    }
+    // base: the tile's first row; rows >= 1: valid rows from there on
+    __device__ __forceinline__ void load(const char* base, int rows, int dim, int64_t stride, unsigned lds, int wave) const {
+        if (rows >= ROWS) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) dma16(base, off[i], lds + (i * WAVES + wave) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) dma16(base, offset(piece(i, wave), rows, dim, (unsigned)(2 * stride)), lds + (i * WAVES + wave) * 1024);
+        }
+    }
+};
+
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void block_sync() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Operand with one row per lane (row0 + c), step s of 16 columns.
+template <int DP>
+__device__ __forceinline__ u32x4 read_rows(const char* tile, int row0, int s) {
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    return *reinterpret_cast<const u32x4*>(tile + (row0 + r) * (2 * DP) + (((2 * s + h) ^ swizzle<DP>(r)) << 4));
+}
+
+// Transposed operand: lane c gets column col0 + c of the rows row0 + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} (row0 a multiple of 16).  A
+// transposing read serves 16 lanes: lane i names 8 bytes (4 columns) of row i / 4 and receives column i of the 4 rows.
+template <int DP>
+__device__ __forceinline__ u32x4 read_cols(const char* tile, int row0, int col0) {
+    const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
+    const int c = (col0 >> 3) + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+    const int r = 4 * h + (i >> 2);
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    const char* a = tile + (row0 + r) * (2 * DP) + ((c ^ swizzle<DP>(r)) << 4) + 8 * (i & 1);
+    const char* b = tile + (row0 + r + 8) * (2 * DP) + ((c ^ swizzle<DP>(r + 8)) << 4) + 8 * (i & 1);
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)a));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)b));
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// two float32 to one word of 16-bit values, round to nearest even
+template <bool BF>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (BF) return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+    else return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+// result registers 8 s .. 8 s + 7 as an operand
+template <bool BF>
+__device__ __forceinline__ u32x4 operand(const f32x16& v, int s) {
+    return u32x4{pack2<BF>(v[8 * s], v[8 * s + 1]), pack2<BF>(v[8 * s + 2], v[8 * s + 3]), pack2<BF>(v[8 * s + 4], v[8 * s + 5]), pack2<BF>(v[8 * s + 6], v[8 * s + 7])};
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// tanh(z) from one exponential: 1 - 2 / (e^(2 z) + 1); absolute error a few 2^-24, exact limits
+__device__ __forceinline__ float tanh_fast(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_fast(2.f * kLog2e * z) + 1.f); }
+
+// Row i of the result registers (see above).
+__device__ __forceinline__ constexpr int reg_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+__device__ __forceinline__ int head_of(const Problem& p, int j) {
+    // neighbouring block numbers go to different XCDs: number the heads so that block j and j + 8 share key heads where they can
+    return (j % p.kv_heads) * p.group + j / p.kv_heads;
+}
+
+}  // namespace attn
+}  // namespace mmfe

@@ -1,0 +1,314 @@
+"""Attention (csrc/attention.hip, csrc/attention_backward.hip) against the float64 oracle (oracle/token_oracle.py), which gives a bound
+for each element: half a step of the 16-bit type for the result, half a step for each rounded softmax value or score gradient that
+enters it, and the float32 errors of the scores, taken through the formulas."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mm():
+    import multi_modal_amd as m
+    m.load_library()
+    assert torch.cuda.is_available()
+    return m
+
+
+@pytest.fixture(scope="module")
+def O():
+    from oracle import token_oracle
+    return token_oracle
+
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def limits(dtype):
+    i = torch.finfo(dtype)
+    return dict(eps=i.eps, tiny=i.smallest_normal * i.eps / 2)
+
+
+def within(name, got, ref, tol):
+    got = got.detach().double()
+    bad = ~((got - ref).abs() <= tol) & ~((got == ref))
+    assert not bad.any(), (name, int(bad.sum()), float(((got - ref).abs() / tol.clamp_min(1e-300))[bad].max()), bad.nonzero()[:4].tolist())
+
+
+def slopes_of(H):
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)])
+
+
+def docs_padded(lens, kv, N, S):
+    return [(b * N, n, b * S, m) for b, (n, m) in enumerate(zip(lens, kv))]
+
+
+def check(mm, O, q, k, v, docs, opts, g=None, scale=None, flat=lambda t: t, lse_flat=lambda t: t, host=None):
+    """q, k, v (any form) on the GPU; `flat` brings a result to (rows, heads, dim), `lse_flat` a lse to (heads, rows)."""
+    host = host or {}
+    fn = mm.attention.attention
+    ref, tol = O.attention(flat(q.detach()), flat(k.detach()), flat(v.detach()), docs, scale=scale, cap=opts.get("cap", 0.0), slopes=host.get("slopes"),
+                           causal=opts.get("causal", False), prefix=host.get("prefix"), g=None if g is None else flat(g), **limits(q.dtype))
+    with torch.no_grad():
+        out, lse = fn(q, k, v, scale=scale, return_lse=True, **opts)
+    assert out.dtype == q.dtype and out.shape == q.shape and lse.dtype == torch.float32
+    within("out", flat(out), ref["o"], tol["o"])
+    within("lse", lse_flat(lse), ref["lse"], tol["lse"])
+    if g is None:
+        return out
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    o2 = fn(q, k, v, scale=scale, **opts)
+    assert torch.equal(o2, out)
+    dq, dk, dv = torch.autograd.grad(o2, [q, k, v], g)
+    for name, got in (("dq", dq), ("dk", dk), ("dv", dv)):
+        assert got.dtype == q.dtype and got.shape == (q if name == "dq" else k).shape
+        within(name, flat(got), ref[name], tol[name])
+    again = torch.autograd.grad(fn(q, k, v, scale=scale, **opts), [q, k, v], g)
+    assert all(torch.equal(a, b) for a, b in zip(again, (dq, dk, dv)))          # no atomics on values: the same bits
+    return out
+
+
+def flat4(t):
+    return t.reshape(-1, *t.shape[2:])
+
+
+def lse4(t):
+    return t.transpose(0, 1).reshape(t.shape[1], -1)
+
+
+PADDED = [
+    # lens, N, kv, S, H, K, D, dtype, causal, prefix, bias, cap
+    ([1], 1, [1], 1, 1, 1, 8, HF, False, False, False, 0.0),
+    ([257], 257, [257], 257, 3, 3, 64, HF, False, False, False, 0.0),
+    ([193, 1, 0, 64, 65, 192], 193, None, 193, 4, 2, 64, BF, False, False, False, 0.0),
+    ([128, 127, 129], 129, None, 129, 2, 1, 128, HF, True, False, False, 0.0),
+    ([300, 31], 300, None, 300, 6, 2, 72, BF, True, True, True, 0.0),
+    ([150, 90], 150, None, 150, 2, 2, 32, HF, False, False, True, 8.0),
+    ([260], 260, None, 260, 2, 2, 128, BF, True, True, False, 5.0),
+    ([33, 64, 10], 64, [200, 10, 0], 201, 4, 2, 64, BF, True, False, False, 0.0),    # more rows than keys: rows that see nothing
+    ([5, 40], 40, [500, 333], 512, 3, 1, 96, HF, False, False, True, 0.0),           # cross attention
+    ([70, 70], 70, [70, 3], 70, 2, 2, 16, HF, True, True, False, 0.0),
+    ([600], 600, None, 600, 1, 1, 40, HF, True, False, True, 30.0),
+    ([0, 0], 5, [3, 0], 9, 2, 2, 64, BF, False, False, False, 0.0),
+]
+
+
+@pytest.mark.parametrize("case", PADDED, ids=lambda c: f"{c[0]}x{c[4]}x{c[6]}")
+def test_padded(mm, O, case):
+    lens, N, kv, S, H, K, D, dtype, causal, prefix, bias, cap = case
+    B = len(lens)
+    gen = torch.Generator().manual_seed(N * 7 + D)
+    q = torch.randn(B, N, H, D, generator=gen).to(dtype).cuda()
+    k, v = (torch.randn(B, S, K, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    g = torch.randn(B, N, H, D, generator=gen).to(dtype).cuda()
+    host = {}
+    opts = dict(causal=causal, cap=cap, lengths=lens)
+    if kv is not None:
+        opts["kv_lengths"] = kv
+    m = kv or lens
+    if prefix:
+        host["prefix"] = [x // 3 + 1 for x in m]
+        opts["prefix"] = torch.tensor(host["prefix"], device="cuda")
+    if bias:
+        host["slopes"] = opts["slopes"] = slopes_of(H)
+    # what no document holds is never read as a value
+    for b in range(B):
+        for t, n in ((q, lens[b]), (g, lens[b]), (k, m[b]), (v, m[b])):
+            t[b, n:] = math.nan
+    out = check(mm, O, q, k, v, docs_padded(lens, m, N, S), opts, g=g, flat=flat4, lse_flat=lse4, host=host)
+    # lengths on the device, and views of a packed projection with heads in front: the same bits
+    opts["lengths"] = torch.tensor(lens, dtype=torch.int64, device="cuda")
+    big = torch.full((B, H, N, D + 24), math.nan, dtype=dtype, device="cuda")
+    big[..., 8:8 + D] = q.transpose(1, 2)
+    assert torch.equal(mm.attention.attention(big[..., 8:8 + D].transpose(1, 2), k, v, **opts), out)
+    odd = torch.empty(q.numel() + 1, dtype=dtype, device="cuda")[1:].view(q.shape).copy_(q)
+    assert torch.equal(mm.attention.attention(odd, k, v, **opts), out)
+
+
+PACKED = [
+    # lens, lead, tail, H, K, D, dtype, causal, prefix, bias, cap
+    ([5], 0, 0, 1, 1, 64, HF, False, False, False, 0.0),
+    ([1, 200, 0, 64, 129, 1, 1, 33], 0, 7, 4, 2, 64, BF, True, False, False, 30.0),
+    ([100, 0, 128, 300], 131, 140, 2, 1, 128, HF, False, False, True, 0.0),
+    ([7] * 150, 3, 0, 2, 2, 32, BF, True, True, False, 0.0),
+    ([0, 0], 4, 9, 2, 1, 64, HF, True, False, False, 0.0),
+]
+
+
+@pytest.mark.parametrize("case", PACKED, ids=lambda c: f"{c[0][:8]}x{c[3]}x{c[5]}")
+def test_packed(mm, O, case):
+    lens, lead, tail, H, K, D, dtype, causal, prefix, bias, cap = case
+    off = [lead]
+    for n in lens:
+        off.append(off[-1] + n)
+    T = off[-1] + tail
+    gen = torch.Generator().manual_seed(T + D)
+    q, g = (torch.randn(T, H, D, generator=gen).to(dtype).cuda() for _ in "qg")
+    k, v = (torch.randn(T, K, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    for t in (q, k, v, g):
+        t[:lead] = math.nan
+        t[off[-1]:] = math.inf
+    host, opts = {}, dict(causal=causal, cap=cap, offsets=torch.tensor(off, dtype=torch.int32, device="cuda"))
+    if prefix:
+        host["prefix"] = opts["prefix"] = [n // 2 for n in lens]
+    if bias:
+        host["slopes"] = opts["slopes"] = slopes_of(H)
+    docs = [(off[d], n, off[d], n) for d, n in enumerate(lens)]
+    out = check(mm, O, q, k, v, docs, opts, g=g, host=host)
+    opts["offsets"] = off
+    assert torch.equal(mm.attention.attention(q, k, v, **opts), out)
+
+
+def test_documents_do_not_touch_each_other(mm):
+    """A document full of NaN and infinities changes no other document's rows or gradients, and each document is what it is alone."""
+    gen = torch.Generator().manual_seed(4)
+    lens = [70, 50, 130]
+    off = [0, 70, 120, 250]
+    q, g = (torch.randn(250, 4, 64, generator=gen).to(BF).cuda() for _ in "qg")
+    k, v = (torch.randn(250, 2, 64, generator=gen).to(BF).cuda() for _ in "kv")
+    fn = mm.attention.attention
+
+    def run(q, k, v, g, **kw):
+        q, k, v = (t.detach().clone().requires_grad_() for t in (q, k, v))
+        o = fn(q, k, v, causal=True, **kw)
+        return (o.detach(),) + torch.autograd.grad(o, [q, k, v], g)
+    clean = run(q, k, v, g, offsets=off)
+    for d in range(3):
+        s = slice(off[d], off[d + 1])
+        alone = run(q[None, s], k[None, s], v[None, s], g[None, s])
+        assert all(torch.equal(a[s], b[0]) for a, b in zip(clean, alone))
+    dirty = [t.clone() for t in (q, k, v, g)]
+    for t, x in zip(dirty, (math.nan, math.inf, -math.inf, math.nan)):
+        t[70:120] = x
+    r = run(*dirty, offsets=off)
+    for a, b in zip(r, clean):
+        assert torch.equal(a[:70], b[:70]) and torch.equal(a[120:], b[120:])
+
+
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_extreme_scores(mm, O, dtype):
+    """Scores of thousands (one key takes all), all keys alike, and scores that rise and fall along the keys past the point where the running
+    maximum is raised."""
+    gen = torch.Generator().manual_seed(6)
+    T, D = 400, 64
+    q = torch.randn(1, T, 2, D, generator=gen)
+    k, v = torch.randn(1, T, 2, D, generator=gen), torch.randn(1, T, 2, D, generator=gen)
+    ramp = torch.linspace(-6, 6, T)[None, :, None, None]
+    docs = [(0, T, 0, T)]
+    for a, b in ((q * 30, k * 30), (torch.zeros_like(q), k), (q.abs(), ramp.expand(k.shape) * 3), (q.abs(), -ramp.expand(k.shape) * 3)):
+        check(mm, O, a.to(dtype).cuda(), b.to(dtype).cuda(), v.to(dtype).cuda(), docs, dict(causal=False), flat=flat4, lse_flat=lse4)
+
+
+@pytest.mark.parametrize("size", [1e-4, 1.0, 1e3])
+def test_float16_gradients_of_every_size(mm, O, size):
+    """Incoming gradients down to 1e-4 over 2000 keys: p (dp - delta) is far below float16's range, its scaled form is not."""
+    gen = torch.Generator().manual_seed(8)
+    T, D = 2000, 64
+    q, k, v = (torch.randn(1, T, 1, D, generator=gen).to(HF).cuda() for _ in "qkv")
+    g = (torch.randn(1, T, 1, D, generator=gen) * size).to(HF).cuda()
+    if size > 1:
+        v = v * 0.01                                            # gradients of q and k stay in float16's own range
+    check(mm, O, q, k, v, [(0, T, 0, T)], dict(causal=True), g=g, flat=flat4, lse_flat=lse4)
+
+
+def test_value_differences(mm):
+    """o is linear in v: <g, o(v + h) - o(v)> is <dv, h> up to the roundings of o."""
+    gen = torch.Generator().manual_seed(11)
+    q, k, v, g, h = (torch.randn(2, 200, 2, 64, generator=gen).to(HF).cuda() for _ in range(5))
+    fn = mm.attention.attention
+    v = v.requires_grad_()
+    w = (v.detach() + h)
+    o = fn(q, k, v, causal=True)
+    (dv,) = torch.autograd.grad(o, [v], g)
+    d = (g.double() * (fn(q, k, w, causal=True).double() - o.detach().double())).sum()
+    step = (w.double() - v.detach().double())
+    size = (g.double().abs() * (fn(q, k, w.abs(), causal=True).double() + fn(q, k, v.detach().abs(), causal=True).double())).sum() \
+        + (dv.double().abs() * step.abs()).sum()
+    assert abs(float(d - (dv.double() * step).sum())) <= 3 * 2.0 ** -11 * float(size)
+
+
+def test_partial_gradients_and_broadcast(mm):
+    """Gradients of some inputs only, an expanded gradient, keys broadcast over the batch."""
+    gen = torch.Generator().manual_seed(12)
+    fn = mm.attention.attention
+    q = torch.randn(3, 40, 2, 64, generator=gen).to(BF).cuda().requires_grad_()
+    k, v = (torch.randn(1, 40, 2, 64, generator=gen).to(BF).cuda().requires_grad_() for _ in "kv")
+    full = torch.autograd.grad(fn(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1)).float().sum(), [q, k, v])
+    each = [torch.autograd.grad(fn(q[b:b + 1], k, v).float().sum(), [q, k, v]) for b in range(3)]
+    assert torch.equal(full[0], each[0][0] + each[1][0] + each[2][0])
+    for i in (1, 2):
+        total = sum(e[i].float() for e in each)
+        assert ((full[i].float() - total).abs() <= 3 * 2.0 ** -8 * sum(e[i].float().abs() for e in each) + 1e-30).all()
+    (only,) = torch.autograd.grad(fn(q, k.detach().expand(3, -1, -1, -1), v.detach().expand(3, -1, -1, -1)).float().sum(), [q])
+    assert torch.equal(only, full[0])
+
+
+def test_streams_and_graph(mm):
+    fn = mm.attention.attention
+    q, k, v, g = (torch.randn(2, 150, 2, 64, device="cuda").to(HF) for _ in range(4))
+    lengths = torch.tensor([150, 77], dtype=torch.int32, device="cuda")
+
+    def step(q, k, v):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        o = fn(q, k, v, lengths=lengths, causal=True)
+        return (o.detach(),) + torch.autograd.grad(o, [q, k, v], g)
+    want = step(q, k, v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(q, k, v)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(q, k, v)
+    for i in range(3):
+        for t in (q, k, v, g):
+            t.copy_(torch.randn(t.shape, device="cuda"))
+        lengths.copy_(torch.tensor([150 - i, 60 + 30 * i]))
+        graph.replay()
+        want = step(q, k, v)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        torch.cuda.synchronize()
+
+
+def test_bad_counts_on_the_device_are_clamped(mm):
+    """Lengths past the rows read and write nothing past them: the tensors lie inside larger ones whose rest stays as it was."""
+    fn = mm.attention.attention
+    pool = torch.randn(3, 4, 100, 2, 64, device="cuda").to(BF)
+    q, k, v = (pool[i, 1:3] for i in range(3))
+    keep = pool.clone()
+    full = fn(q, k, v)
+    assert torch.equal(fn(q, k, v, lengths=torch.tensor([100000, 2 ** 31 - 1], device="cuda")), full)
+    none = fn(q, k, v, lengths=torch.tensor([-5, -2 ** 31], device="cuda"))
+    assert (none == 0).all()
+    p = pool[0, 1], pool[1, 1], pool[2, 1]
+    o = fn(*p, offsets=torch.tensor([0, 40, 10 ** 6], device="cuda"))
+    assert torch.equal(o, fn(*p, offsets=[0, 40, 100]))
+    assert torch.equal(pool, keep)
+
+
+def test_refusals(mm):
+    fn = mm.attention.attention
+    q, k, v = (torch.randn(2, 10, 4, 64, device="cuda").to(BF) for _ in "qkv")
+    for call, error in [
+        (lambda: fn(q, k[:, :, :3], v[:, :, :3]), ValueError), (lambda: fn(q, k, v[:, :5]), ValueError), (lambda: fn(q, k[:1], v[:1]), ValueError),
+        (lambda: fn(q.float(), k.float(), v.float()), TypeError), (lambda: fn(q, k.to(HF), v), TypeError), (lambda: fn(q[..., :20], k[..., :20], v[..., :20]), ValueError),
+        (lambda: fn(q[0], k[0], v[0]), ValueError), (lambda: fn(q, k, v, offsets=[0, 10]), ValueError), (lambda: fn(q, k, v, lengths=[1]), ValueError),
+        (lambda: fn(q, k, v, lengths=[1, 11]), ValueError), (lambda: fn(q, k, v, lengths=[1.0, 2.0]), TypeError), (lambda: fn(q, k, v, prefix=[1, 1]), ValueError),
+        (lambda: fn(q, k, v, cap=-1.0), ValueError), (lambda: fn(q, k, v, scale=0.0), ValueError), (lambda: fn(q, k, v, scale=math.nan), ValueError),
+        (lambda: fn(q, k, v, slopes=torch.ones(3)), ValueError), (lambda: fn(q, k, v, slopes=torch.ones(4, requires_grad=True)), ValueError),
+        (lambda: fn(q, k, v, kv_offsets=[0, 1]), ValueError), (lambda: fn(q[0], k[0], v[0], offsets=[0, 5, 4]), ValueError),
+        (lambda: fn(q[0], k[0], v[0], offsets=[0, 11]), ValueError), (lambda: fn(q[0], k[0, :5], v[0, :5], offsets=[0, 5]), ValueError),
+        (lambda: fn(q[0], k[0], v[0], offsets=[0, 5], lengths=[1]), ValueError), (lambda: fn(q, k.cpu(), v), ValueError),
+    ]:
+        with pytest.raises(error):
+            call()
+    assert fn(q[:0], k[:0], v[:0]).shape == (0, 10, 4, 64)
+    assert fn(q[:, :0], k, v).shape == (2, 0, 4, 64)
+    assert (fn(q, k[:, :0], v[:, :0]) == 0).all()
+    c = fn(q.cpu(), k.cpu(), v.cpu())
+    assert not c.is_cuda and torch.equal(c, fn(q, k, v).cpu())

@@ -121,3 +121,82 @@ def test_share_of_views():
 def test_clip_entry_takes_empty_tensors(N):
     """Tensors without elements have no address: two of them share nothing, whatever their types."""
     assert clip(N, [None, 1 << 20, None], [0, 10, 0], [0, 0, 1], [None, 1 << 20, None], [1, 0, 1]) not in (0, -1)
+
+
+@pytest.mark.parametrize("opts", [dict(), dict(cap=2.0), dict(slope=0.3), dict(causal=True, prefix=3), dict(causal=True, cap=1.0, slope=0.1)])
+def test_oracle_gradients_against_differences(opts):
+    """The formulas the kernels' gradients are held to, against central differences in float64."""
+    from oracle import token_oracle as O
+    gen = torch.Generator().manual_seed(1)
+    q, k, v, g = (torch.randn(n, 8, generator=gen, dtype=torch.float64) for n in (5, 7, 7, 5))
+    r = O.attention_head(q, k, v, 0.4, g=g, **opts)
+    for name, x in (("dq", q), ("dk", k), ("dv", v)):
+        for _ in range(6):
+            d = torch.randn(x.shape, generator=gen, dtype=torch.float64)
+            h = 1e-5
+            def loss(s):
+                a = dict(dq=q, dk=k, dv=v)
+                a[name] = x + s * d
+                return float((O.attention_head(*a.values(), 0.4, **opts)["o"] * g).sum())
+            assert abs((loss(h) - loss(-h)) / (2 * h) - float((r[name] * d).sum())) <= 1e-8 * (1 + float((r[name] * d).abs().sum()))
+    # and against torch's own differentiation of softmax
+    if not opts:
+        qq, kk, vv = (t.clone().requires_grad_() for t in (q, k, v))
+        o = torch.softmax(0.4 * qq @ kk.T, 1) @ vv
+        assert torch.allclose(o, r["o"]) and all(torch.allclose(a, r[n]) for a, n in zip(torch.autograd.grad(o, [qq, kk, vv], g), ("dq", "dk", "dv")))
+
+
+def test_attention_wrapper_refuses(N):
+    """Checks that come before a device is asked for."""
+    from multi_modal_amd.attention import attention as fn
+    q = torch.zeros(2, 10, 4, 64, dtype=torch.bfloat16)
+    for call, error in [
+        (lambda: fn(q, q[:, :, :3], q[:, :, :3]), ValueError), (lambda: fn(q.float(), q.float(), q.float()), TypeError),
+        (lambda: fn(q[..., :12], q[..., :12], q[..., :12]), ValueError), (lambda: fn(q, q, q, offsets=[0, 10]), ValueError),
+        (lambda: fn(q, q, q, prefix=[1, 1]), ValueError), (lambda: fn(q, q, q, cap=math.inf), ValueError), (lambda: fn(q, q, q, scale=-1.0), ValueError),
+        (lambda: fn(q[0], q[0], q[0], offsets=[]), ValueError),
+    ]:
+        with pytest.raises(error):
+            call()
+
+
+def test_attention_entries_refuse(N):
+    """The C entries check sizes, types, alignment and pointers on the host; device 99 is what a good call is refused for."""
+    lib = N.load_library()
+    A = 1 << 20
+
+    def args(**kw):
+        a = dict(struct_size=ctypes.sizeof(N.AttentionArgs), dtype=2, n_docs=2, heads=4, kv_heads=2, dim=64, packed=0, causal=0, scale=0.1, cap=0.0, q_rows=10,
+                 k_rows=10, q=A, k=A, v=A, out=A, lse=A)
+        a.update(kw)
+        s = N.AttentionArgs(**{n: v for n, v in a.items() if "stride" not in n})
+        for n in ("q_stride", "k_stride", "v_stride", "out_stride"):
+            setattr(s, n, (ctypes.c_int64 * 3)(*a.get(n, (2560, 256, 64))))
+        s.lse_stride = (ctypes.c_int64 * 2)(40, 10)
+        return s
+
+    def forward(**kw):
+        return lib.mmfe_attention_forward(ctypes.byref(args(**kw)), 99, None)
+
+    def backward(grads=None, **kw):
+        g = dict(struct_size=ctypes.sizeof(N.AttentionGrads), grad_out=A, grad_q=A, grad_k=A, grad_v=A, scratch=A, norms=A)
+        g.update(grads or {})
+        s = N.AttentionGrads(**{n: v for n, v in g.items() if "stride" not in n})
+        for n in ("grad_out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride"):
+            setattr(s, n, (ctypes.c_int64 * 3)(*g.get(n, (2560, 256, 64))))
+        return lib.mmfe_attention_backward(ctypes.byref(args(**kw)), ctypes.byref(s), 99, None)
+    good = forward()
+    assert good not in (0, -1) and backward() == good
+    wrong = [dict(struct_size=8), dict(dtype=0), dict(dim=12), dict(dim=136), dict(dim=0), dict(n_docs=-1), dict(q_rows=-1), dict(k_rows=1 << 31), dict(heads=3),
+             dict(kv_heads=0), dict(scale=0.0), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(packed=1), dict(prefix=A), dict(q=None), dict(k=None),
+             dict(v=None), dict(out=None), dict(q=A + 8), dict(k_stride=(2560, 260, 64)), dict(v_stride=(2560, 256, 65)), dict(out_stride=(4, 256, 64)),
+             dict(k_stride=(0, 1 << 25, 64)), dict(q_stride=(-8, 256, 64)), dict(slopes=A, k_rows=1 << 25)]
+    for kw in wrong:
+        assert forward(**kw) == -1, kw
+        assert backward(**kw) == -1, kw
+    for kw in (dict(struct_size=4), dict(grad_out=None), dict(grad_q=None), dict(grad_k=None), dict(grad_v=None), dict(scratch=None), dict(grad_q=A + 2),
+               dict(grad_k_stride=(2560, 256, 4))):
+        assert backward(grads=kw) == -1, kw
+    assert backward(lse=None) == -1 and backward(grads=dict(norms=None), dtype=1) == -1 and backward(grads=dict(norms=None)) == good
+    assert lib.mmfe_attention_forward(None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, 0, None) == -1
+    assert forward(n_docs=0, q=None, k=None, v=None, out=None) == 0 and forward(q_rows=0, q=None, out=None) == 0
