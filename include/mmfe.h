@@ -327,13 +327,17 @@ typedef struct mmfe_attention_args {
     const int32_t* prefix;    /* n_docs entries or NULL; needs causal */
     const float* slopes;      /* heads entries or NULL */
     void* out;
+    void* out_rest;           /* like out (same strides): what the rounding of out lost, for the gradients; NULL: not wanted */
     float* lse;               /* (n_docs,) heads, q_rows by lse_stride; NULL: not wanted (backward needs it) */
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* batch, row, head */
     int64_t lse_stride[2];    /* batch, head; rows are contiguous */
 } mmfe_attention_args;
-int mmfe_attention_forward(const mmfe_attention_args* args, int device, void* hip_stream);
+/* Bytes of device memory mmfe_attention_forward needs for these arguments (few rows over many keys are cut into chunks of keys
+ * whose results are joined): 16-byte aligned, the call's own until it has run.  0: none.  -1: the arguments are refused. */
+int64_t mmfe_attention_workspace(const mmfe_attention_args* args);
+int mmfe_attention_forward(const mmfe_attention_args* args, void* workspace, int device, void* hip_stream);
 
-/* Gradients of q, k and v from the forward call's arguments (with its out and lse) and the gradient of out.  Those of a shared key
+/* Gradients of q, k and v from the forward call's arguments (with its out, lse and, where it was stored, out_rest) and the gradient of out.  Those of a shared key
  * head are summed over its query heads; rows outside the documents get zeros.  Sums have a fixed order: the same call gives the
  * same bits.  lse must be the dense (n_docs,) heads, q_rows array of the forward call. */
 typedef struct mmfe_attention_grads {

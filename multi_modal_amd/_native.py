@@ -36,7 +36,7 @@ EXPORTED_SYMBOLS = (
     "mmfe_plan_kernel",
     "mmfe_patch_embed_create", "mmfe_patch_embed_destroy", "mmfe_patch_embed_shape", "mmfe_patch_embed_run", "mmfe_patch_embed_update",
     "mmfe_rotary_create", "mmfe_rotary_destroy", "mmfe_rotary_run",
-    "mmfe_attention_forward", "mmfe_attention_backward",
+    "mmfe_attention_workspace", "mmfe_attention_forward", "mmfe_attention_backward",
     "mmfe_grad_partials", "mmfe_grad_clip",
 )
 
@@ -88,7 +88,7 @@ class AttentionArgs(ctypes.Structure):
     """mmfe_attention_args"""
     _fields_ = [(n, ctypes.c_int32) for n in ("struct_size", "dtype", "n_docs", "heads", "kv_heads", "dim", "packed", "causal")] + [
         ("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_rows", ctypes.c_int64), ("k_rows", ctypes.c_int64)] + [
-        (n, ctypes.c_void_p) for n in ("q", "k", "v", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "out", "lse")] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "out", "out_rest", "lse")] + [
         (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("lse_stride", ctypes.c_int64 * 2)]
 
 
@@ -165,7 +165,9 @@ def bind_library(path: str):
     lib.mmfe_rotary_run.restype = ctypes.c_int
     lib.mmfe_rotary_run.argtypes = [ctypes.c_void_p, ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
     lib.mmfe_attention_forward.restype = ctypes.c_int
-    lib.mmfe_attention_forward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_forward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_workspace.restype = c_i64
+    lib.mmfe_attention_workspace.argtypes = [ctypes.POINTER(AttentionArgs)]
     lib.mmfe_attention_backward.restype = ctypes.c_int
     lib.mmfe_attention_backward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionGrads), ctypes.c_int, ctypes.c_void_p]
     lib.mmfe_grad_partials.restype = c_i64
@@ -366,8 +368,14 @@ class RotaryHandle:
             pass
 
 
-def attention_forward(args: AttentionArgs, device: int, stream: int) -> None:
-    check(load_library().mmfe_attention_forward(ctypes.byref(args), device, stream or None), "mmfe_attention_forward")
+def attention_workspace(args: AttentionArgs) -> int:
+    n = load_library().mmfe_attention_workspace(ctypes.byref(args))
+    check(0 if n >= 0 else -1, "mmfe_attention_workspace")
+    return n
+
+
+def attention_forward(args: AttentionArgs, workspace_ptr: int, device: int, stream: int) -> None:
+    check(load_library().mmfe_attention_forward(ctypes.byref(args), workspace_ptr or None, device, stream or None), "mmfe_attention_forward")
 
 
 def attention_backward(args: AttentionArgs, grads: AttentionGrads, device: int, stream: int) -> None:

@@ -65,35 +65,39 @@ class _Call:
 
     __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes")
 
-    def args(self, q, k, v, out, lse) -> N.AttentionArgs:
+    def args(self, q, k, v, out, rest, lse) -> N.AttentionArgs:
         return N.AttentionArgs(
             _ARGS_SIZE, OUT_CODES[q.dtype], self.n_docs, q.shape[-2], k.shape[-2], q.shape[-1], self.packed, self.causal, self.scale, self.cap,
             q.shape[-3], k.shape[-3], q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(self.q_len), _ptr(self.k_len), _ptr(self.q_off), _ptr(self.k_off),
-            _ptr(self.prefix), _ptr(self.slopes), out.data_ptr(), _ptr(lse), _strides(q), _strides(k), _strides(v), _strides(out),
+            _ptr(self.prefix), _ptr(self.slopes), out.data_ptr(), _ptr(rest), _ptr(lse), _strides(q), _strides(k), _strides(v), _strides(out),
             (0, 0) if lse is None else (lse.stride(0), lse.stride(1)) if lse.dim() == 3 else (0, lse.stride(0)))
 
-    def forward(self, q, k, v, want_lse: bool):
+    def forward(self, q, k, v, want_lse: bool, want_rest: bool = False):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        rest = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_rest else None
         lse = None
         if want_lse:
             shape = (q.shape[-2], q.shape[-3])
             lse = torch.empty(shape if self.packed else (q.shape[0],) + shape, dtype=torch.float32, device=q.device)
-        N.attention_forward(self.args(q, k, v, out, lse), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
-        return out, lse
+        args = self.args(q, k, v, out, rest, lse)
+        need = N.attention_workspace(args) if q.shape[-3] <= 64 and not self.packed else 0
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        N.attention_forward(args, _ptr(work), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        return out, rest, lse
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, call):
-        out, lse = call.forward(q, k, v, True)
+        out, rest, lse = call.forward(q, k, v, True, True)
         ctx.call = call
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     def backward(ctx, grad_out, _):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         call = ctx.call
         g = _rows(grad_out)
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -101,7 +105,7 @@ class _AttentionFn(torch.autograd.Function):
         norms = torch.zeros(2 * call.n_docs * k.shape[-2], dtype=torch.int32, device=q.device) if q.dtype == torch.float16 else None
         grads = N.AttentionGrads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _strides(g), _strides(gq), _strides(gk),
                                  _strides(gv), scratch.data_ptr(), _ptr(norms))
-        N.attention_backward(call.args(q, k, v, out, lse), grads, q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        N.attention_backward(call.args(q, k, v, out, rest, lse), grads, q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None
 
@@ -188,7 +192,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _AttentionFn.apply(q, k, v, call)
     else:
-        out, lse = call.forward(q, k, v, return_lse)
+        out, _, lse = call.forward(q, k, v, return_lse)
     if origin.type != "cuda":
         out, lse = out.to(origin), None if lse is None else lse.to(origin)
     return (out, lse) if return_lse else out

@@ -12,6 +12,13 @@
 //
 // What is rounded: p to the tensors' 16-bit type for the second product (half a step each, independent, so the error of o is that
 // of its own rounding again); the sums of p are taken before that rounding, in float32, as are maximum, sum and both accumulators.
+// Documents of at most kShortKeys keys add a second product with what the rounding of p lost: there an error has few others to average
+// with, in o and through delta = g . o in the gradients (grad_q of 3-key documents was 2.0 times as far from the exact one as a
+// float32 computation rounded once), and their time is launch and latency.
+// A call whose gradients will be wanted also stores the rest of o, what its rounding to 16 bits lost, for delta.
+//
+// Few rows over many keys (new tokens over what a stream has kept) would leave most of the machine idle in that form: split_kernel
+// below cuts the keys into chunks, one block each, and join_kernel puts the chunks' results together.
 // The running maximum is raised only when a row's scores exceed it by more than 8 (in log2 units): p stays below 2^8, which both
 // types hold, and most tiles skip the rescaling of o.
 #include "attention_tiles.h"
@@ -22,9 +29,12 @@ namespace mmfe {
 using namespace attn;
 namespace {
 
+constexpr int kSplitTile = 32;         // keys of a wave's tile in split_kernel
+
 struct ForwardArgs {
     Problem p;
     Rows out;
+    char* rest;                       // like out: what its rounding lost; NULL: not wanted
     float* lse;                       // (batch, heads, rows) or (heads, rows); NULL: not wanted
     int64_t lse_b, lse_h;
     int grid_tiles;
@@ -121,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
         float mx = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(x[0][i], x[1][i]));
-        mx = fmaxf(mx, other_half(mx));
+        mx = both_max(mx);
         if (__any((mx - m) * c > 8.f)) {
             const float up = fmaxf(m, mx);
             const float alpha = exp2_fast(up == -INFINITY ? 0.f : (m - up) * c);
@@ -145,32 +155,309 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
             const u32x4 pf = operand<BF>(x[s >> 1], s & 1);
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) o[i] = mfma<BF>(read_cols<DP>(vt, 16 * s, 32 * i), pf, o[i]);
+            if (nk <= kShortKeys) {
+                const u32x4 rf = operand_rest<BF>(x[s >> 1], s & 1, pf);
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) o[i] = mfma<BF>(read_cols<DP>(vt, 16 * s, 32 * i), rf, o[i]);
+            }
         }
     }
-    l += other_half(l);
+    l = both_sum(l);
     if (row >= d.rows) return;
     const bool some = lim > 0;
     const float inv = some ? 1.f / l : 0.f;
-    char* out = const_cast<char*>(row_base(a.out, d, d.q0 + row, head));
+    const int64_t at = 2 * (d.batch * a.out.b + (d.q0 + row) * a.out.n + head * a.out.h);
+    char* out = static_cast<char*>(const_cast<void*>(a.out.p)) + at;
+    char* rest = a.rest ? a.rest + at : nullptr;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int e = 32 * i + 8 * g;
-            if (e < p.dim) {
-                u32x2 w{0, 0};
-                if (some) w = u32x2{pack2<BF>(o[i][4 * g] * inv, o[i][4 * g + 1] * inv), pack2<BF>(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv)};
-                *reinterpret_cast<u32x2*>(out + 2 * (e + 4 * half)) = w;
-            }
+            if (e >= p.dim) continue;
+            const int to = 2 * (e + 4 * half);
+            if (some) store4<BF>(out + to, rest ? rest + to : nullptr, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
+            else store4<BF>(out + to, rest ? rest + to : nullptr, 0.f, 0.f, 0.f, 0.f);
         }
     if (a.lse != nullptr && half == 0)
         a.lse[d.batch * a.lse_b + head * a.lse_h + d.q0 + row] = some ? (m * c + __builtin_amdgcn_logf(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
+// ---- few rows over many keys ----
+//
+// The rows of one key head are its query heads' rows, row r = (token r / group, query head r % group), so that a group reads its keys
+// once; a block takes 32 of them and one chunk of the keys.  Its 4 waves work on tiles of 32 keys of their own (every fourth one), each
+// with its own double-buffered LDS tiles and no barrier, and meet once at the end.  Bound by reading k and v: the products run at
+// 32 rows whatever the number of valid ones, and p enters with both halves (hi + rest), which costs nothing here.
+
+struct SplitArgs {
+    ForwardArgs f;
+    int chunk, n_splits, row_tiles;
+    float* part;                      // (unit, split, 32, dim) partial results over their own maximum; (unit, split, 32, 2) maximum and sum behind them
+    float* part_ml;
+};
+
+// Row r of a unit.
+struct SplitRow {
+    int token, head;
+    bool valid;
+    __device__ __forceinline__ SplitRow(const Problem& p, int r, int kvh, int nq) {
+        token = r / p.group;
+        head = kvh * p.group + r - token * p.group;
+        valid = token < nq;
+    }
+};
+
+template <bool BF>
+__device__ __forceinline__ void finish_row(const ForwardArgs& f, int doc, const SplitRow& r, int e, bool some, float m, float l, float4 v) {
+    const int64_t at = 2 * (doc * f.out.b + r.token * f.out.n + r.head * f.out.h + e);
+    const float inv = some ? 1.f / l : 0.f;
+    char* out = static_cast<char*>(const_cast<void*>(f.out.p)) + at;
+    if (some) store4<BF>(out, f.rest ? f.rest + at : nullptr, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    else store4<BF>(out, f.rest ? f.rest + at : nullptr, 0.f, 0.f, 0.f, 0.f);
+    if (e == 0 && f.lse != nullptr)
+        f.lse[doc * f.lse_b + r.head * f.lse_h + r.token] = some ? (m + __builtin_amdgcn_logf(l)) * (1.f / kLog2e) : -INFINITY;
+}
+
+template <bool BF, int DP>
+__global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // per wave: 2 x [k tile][v tile]
+    const Problem& p = a.f.p;
+    constexpr int kTileBytes = kSplitTile * DP * 2;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    const int unit = blockIdx.x / a.n_splits, split = blockIdx.x - unit * a.n_splits;
+    const int kvh = unit % p.kv_heads, rt = (unit / p.kv_heads) % a.row_tiles;
+    const int b = unit / p.kv_heads / a.row_tiles;
+    Doc d;
+    (void)find_doc<true>(p, b, kRows, d);                             // padded, one "tile" per document
+    const int nq = d.nq, nk = d.nk, off = nk - nq;
+    const int n_rows = min(32, (int)p.q_rows * p.group - 32 * rt);    // rows that exist, valid or not
+    auto limit = [&](int token) { return token >= nq ? 0 : p.causal ? min(nk, max(d.prefix, token + off + 1)) : nk; };
+    const int last_token = min((32 * rt + n_rows - 1) / p.group, nq - 1);
+    const int max_lim = last_token >= 0 && 32 * rt / p.group < nq ? limit(last_token) : 0;
+    const int full_lim = limit(32 * rt / p.group);
+    const int s0 = split * a.chunk, s1 = min(s0 + a.chunk, max_lim);
+    float2* ml = reinterpret_cast<float2*>(a.part_ml) + (int64_t)blockIdx.x * 32;
+    if (s0 >= s1 && a.n_splits > 1) {                                 // nothing of this chunk is visible to these rows
+        if (threadIdx.x < n_rows) ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    const SplitRow mine(p, 32 * rt + col, kvh, nq);
+    const int lim = col < n_rows ? limit(mine.token) : 0;
+    const int n_tiles = s1 > s0 ? (s1 - s0 + kSplitTile - 1) / kSplitTile : 0;
+
+    Loader<DP, kSplitTile, 1> lk, lv;
+    lk.init(p.dim, p.k.n, 0);
+    lv.init(p.dim, p.v.n, 0);
+    const unsigned lds0 = uniform(lds_address(smem) + wave * 4 * kTileBytes);
+    auto stage = [&](int t, int buf) {
+        const int j0 = s0 + t * kSplitTile;
+        const unsigned dst = uniform(lds0 + buf * 2 * kTileBytes);
+        lk.load(row_base(p.k, d, j0, kvh), nk - j0, p.dim, p.k.n, dst, 0);
+        lv.load(row_base(p.v, d, j0, kvh), nk - j0, p.dim, p.v.n, dst + kTileBytes, 0);
+    };
+    u32x4 qf[DP / 16];
+    {
+        const bool ok = mine.valid && col < n_rows;
+        const char* q = row_base(p.q, d, ok ? mine.token : 0, ok ? mine.head : 0);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            qf[s] = u32x4{0, 0, 0, 0};
+            if (ok && 16 * s + 8 * half < p.dim) qf[s] = *reinterpret_cast<const u32x4*>(q + 32 * s + 16 * half);
+        }
+    }
+    const bool shaped = p.cap > 0.f || p.slopes != nullptr;
+    const float c = shaped ? 1.f : p.scale * kLog2e;
+    const float slope = p.slopes && col < n_rows ? p.slopes[mine.head] * kLog2e : 0.f;
+    const float cap_in = p.cap > 0.f ? p.scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
+    if (wave < n_tiles) stage(wave, 0);
+
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
+    float m = -INFINITY, l = 0.f;
+    int buf = 0;
+    for (int t = wave; t < n_tiles; t += kWaves, buf ^= 1) {
+        if (t + kWaves < n_tiles) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the other buffer has been read
+            stage(t + kWaves, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * Loader<DP, kSplitTile, 1>::kCount) : "memory");      // all but the tile just asked for
+        } else wait_all();
+        const int j0 = s0 + t * kSplitTile;
+        const char* kt = smem + (wave * 2 + buf) * 2 * kTileBytes;
+        const char* vt = kt + kTileBytes;
+        f32x16 x{};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) x = mfma<BF>(read_rows<DP>(kt, 0, s), qf[s], x);
+        if (shaped) {
+            const float at = (float)(mine.token + off - j0 - 4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float v = p.cap > 0.f ? cap_out * tanh_fast(x[i] * cap_in) : x[i] * (p.scale * kLog2e);
+                if (p.slopes) v -= slope * fabsf(at - (float)reg_row(i));
+                x[i] = v;
+            }
+        }
+        if (j0 + kSplitTile > full_lim || j0 + kSplitTile > s1) {
+            const int left = min(lim, s1) - j0 - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = reg_row(i) < left ? x[i] : -INFINITY;
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+        mx = both_max(mx);
+        if (__any((mx - m) * c > 8.f)) {
+            const float up = fmaxf(m, mx);
+            const float alpha = exp2_fast(up == -INFINITY ? 0.f : (m - up) * c);
+            m = up;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = exp2_fast(fmaf(x[i], c, -mc));
+            sum += x[i];
+        }
+        l += sum;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const u32x4 pf = operand<BF>(x, s), rf = operand_rest<BF>(x, s, pf);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                const u32x4 vf = read_cols<DP>(vt, 16 * s, 32 * i);
+                o[i] = mfma<BF>(vf, pf, o[i]);
+                o[i] = mfma<BF>(vf, rf, o[i]);
+            }
+        }
+    }
+    l = both_sum(l);
+    m = m * c;                                                        // log2 units (c > 0; -inf stays)
+    // the waves' results meet in LDS: [wave][row][DP + 4] values, [wave][row] maximum and sum
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_sync();
+    constexpr int kPitch = DP + 4;
+    float* wo = reinterpret_cast<float*>(smem);
+    float2* wml = reinterpret_cast<float2*>(wo + kWaves * 32 * kPitch);
+    if (col < n_rows) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4*>(wo + (wave * 32 + col) * kPitch + 32 * i + 8 * g + 4 * half) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+        if (half == 0) wml[wave * 32 + col] = make_float2(m, l);
+    }
+    __syncthreads();
+    const int pieces = p.dim / 4;
+    for (int i = threadIdx.x; i < n_rows * pieces; i += kThreads) {
+        const int r = i / pieces, e = 4 * (i - r * pieces);
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wml[w * 32 + r].x);
+        float total = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 s = wml[w * 32 + r];
+            if (s.y == 0.f) continue;                                 // saw no key
+            const float k = exp2_fast(s.x - top);
+            const float4 u = *reinterpret_cast<const float4*>(wo + (w * 32 + r) * kPitch + e);
+            total += k * s.y;
+            v.x += k * u.x; v.y += k * u.y; v.z += k * u.z; v.w += k * u.w;
+        }
+        const SplitRow row(p, 32 * rt + r, kvh, nq);
+        if (a.n_splits == 1) finish_row<BF>(a.f, b, row, e, limit(row.token) > 0, top, total, v);
+        else {
+            *reinterpret_cast<float4*>(a.part + ((int64_t)blockIdx.x * 32 + r) * p.dim + e) = v;
+            if (e == 0) ml[r] = make_float2(top, total);
+        }
+    }
+}
+
+// One block per row: kThreads / (dim / 4) chunks at a time, then the chunks' sums in LDS.
+template <bool BF>
+__global__ void __launch_bounds__(kThreads) join_kernel(const SplitArgs a) {
+    __shared__ float4 lds_v[kThreads];
+    __shared__ float2 lds_ml[kThreads];
+    const Problem& p = a.f.p;
+    const int unit = blockIdx.x >> 5, r = blockIdx.x & 31;
+    const int kvh = unit % p.kv_heads, rt = (unit / p.kv_heads) % a.row_tiles;
+    const int b = unit / p.kv_heads / a.row_tiles;
+    if (32 * rt + r >= (int)p.q_rows * p.group) return;
+    Doc d;
+    (void)find_doc<true>(p, b, kRows, d);
+    const int pieces = p.dim / 4, groups = kThreads / pieces;
+    const int g = threadIdx.x / pieces, e = 4 * (threadIdx.x - g * pieces);
+    float top = -INFINITY, total = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (g < groups)
+        for (int s = g; s < a.n_splits; s += groups) {
+            const int64_t at = (int64_t)(unit * a.n_splits + s) * 32 + r;
+            const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[at];
+            if (ml.y == 0.f) continue;
+            const float4 u = *reinterpret_cast<const float4*>(a.part + at * p.dim + e);
+            const float up = fmaxf(top, ml.x);
+            const float k0 = exp2_fast(top - up), k1 = exp2_fast(ml.x - up);
+            top = up;
+            total = total * k0 + ml.y * k1;
+            v.x = v.x * k0 + u.x * k1; v.y = v.y * k0 + u.y * k1; v.z = v.z * k0 + u.z * k1; v.w = v.w * k0 + u.w * k1;
+        }
+    lds_v[threadIdx.x] = v;
+    lds_ml[threadIdx.x] = make_float2(top, total);
+    __syncthreads();
+    if (g != 0) return;
+    for (int o = 1; o < groups; ++o) top = fmaxf(top, lds_ml[o * pieces + threadIdx.x].x);
+    total = 0.f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int o = 0; o < groups; ++o) {
+        const float2 ml = lds_ml[o * pieces + threadIdx.x];
+        if (ml.y == 0.f) continue;
+        const float k = exp2_fast(ml.x - top);
+        const float4 u = lds_v[o * pieces + threadIdx.x];
+        total += k * ml.y;
+        v.x += k * u.x; v.y += k * u.y; v.z += k * u.z; v.w += k * u.w;
+    }
+    const SplitRow row(p, 32 * rt + r, kvh, d.nq);
+    const int lim = !row.valid ? 0 : p.causal ? min(d.nk, max(d.prefix, row.token + d.nk - d.nq + 1)) : d.nk;
+    finish_row<BF>(a.f, b, row, e, lim > 0, top, total, v);
+}
+
 typedef void (*forward_fn)(const ForwardArgs);
+typedef void (*split_fn)(const SplitArgs);
 template <bool BF>
 forward_fn pick_forward(int dim) {
     return dim <= 32 ? &forward_kernel<BF, 32> : dim <= 64 ? &forward_kernel<BF, 64> : &forward_kernel<BF, 128>;
+}
+template <bool BF>
+split_fn pick_split(int dim) {
+    return dim <= 32 ? &split_kernel<BF, 32> : dim <= 64 ? &split_kernel<BF, 64> : &split_kernel<BF, 128>;
+}
+
+// Keys of a chunk and chunks of a unit, or no chunks: the row kernel serves the call.
+struct Cut {
+    int row_tiles = 0, chunk = 0, n_splits = 0;
+    int64_t units = 0;
+};
+Cut cut_keys(const mmfe_attention_args* a) {
+    Cut c;
+    if (a->packed || a->q_rows < 1 || a->n_docs < 1) return c;
+    const int64_t rows = a->q_rows * (a->heads / a->kv_heads);
+    if (a->q_rows > 64 || rows > 1024 || a->k_rows <= kShortKeys) return c;
+    c.row_tiles = (int)((rows + 31) / 32);
+    c.units = (int64_t)a->n_docs * c.row_tiles * a->kv_heads;
+    // About 2048 blocks if every document fills its room, in chunks of 256 keys at least; up to 512 keys stay in one block (a wave then has 4 tiles,
+    // less than the second launch takes)
+    int64_t chunk = (a->k_rows * c.units + 2047) / 2048;
+    chunk = (chunk + 127) / 128 * 128;
+    if (chunk < 256) chunk = 256;
+    if (a->k_rows <= 512) chunk = 512;
+    c.chunk = (int)chunk;
+    c.n_splits = (int)((a->k_rows + chunk - 1) / chunk);
+    if (c.n_splits < 1) c.n_splits = 1;
+    return c;
 }
 
 }  // namespace
@@ -235,7 +522,14 @@ using namespace mmfe;
 
 extern "C" {
 
-int mmfe_attention_forward(const mmfe_attention_args* a, int device, void* hip_stream) {
+int64_t mmfe_attention_workspace(const mmfe_attention_args* a) {
+    Problem p{};
+    if (make_problem(a, p)) return -1;
+    const Cut c = cut_keys(a);
+    return c.n_splits > 1 ? c.units * c.n_splits * 32 * (a->dim + 2) * (int64_t)sizeof(float) : 0;
+}
+
+int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int device, void* hip_stream) {
     ForwardArgs f{};
     int rc = make_problem(a, f.p);
     if (rc) return rc;
@@ -245,11 +539,35 @@ int mmfe_attention_forward(const mmfe_attention_args* a, int device, void* hip_s
     if (bad_rows("out", a->out, a->out_stride)) return MMFE_EINVAL;
     if (tiles * a->heads > 0x7fffffffll) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
     f.out = Rows{a->out, a->out_stride[0], a->out_stride[1], a->out_stride[2]};
+    f.rest = static_cast<char*>(a->out_rest);
+    if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     f.lse = a->lse; f.lse_b = a->lse_stride[0]; f.lse_h = a->lse_stride[1];
     f.grid_tiles = (int)tiles;
+    const Cut c = cut_keys(a);
+    if (c.n_splits > 1 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
+    if (c.units * c.n_splits > 0x7fffffffll || c.units > 0x3ffffff) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
     OnDevice on(device);
     if (on.rc) return on.rc;
-    const forward_fn fn = a->dtype == MMFE_OUT_BF16 ? pick_forward<true>(a->dim) : pick_forward<false>(a->dim);
+    const bool bf = a->dtype == MMFE_OUT_BF16;
+    if (c.n_splits > 0) {
+        SplitArgs s{};
+        s.f = f;
+        s.f.p.tiles = 1;
+        s.chunk = c.chunk; s.n_splits = c.n_splits; s.row_tiles = c.row_tiles;
+        s.part = static_cast<float*>(workspace);
+        s.part_ml = c.n_splits > 1 ? s.part + c.units * c.n_splits * 32 * a->dim : nullptr;
+        const split_fn fn = bf ? pick_split<true>(a->dim) : pick_split<false>(a->dim);
+        const int dp = padded_dim(a->dim);
+        const size_t tiles = (size_t)kWaves * 4 * kSplitTile * dp * 2, meet = (size_t)kWaves * 32 * ((dp + 4) * 4 + 8);
+        const size_t lds = tiles > meet ? tiles : meet;
+        int blocks = 1, cus = 256;
+        rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);
+        if (rc) return rc;
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(c.units * c.n_splits)), dim3(kThreads), lds, reinterpret_cast<hipStream_t>(hip_stream), s);
+        if (c.n_splits > 1) hipLaunchKernelGGL(bf ? &join_kernel<true> : &join_kernel<false>, dim3((uint32_t)(c.units * 32)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(hip_stream), s);
+        return launched("attention");
+    }
+    const forward_fn fn = bf ? pick_forward<true>(a->dim) : pick_forward<false>(a->dim);
     const size_t lds = 4 * (size_t)kTile * padded_dim(a->dim) * 2;
     int blocks = 1, cus = 256;
     rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);

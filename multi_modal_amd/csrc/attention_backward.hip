@@ -9,7 +9,8 @@
 // forms scores as rows x keys (a lane has one key), the row pass as keys x rows (a lane has one row); sums over the lane's own index stay in
 // registers for the whole walk.
 //
-// What is rounded: p and ds to the 16-bit type, for the second products; delta, dp, and all sums are float32.  float16 has 5
+// What is rounded: p and ds to the 16-bit type, for the second products; dp and all sums are float32, and delta is formed from o and
+// the rest that its rounding lost.  Short documents add second products with what the rounding of p and ds lost, as the forward pass does.  float16 has 5
 // exponent bits, which products p (dp - delta) of long rows and small gradients fall out of.  Its values are therefore scaled by
 // powers of two, exactly: p by 2^8, and (dp - delta) by phi = 2^(6 - ceil(log2(max |g_i| max |v_j|))) per document and key head, with which
 // |dp| phi <= 2^6 by Cauchy and Schwarz, |delta| phi too (o is a mean of v), and |ds| <= 2^15: nothing overflows, and values down to
@@ -34,6 +35,7 @@ namespace {
 struct BackwardArgs {
     Problem p;
     Rows out, g, dq, dk, dv;
+    const char* rest;                 // like out: what its rounding lost, or NULL
     const float* lse;
     float *lse2, *delta;              // like lse: lse in log2 units (less the shift of p; +inf for rows without keys), g . o
     int64_t lse_b, lse_h;
@@ -43,12 +45,6 @@ struct BackwardArgs {
 
 template <bool BF>
 constexpr float kShift = BF ? 0.f : 8.f;
-
-template <bool BF>
-__device__ __forceinline__ float widen(unsigned w, int hi) {
-    if constexpr (BF) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
-    else return (float)__builtin_bit_cast(_Float16, (unsigned short)(hi ? w >> 16 : w));
-}
 
 __device__ __forceinline__ void block_max(float v, unsigned* to) {
     __shared__ float m[kWaves];
@@ -73,12 +69,15 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const BackwardArgs a) {
         const int row = d.tile * kRows + r;
         float dot = 0.f, sq = 0.f;
         if (row < d.nq && e < p.dim) {
-            const u32x4 o = *reinterpret_cast<const u32x4*>(row_base(a.out, d, d.q0 + row, head) + 2 * e);
+            const int64_t at = 2 * (d.batch * a.out.b + (d.q0 + row) * a.out.n + head * a.out.h + e);
+            const u32x4 o = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.out.p) + at);
+            u32x4 rest{0, 0, 0, 0};
+            if (a.rest != nullptr) rest = *reinterpret_cast<const u32x4*>(a.rest + at);
             const u32x4 g = *reinterpret_cast<const u32x4*>(row_base(a.g, d, d.q0 + row, head) + 2 * e);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float x = widen<BF>(g[i >> 1], i & 1);
-                dot = fmaf(x, widen<BF>(o[i >> 1], i & 1), dot);
+                dot = fmaf(x, widen<BF>(o[i >> 1], i & 1) + widen<BF>(rest[i >> 1], i & 1), dot);
                 if constexpr (!BF) sq = fmaf(x, x, sq);
             }
         }
@@ -289,6 +288,11 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
                 const u32x4 pf = operand<BF>(x, s);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) dv[i] = mfma<BF>(read_cols<DP>(gt, 32 * b + 16 * s, 32 * i), pf, dv[i]);
+                if (nk <= kShortKeys) {
+                    const u32x4 rf = operand_rest<BF>(x, s, pf);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) dv[i] = mfma<BF>(read_cols<DP>(gt, 32 * b + 16 * s, 32 * i), rf, dv[i]);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] *= dp[i];
@@ -301,6 +305,11 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
                 const u32x4 df = operand<BF>(x, s);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) dk[i] = mfma<BF>(read_cols<DP>(qt, 32 * b + 16 * s, 32 * i), df, dk[i]);
+                if (nk <= kShortKeys) {
+                    const u32x4 rf = operand_rest<BF>(x, s, df);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) dk[i] = mfma<BF>(read_cols<DP>(qt, 32 * b + 16 * s, 32 * i), rf, dk[i]);
+                }
             }
         }
         g = gn;
@@ -308,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
     }
     if (key >= d.rows) return;
     const float back = __builtin_amdgcn_exp2f(-kShift<BF>);
-    store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, d.k0 + key, kvh)), dk, p.dim, p.scale * back / phi, key < nk && steps > 0);
+    store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, d.k0 + key, kvh)), dk, p.dim, p.scale * back / phi, key < nk && steps > 0 && nk > 1);      // a softmax over one key is constant
     store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, d.k0 + key, kvh)), dv, p.dim, back, key < nk && steps > 0);
 }
 
@@ -409,11 +418,16 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
                 const u32x4 df = operand<BF>(x, s);
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i) dq[i] = mfma<BF>(read_cols<DP>(kt, 32 * b + 16 * s, 32 * i), df, dq[i]);
+                if (nk <= kShortKeys) {
+                    const u32x4 rf = operand_rest<BF>(x, s, df);
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) dq[i] = mfma<BF>(read_cols<DP>(kt, 32 * b + 16 * s, 32 * i), rf, dq[i]);
+                }
             }
         }
     }
     if (row >= d.rows) return;
-    store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi, lim > 0);
+    store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi, lim > 1);       // a softmax over one key is constant
 }
 
 template <bool BF, int DP>
@@ -453,13 +467,14 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     if (any_q && (a->out == nullptr || a->lse == nullptr || g->grad_out == nullptr || g->grad_q == nullptr || g->scratch == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
     if (any_k && (g->grad_k == nullptr || g->grad_v == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
     if (a->dtype == MMFE_OUT_F16 && (any_q || any_k) && a->n_docs > 0 && g->norms == nullptr) { set_error("attention: NULL norms"); return MMFE_EINVAL; }
+    if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride) || bad_rows("grad_out", g->grad_out, g->grad_out_stride) || bad_rows("grad_q", g->grad_q, g->grad_q_stride) ||
         bad_rows("grad_k", g->grad_k, g->grad_k_stride) || bad_rows("grad_v", g->grad_v, g->grad_v_stride)) return MMFE_EINVAL;
     if (count_tiles(b.p, a->q_rows, kRows) * a->heads > 0x7fffffffll || count_tiles(b.p, a->k_rows, kRows) * a->kv_heads > 0x7fffffffll) {
         set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL;
     }
     auto rows = [](const void* ptr, const int64_t* s) { return Rows{ptr, s[0], s[1], s[2]}; };
-    b.out = rows(a->out, a->out_stride); b.g = rows(g->grad_out, g->grad_out_stride);
+    b.out = rows(a->out, a->out_stride); b.rest = static_cast<const char*>(a->out_rest); b.g = rows(g->grad_out, g->grad_out_stride);
     b.dq = rows(g->grad_q, g->grad_q_stride); b.dk = rows(g->grad_k, g->grad_k_stride); b.dv = rows(g->grad_v, g->grad_v_stride);
     b.lse = a->lse; b.lse_b = a->lse_stride[0]; b.lse_h = a->lse_stride[1];
     const int64_t n = (a->packed ? 1 : (int64_t)a->n_docs) * a->heads * a->q_rows;

@@ -29,6 +29,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kRows = 128;            // rows of a block: 32 per wave
 constexpr int kTile = 64;             // rows of a streamed tile
+constexpr int kShortKeys = 128;       // documents of at most so many keys: 16-bit operands made of float32 values enter with their rest
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A tensor of (batch, row, head) vectors with unit stride inside; strides in elements, batch = 0 where documents are packed.
@@ -254,7 +255,37 @@ __device__ __forceinline__ u32x4 operand(const f32x16& v, int s) {
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// over the two lanes (half 0 and 1) of a column
+__device__ __forceinline__ float both_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <bool BF>
+__device__ __forceinline__ float widen(unsigned w, int hi) {
+    if constexpr (BF) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
+    else return (float)__builtin_bit_cast(_Float16, (unsigned short)(hi ? w >> 16 : w));
+}
+// what operand(v, s), given as `hi`, lost to rounding, as another operand
+template <bool BF>
+__device__ __forceinline__ u32x4 operand_rest(const f32x16& v, int s, u32x4 hi) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack2<BF>(v[8 * s + 2 * i] - widen<BF>(hi[i], 0), v[8 * s + 2 * i + 1] - widen<BF>(hi[i], 1));
+    return r;
+}
+// four results (4 consecutive columns of a lane's row) to 16-bit memory, and what that rounding lost next to it
+template <bool BF>
+__device__ __forceinline__ void store4(char* to, char* rest, float a, float b, float c, float d) {
+    const u32x2 w{pack2<BF>(a, b), pack2<BF>(c, d)};
+    *reinterpret_cast<u32x2*>(to) = w;
+    if (rest != nullptr)
+        *reinterpret_cast<u32x2*>(rest) = u32x2{pack2<BF>(a - widen<BF>(w.x, 0), b - widen<BF>(w.x, 1)), pack2<BF>(c - widen<BF>(w.y, 0), d - widen<BF>(w.y, 1))};
+}
 
 // tanh(z) from one exponential: 1 - 2 / (e^(2 z) + 1); absolute error a few 2^-24, exact limits
 __device__ __forceinline__ float tanh_fast(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_fast(2.f * kLog2e * z) + 1.f); }

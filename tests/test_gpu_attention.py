@@ -161,6 +161,74 @@ def test_packed(mm, O, case):
     assert torch.equal(mm.attention.attention(q, k, v, **opts), out)
 
 
+TOKENS = [
+    # q rows, lens of keys, room, H, K, D, dtype, causal, prefix, bias, cap
+    (1, [1, 0, 31, 32, 33, 4000], 4096, 8, 2, 128, BF, True, False, False, 0.0),
+    (1, [500], 512, 12, 12, 64, HF, True, False, True, 0.0),
+    (5, [5, 3000, 129, 2], 3001, 6, 2, 72, BF, True, True, False, 20.0),
+    (64, [700, 64], 700, 4, 1, 32, HF, True, False, True, 0.0),
+    (33, [9000, 40], 9001, 4, 4, 64, BF, False, False, False, 0.0),
+    (2, [1025, 1024, 1023], 1025, 16, 1, 8, HF, False, False, False, 0.0),
+    (1, [70000], 70001, 3, 1, 64, BF, True, False, False, 0.0),
+]
+
+
+@pytest.mark.parametrize("case", TOKENS, ids=lambda c: f"{c[0]}x{c[1][-1]}x{c[3]}x{c[5]}")
+def test_few_rows_over_many_keys(mm, O, case):
+    n, kv, room, H, K, D, dtype, causal, prefix, bias, cap = case
+    B = len(kv)
+    gen = torch.Generator().manual_seed(room)
+    lens = [n] * (B - 1) + [max(1, n - 1)]
+    q, g = (torch.randn(B, n, H, D, generator=gen).to(dtype).cuda() for _ in "qg")
+    k, v = (torch.randn(B, room, K, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    for b in range(B):
+        k[b, kv[b]:] = math.nan
+        v[b, kv[b]:] = math.nan
+        q[b, lens[b]:] = math.nan
+        g[b, lens[b]:] = math.nan
+    host, opts = {}, dict(causal=causal, cap=cap, lengths=lens, kv_lengths=torch.tensor(kv, device="cuda"))
+    if prefix:
+        host["prefix"] = opts["prefix"] = [m // 2 for m in kv]
+    if bias:
+        host["slopes"] = opts["slopes"] = slopes_of(H)
+    out = check(mm, O, q, k, v, docs_padded(lens, kv, n, room), opts, g=g, flat=flat4, lse_flat=lse4, host=host)
+    for b in (0, B - 1):            # alone, with no more room than it needs
+        m = max(kv[b], 1)
+        o = dict(opts, lengths=lens[b:b + 1], kv_lengths=kv[b:b + 1])
+        if prefix:
+            o["prefix"] = opts["prefix"][b:b + 1]
+        alone = mm.attention.attention(q[b:b + 1], k[b:b + 1, :m], v[b:b + 1, :m], **o)
+        assert ((alone[0].double() - out[b].double()).abs() <= 2 * torch.finfo(dtype).eps * out[b].double().abs() + 1e-3).all()
+
+
+def test_one_nan_key_reaches_its_rows(mm):
+    """A NaN in a key that a row sees makes that row NaN, whichever chunk it lies in, and no other document's."""
+    fn = mm.attention.attention
+    k, v = (torch.randn(2, 3000, 1, 64, device="cuda").to(BF) for _ in "kv")
+    q = torch.randn(2, 1, 4, 64, device="cuda").to(BF)
+    want = fn(q, k, v)
+    for at in (0, 31, 32, 1500, 2999):
+        bad = k.clone()
+        bad[0, at] = math.nan
+        o = fn(q, bad, v)
+        assert o[0].isnan().all() and torch.equal(o[1], want[1])
+        o = fn(q, bad, v, kv_lengths=[at, 3000])
+        assert o[0].isfinite().all() and torch.equal(o[1], want[1])
+
+
+def test_one_key_has_no_score_gradient(mm):
+    """A softmax over one key is constant: gradients of q and k are exactly zero, that of v is the incoming one."""
+    fn = mm.attention.attention
+    for n in (1, 3):
+        q, g = (torch.randn(2, n, 2, 64, device="cuda").to(BF) for _ in "qg")
+        k, v = (torch.randn(2, 1, 2, 64, device="cuda").to(BF) for _ in "kv")
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+        o = fn(q, k, v)
+        assert torch.equal(o, v.expand(2, n, 2, 64))
+        dq, dk, dv = torch.autograd.grad(o, [q, k, v], g)
+        assert (dq == 0).all() and (dk == 0).all() and (n > 1 or torch.equal(dv, g))
+
+
 def test_documents_do_not_touch_each_other(mm):
     """A document full of NaN and infinities changes no other document's rows or gradients, and each document is what it is alone."""
     gen = torch.Generator().manual_seed(4)

@@ -176,7 +176,7 @@ def test_attention_entries_refuse(N):
         return s
 
     def forward(**kw):
-        return lib.mmfe_attention_forward(ctypes.byref(args(**kw)), 99, None)
+        return lib.mmfe_attention_forward(ctypes.byref(args(**kw)), A, 99, None)
 
     def backward(grads=None, **kw):
         g = dict(struct_size=ctypes.sizeof(N.AttentionGrads), grad_out=A, grad_q=A, grad_k=A, grad_v=A, scratch=A, norms=A)
@@ -191,6 +191,11 @@ def test_attention_entries_refuse(N):
              dict(kv_heads=0), dict(scale=0.0), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(packed=1), dict(prefix=A), dict(q=None), dict(k=None),
              dict(v=None), dict(out=None), dict(q=A + 8), dict(k_stride=(2560, 260, 64)), dict(v_stride=(2560, 256, 65)), dict(out_stride=(4, 256, 64)),
              dict(k_stride=(0, 1 << 25, 64)), dict(q_stride=(-8, 256, 64)), dict(slopes=A, k_rows=1 << 25)]
+    assert lib.mmfe_attention_forward(ctypes.byref(args(k_rows=10 ** 6)), None, 99, None) == -1          # 10 rows over many keys: a workspace
+    assert lib.mmfe_attention_forward(ctypes.byref(args(k_rows=10 ** 6)), A + 8, 99, None) == -1
+    assert lib.mmfe_attention_workspace(ctypes.byref(args(k_rows=10 ** 6))) > 0 and lib.mmfe_attention_workspace(ctypes.byref(args())) == 0
+    assert lib.mmfe_attention_workspace(ctypes.byref(args(dim=12))) == -1
+    wrong.append(dict(out_rest=A + 2))
     for kw in wrong:
         assert forward(**kw) == -1, kw
         assert backward(**kw) == -1, kw
@@ -198,5 +203,5 @@ def test_attention_entries_refuse(N):
                dict(grad_k_stride=(2560, 256, 4))):
         assert backward(grads=kw) == -1, kw
     assert backward(lse=None) == -1 and backward(grads=dict(norms=None), dtype=1) == -1 and backward(grads=dict(norms=None)) == good
-    assert lib.mmfe_attention_forward(None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, 0, None) == -1
+    assert lib.mmfe_attention_forward(None, None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, 0, None) == -1
     assert forward(n_docs=0, q=None, k=None, v=None, out=None) == 0 and forward(q_rows=0, q=None, out=None) == 0
