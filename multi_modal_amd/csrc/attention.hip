@@ -8,7 +8,7 @@
 // A wave owns 32 rows and computes the TRANSPOSED scores of 32 keys x 32 rows at a time (keys as the first operand), so that a
 // lane holds scores of one row only: maximum and sum are register arithmetic plus one exchange between the wave's halves, the
 // running state is one value per lane, and the scores, rounded to the 16-bit type, are the second operand of the next product
-// (o^T += v^T p^T) as they stand.  Keys and values come by LDS-DMA into double-buffered tiles of 64 rows that the 4 waves share.
+// (o^T += v^T p^T) as they stand.  Keys and values come by LDS-DMA, in tiles of 32 rows that the 4 waves share, several steps ahead.
 //
 // What is rounded: p to the tensors' 16-bit type for the second product (half a step each, independent, so the error of o is that
 // of its own rounding again); the sums of p are taken before that rounding, in float32, as are maximum, sum and both accumulators.
@@ -40,11 +40,81 @@ struct ForwardArgs {
     int grid_tiles;
 };
 
-template <bool BF, int DP>
+// How scores leave the linear form (bits); anything but kPlain takes them to log2 units before the maximum.
+enum { kPlain = 0, kBias = 1, kCap = 2 };
+
+template <int SHAPE>
+struct Shape {
+    float c, slope, cap_in, cap_out;
+    __device__ __forceinline__ Shape(const Problem& p, int head) {
+        c = p.scale * kLog2e;
+        slope = SHAPE & kBias ? p.slopes[head] * kLog2e : 0.f;
+        cap_in = SHAPE & kCap ? p.scale / p.cap : 0.f;
+        cap_out = SHAPE & kCap ? p.cap * kLog2e : 0.f;
+    }
+    // x: products of 32 keys from j0 on; at = row + off - j0 - 4 * half: distance to the lane's first key
+    __device__ __forceinline__ void apply(f32x16& x, float at) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (SHAPE & kCap) x[i] = cap_out * tanh_fast(x[i] * cap_in);
+            if constexpr (SHAPE == kBias) x[i] = fmaf(x[i], c, -slope * fabsf(at - (float)reg_row(i)));
+            if constexpr (SHAPE == (kBias | kCap)) x[i] = fmaf(-slope, fabsf(at - (float)reg_row(i)), x[i]);
+        }
+    }
+    // factor from the units the maximum is kept in to log2 units
+    __device__ __forceinline__ float unit() const { return SHAPE == kPlain ? c : 1.f; }
+};
+
+// Softmax state of a lane's row, and what 32 keys do to it.
+struct State {
+    float m = -INFINITY, l = 0.f;
+    __device__ __forceinline__ static float largest(const f32x16& a) {
+        float m = a[0], k = a[1];
+#pragma unroll
+        for (int i = 2; i < 16; i += 4) {
+            m = max2(max2(m, a[i]), a[i + 1]);
+            if (i + 2 < 16) k = max2(max2(k, a[i + 2]), a[i + 3]);
+        }
+        return both_max(max2(m, k));
+    }
+    // raises the running maximum when scores exceed it by more than 8 log2 units; true: o and l have to be scaled by alpha
+    __device__ __forceinline__ bool raise(float mx, float unit, float& alpha) {
+        if (!__any((mx - m) * unit > 8.f)) return false;
+        const float up = max2(m, mx);
+        alpha = exp2_fast(up == -INFINITY ? 0.f : (m - up) * unit);
+        m = up;
+        l *= alpha;
+        return true;
+    }
+    __device__ __forceinline__ void exponentials(f32x16& x, float unit) {
+        const float mc = m == -INFINITY ? 0.f : m * unit;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            x[i] = exp2_fast(fmaf(x[i], unit, -mc));
+            x[i + 1] = exp2_fast(fmaf(x[i + 1], unit, -mc));
+            s0 += x[i];
+            s1 += x[i + 1];
+        }
+        l += s0 + s1;
+    }
+};
+
+__device__ __forceinline__ void hide(f32x16& x, int left) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = reg_row(i) < left ? x[i] : -INFINITY;
+}
+
+// Keys of a step, and tiles of keys (and of values) in LDS.
+constexpr int kStepKeys = 32;
+constexpr int kRing = 4;
+static_assert(kStepKeys * kRing >= kShortKeys, "a short document's keys are in LDS at once");
+
+template <bool BF, int DP, int SHAPE>
 __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(16))) char smem[];               // [kRing k tiles][kRing v tiles]
     const Problem& p = a.p;
-    constexpr int kTileBytes = kTile * DP * 2;
+    constexpr int kTileBytes = kStepKeys * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int j = blockIdx.x % p.heads;
     const int t0 = blockIdx.x / p.heads;
@@ -62,18 +132,27 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     const int wave_lim = w0 < nq ? limit(w0 + 31) : 0;
     const int full_lim = w0 < nq ? limit(w0) : 0;                             // keys that all rows of the wave see
     const int lim = row < nq ? limit(row) : 0;
-    const int n_tiles = block_lim > 0 ? (block_lim + kTile - 1) / kTile : 0;
+    const int n = block_lim > 0 ? (block_lim + kStepKeys - 1) / kStepKeys : 0;            // steps
 
-    Loader<DP, kTile, kWaves> lk, lv;
+    typedef Loader<DP, kStepKeys, kWaves> Load;
+    Load lk, lv;
     lk.init(p.dim, p.k.n, wave);
     lv.init(p.dim, p.v.n, wave);
     const unsigned lds0 = lds_address(smem);
-    auto stage = [&](int t, int buf) {
-        const unsigned dst = uniform(lds0 + buf * 2 * kTileBytes);
-        lk.load(row_base(p.k, d, d.k0 + (int64_t)t * kTile, kvh), nk - t * kTile, p.dim, p.k.n, dst, wave);
-        lv.load(row_base(p.v, d, d.k0 + (int64_t)t * kTile, kvh), nk - t * kTile, p.dim, p.v.n, dst + kTileBytes, wave);
+    auto load_k = [&](int t) {
+        lk.load(row_base(p.k, d, d.k0 + (int64_t)t * kStepKeys, kvh), nk - t * kStepKeys, p.dim, p.k.n, uniform(lds0 + (t % kRing) * kTileBytes), wave);
     };
-    if (n_tiles > 0) stage(0, 0);
+    auto load_v = [&](int t) {
+        lv.load(row_base(p.v, d, d.k0 + (int64_t)t * kStepKeys, kvh), nk - t * kStepKeys, p.dim, p.v.n, uniform(lds0 + (kRing + t % kRing) * kTileBytes), wave);
+    };
+    // in the order in which the steps need them
+    if (n > 0) load_k(0);
+    if (n > 1) load_k(1);
+#pragma unroll
+    for (int t = 0; t < kRing - 2; ++t) {
+        if (t < n) load_v(t);
+        if (t + 2 < n) load_k(t + 2);
+    }
 
     u32x4 qf[DP / 16];
     {
@@ -85,84 +164,100 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
             if (nq > 0 && 16 * s + 8 * half < p.dim) qf[s] = *reinterpret_cast<const u32x4*>(q + 32 * s + 16 * half);
         }
     }
-    const bool shaped = p.cap > 0.f || p.slopes != nullptr;                    // scores leave the linear form: they are taken to log2 units first
-    const float c = shaped ? 1.f : p.scale * kLog2e;
-    const float slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;
-    const float cap_in = p.cap > 0.f ? p.scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
-
-    f32x16 o[DP / 32];
+    const Shape<SHAPE> sh(p, head);
+    const float unit = sh.unit();
+    f32x16 o[DP / 32], x{};
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
-    float m = -INFINITY, l = 0.f;
+    State st;
 
-    for (int t = 0; t < n_tiles; ++t) {
-        wait_all();                    // this wave's part of tile t is there, and its reads of the other buffer are done
-        block_sync();                  // ... and so for every wave
-        if (t + 1 < n_tiles) stage(t + 1, (t + 1) & 1);
-        const int j0 = t * kTile;
-        if (j0 >= wave_lim) continue;
-        const char* kt = smem + (t & 1) * 2 * kTileBytes;
-        const char* vt = kt + kTileBytes;
-        f32x16 x[2];
+    auto scores = [&](int t) {
+        const char* kt = smem + (t % kRing) * kTileBytes;
+        f32x16 y{};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            x[b] = f32x16{};
+        for (int s = 0; s < DP / 16; ++s) y = mfma<BF>(read_rows<DP>(kt, 0, s), qf[s], y);
+        return y;
+    };
+    auto values = [&](int t, int s, u32x4 pf) {
+        const char* vt = smem + (kRing + t % kRing) * kTileBytes;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) x[b] = mfma<BF>(read_rows<DP>(kt, 32 * b, s), qf[s], x[b]);
-        }
-        if (shaped) {
-            const float at = (float)(row + off - j0 - 4 * half);
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float v = p.cap > 0.f ? cap_out * tanh_fast(x[b][i] * cap_in) : x[b][i] * (p.scale * kLog2e);
-                    if (p.slopes) v -= slope * fabsf(at - (float)(32 * b + reg_row(i)));
-                    x[b][i] = v;
-                }
-        }
-        if (j0 + kTile > full_lim) {
-            const int left = lim - j0 - 4 * half;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[b][i] = 32 * b + reg_row(i) < left ? x[b][i] : -INFINITY;
-        }
-        float mx = fmaxf(x[0][0], x[1][0]);
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(x[0][i], x[1][i]));
-        mx = both_max(mx);
-        if (__any((mx - m) * c > 8.f)) {
-            const float up = fmaxf(m, mx);
-            const float alpha = exp2_fast(up == -INFINITY ? 0.f : (m - up) * c);
-            m = up;
-            l *= alpha;
+        for (int i = 0; i < DP / 32; ++i) o[i] = mfma<BF>(read_cols<DP>(vt, 16 * s, 32 * i), pf, o[i]);
+    };
+    auto shape_and_hide = [&](int t) {
+        const int j0 = t * kStepKeys;
+        if constexpr (SHAPE != kPlain) sh.apply(x, (float)(row + off - j0 - 4 * half));
+        if (j0 + kStepKeys > full_lim) hide(x, lim - j0 - 4 * half);
+    };
+    auto rescale = [&](float mx) {
+        float alpha;
+        if (st.raise(mx, unit, alpha)) {
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
-        float sum = 0.f;
+    };
+
+    const bool at_once = nk <= kShortKeys;                                    // at most kRing tiles: all of them are asked for here
+    if (at_once)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int t = kRing - 2; t < kRing; ++t)
+            if (t < n) load_v(t);
+    wait_all();
+    block_sync();
+    arrived(qf);
+    if (at_once) {
+        for (int t = 0; t < n && t * kStepKeys < wave_lim; ++t) {
+            x = scores(t);
+            shape_and_hide(t);
+            rescale(State::largest(x));
+            st.exponentials(x, unit);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[b][i] = exp2_fast(fmaf(x[b][i], c, -mc));
-                sum += x[b][i];
-            }
-        l += sum;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const u32x4 pf = operand<BF>(x[s >> 1], s & 1);
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) o[i] = mfma<BF>(read_cols<DP>(vt, 16 * s, 32 * i), pf, o[i]);
-            if (nk <= kShortKeys) {
-                const u32x4 rf = operand_rest<BF>(x[s >> 1], s & 1, pf);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) o[i] = mfma<BF>(read_cols<DP>(vt, 16 * s, 32 * i), rf, o[i]);
+            for (int s = 0; s < 2; ++s) {
+                const u32x4 pf = operand<BF>(x, s);
+                values(t, s, pf);
+                values(t, s, operand_rest<BF>(x, s, pf));
             }
         }
+    } else if (n > 0) {
+        // Products of one step run beside the softmax of another: step t turns the scores of its 32 keys, computed a step earlier, into p,
+        // while the matrix pipe adds step t - 1 to o (beside the maximum) and forms the scores of step t + 1 (beside the exponentials).
+        // So step t needs k of t + 1 and v of t - 1; their buffers' former tiles were used up in step t - 1 at the latest, and it asks for
+        // k of t + kRing and v of t + kRing - 2: kRing - 1 steps ahead of their use.
+        constexpr int kAhead = (kRing - 2) * 2 * Load::kCount;
+        u32x4 pf[2];
+        if (wave_lim > 0) x = scores(0);
+        for (int t = 0; t < n; ++t) {
+            if (t - 1 + kRing < n) wait_but<kAhead>();     // the last kRing - 2 steps asked for a whole tile of each
+            else wait_all();
+            block_sync();              // every wave's parts have arrived, and its reads of the buffers that are asked for now are done
+            if (t + kRing < n) load_k(t + kRing);
+            if (t + kRing - 2 < n) load_v(t + kRing - 2);
+            const int j0 = t * kStepKeys;
+            if (j0 < wave_lim) {
+                shape_and_hide(t);
+                const float mx = State::largest(x);
+                if (t > 0) {
+                    values(t - 1, 0, pf[0]);
+                    values(t - 1, 1, pf[1]);
+                }
+                rescale(mx);
+                const f32x16 y = scores(t + 1);      // past the last step: of whatever the buffer holds, and dropped
+                st.exponentials(x, unit);
+                pf[0] = operand<BF>(x, 0);
+                pf[1] = operand<BF>(x, 1);
+                x = y;
+            } else if (t > 0 && j0 - kStepKeys < wave_lim) {
+                values(t - 1, 0, pf[0]);
+                values(t - 1, 1, pf[1]);
+            }
+        }
+        wait_all();
+        block_sync();
+        if ((n - 1) * kStepKeys < wave_lim) {
+            values(n - 1, 0, pf[0]);
+            values(n - 1, 1, pf[1]);
+        }
     }
-    l = both_sum(l);
+    const float l = both_sum(st.l);
     if (row >= d.rows) return;
     const bool some = lim > 0;
     const float inv = some ? 1.f / l : 0.f;
@@ -180,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
             else store4<BF>(out + to, rest ? rest + to : nullptr, 0.f, 0.f, 0.f, 0.f);
         }
     if (a.lse != nullptr && half == 0)
-        a.lse[d.batch * a.lse_b + head * a.lse_h + d.q0 + row] = some ? (m * c + __builtin_amdgcn_logf(l)) * (1.f / kLog2e) : -INFINITY;
+        a.lse[d.batch * a.lse_b + head * a.lse_h + d.q0 + row] = some ? (st.m * unit + __builtin_amdgcn_logf(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
 // ---- few rows over many keys ----
@@ -277,6 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
     for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.f;
     int buf = 0;
+    wait_all();
+    arrived(qf);
     for (int t = wave; t < n_tiles; t += kWaves, buf ^= 1) {
         if (t + kWaves < n_tiles) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the other buffer has been read
@@ -427,9 +524,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const SplitArgs a) {
 
 typedef void (*forward_fn)(const ForwardArgs);
 typedef void (*split_fn)(const SplitArgs);
+template <bool BF, int SHAPE>
+forward_fn pick_dim(int dim) {
+    return dim <= 32 ? &forward_kernel<BF, 32, SHAPE> : dim <= 64 ? &forward_kernel<BF, 64, SHAPE> : &forward_kernel<BF, 128, SHAPE>;
+}
 template <bool BF>
-forward_fn pick_forward(int dim) {
-    return dim <= 32 ? &forward_kernel<BF, 32> : dim <= 64 ? &forward_kernel<BF, 64> : &forward_kernel<BF, 128>;
+forward_fn pick_forward(int dim, bool bias, bool cap) {
+    if (bias) return cap ? pick_dim<BF, kBias | kCap>(dim) : pick_dim<BF, kBias>(dim);
+    return cap ? pick_dim<BF, kCap>(dim) : pick_dim<BF, kPlain>(dim);
 }
 template <bool BF>
 split_fn pick_split(int dim) {
@@ -567,8 +669,9 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
         if (c.n_splits > 1) hipLaunchKernelGGL(bf ? &join_kernel<true> : &join_kernel<false>, dim3((uint32_t)(c.units * 32)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(hip_stream), s);
         return launched("attention");
     }
-    const forward_fn fn = bf ? pick_forward<true>(a->dim) : pick_forward<false>(a->dim);
-    const size_t lds = 4 * (size_t)kTile * padded_dim(a->dim) * 2;
+    const bool bias = a->slopes != nullptr, cap = a->cap > 0.f;
+    const forward_fn fn = bf ? pick_forward<true>(a->dim, bias, cap) : pick_forward<false>(a->dim, bias, cap);
+    const size_t lds = 2 * (size_t)kRing * kStepKeys * padded_dim(a->dim) * 2;
     int blocks = 1, cus = 256;
     rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);
     if (rc) return rc;

@@ -229,6 +229,9 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
 
+    wait_all();
+    arrived(kf);
+    arrived(vf);
     int g = 0, t = t_first;
     for (int step = 0; step < steps; ++step) {
         wait_all();
@@ -366,6 +369,9 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dq[i] = f32x16{};
 
+    wait_all();
+    arrived(qf);
+    arrived(gf);
     for (int t = 0; t < n_tiles; ++t) {
         wait_all();
         block_sync();

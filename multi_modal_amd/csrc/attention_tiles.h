@@ -178,10 +178,14 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 template <int DP, int ROWS, int WAVES>
 struct Loader {
     static constexpr int kPieces = DP / 8;
-    static constexpr int kCount = ROWS * kPieces / 64 / WAVES;      // DMA instructions of a wave
-    static_assert(kCount * 64 * WAVES == ROWS * kPieces, "whole instructions");
-    unsigned off[kCount];                                           // byte offsets from the tile's first row
-    __device__ __forceinline__ static int piece(int i, int wave) { return (i * WAVES + wave) * 64 + (int)(threadIdx.x & 63); }
+    static constexpr int kAll = ROWS * kPieces / 64;                // DMA instructions
+    static constexpr int kCount = kAll > WAVES ? kAll / WAVES : 1;  // of a wave (where there are fewer than waves, some bring the same pieces)
+    static constexpr int kStep = 64 * WAVES / kPieces;              // rows from one of them to the next
+    static constexpr int kKept = kStep % 16 == 0 ? 1 : kCount;      // the swizzle repeats every 16 rows
+    static_assert(kAll * 64 == ROWS * kPieces && (kAll % WAVES == 0 || WAVES % kAll == 0), "whole instructions");
+    unsigned off[kKept];                                            // byte offsets from the tile's first row
+    __device__ __forceinline__ static int number(int i, int wave) { return (i * WAVES + wave) % kAll; }
+    __device__ __forceinline__ static int piece(int i, int wave) { return number(i, wave) * 64 + (int)(threadIdx.x & 63); }
     __device__ __forceinline__ static unsigned offset(int ci, int rows, int dim, unsigned stride) {
         const int r0 = ci / kPieces;
         const int c = (ci & (kPieces - 1)) ^ swizzle<DP>(r0);
@@ -190,25 +194,37 @@ struct Loader {
     }
     __device__ __forceinline__ void init(int dim, int64_t stride, int wave) {
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) off[i] = offset(piece(i, wave), ROWS, dim, (unsigned)(2 * stride));
+        for (int i = 0; i < kKept; ++i) off[i] = offset(piece(i, wave), ROWS, dim, (unsigned)(2 * stride));
     }
     // base: the tile's first row; rows >= 1: valid rows from there on
     __device__ __forceinline__ void load(const char* base, int rows, int dim, int64_t stride, unsigned lds, int wave) const {
         if (rows >= ROWS) {
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) dma16(base, off[i], lds + (i * WAVES + wave) * 1024);
+            for (int i = 0; i < kCount; ++i)
+                dma16(kKept == 1 ? base + i * kStep * 2 * stride : base, off[kKept == 1 ? 0 : i], lds + number(i, wave) * 1024);
         } else {
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) dma16(base, offset(piece(i, wave), rows, dim, (unsigned)(2 * stride)), lds + (i * WAVES + wave) * 1024);
+            for (int i = 0; i < kCount; ++i) dma16(base, offset(piece(i, wave), rows, dim, (unsigned)(2 * stride)), lds + number(i, wave) * 1024);
         }
     }
 };
 
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// all but the youngest N of this wave's DMAs have arrived; its LDS reads are done
+template <int N>
+__device__ __forceinline__ void wait_but() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory"); }
 __device__ __forceinline__ void block_sync() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+// Operands loaded from memory before a loop, once they have been waited for: says so to the compiler, which would otherwise wait for
+// them (and so for every DMA in flight) at their first use in every pass of the loop.
+template <int N>
+__device__ __forceinline__ void arrived(u32x4 (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 
 // Operand with one row per lane (row0 + c), step s of 16 columns.
@@ -255,10 +271,13 @@ __device__ __forceinline__ u32x4 operand(const f32x16& v, int s) {
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// The larger one, NaN if either is: v_maximum_f32 and, of three, v_maximum3_f32, without the canonicalising moves that fmaxf takes
+// along (51 of 59 instructions of a tile's row maximum were those).
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // over the two lanes (half 0 and 1) of a column
 __device__ __forceinline__ float both_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return max2(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float both_sum(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
