@@ -37,7 +37,6 @@ struct ForwardArgs {
     char* rest;                       // like out: what its rounding lost; NULL: not wanted
     float* lse;                       // (batch, heads, rows) or (heads, rows); NULL: not wanted
     int64_t lse_b, lse_h;
-    int grid_tiles;
 };
 
 // How scores leave the linear form (bits); anything but kPlain takes them to log2 units before the maximum.
@@ -117,9 +116,8 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     constexpr int kTileBytes = kStepKeys * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int j = blockIdx.x % p.heads;
-    const int t0 = blockIdx.x / p.heads;
     Doc d;
-    if (!find_doc<true>(p, a.grid_tiles - 1 - t0, kRows, d)) return;          // last tiles first: under a causal mask they are the long ones
+    if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
     const int head = head_of(p, j), kvh = head / p.group;
     const int row0 = d.tile * kRows, w0 = row0 + 32 * wave, row = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
@@ -587,7 +585,7 @@ int make_problem(const mmfe_attention_args* a, Problem& p) {
     if (a->q_rows > (1 << 30) || a->k_rows > (1 << 30) || a->n_docs > (1 << 24)) { set_error("attention: too many rows"); return MMFE_EINVAL; }
     if (a->slopes != nullptr && (a->q_rows > (1 << 24) || a->k_rows > (1 << 24))) { set_error("attention: distances are float32: at most 2^24 rows with slopes"); return MMFE_EINVAL; }
     if (!(a->scale > 0.f) || !std::isfinite(a->scale) || !(a->cap >= 0.f) || !std::isfinite(a->cap)) { set_error("attention: scale > 0 and cap >= 0 must be finite"); return MMFE_EINVAL; }
-    if (a->packed && a->n_docs > 0 && (a->q_off == nullptr || a->k_off == nullptr)) { set_error("attention: packed documents need offsets"); return MMFE_EINVAL; }
+    if (a->packed && (a->q_off == nullptr || a->k_off == nullptr)) { set_error("attention: packed documents need offsets"); return MMFE_EINVAL; }
     if (a->prefix != nullptr && !a->causal) { set_error("attention: a prefix belongs to a causal mask"); return MMFE_EINVAL; }
     const bool any_q = a->q_rows > 0 && (a->packed || a->n_docs > 0), any_k = a->k_rows > 0 && (a->packed || a->n_docs > 0);
     if ((any_q && a->q == nullptr) || (any_k && (a->k == nullptr || a->v == nullptr))) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
@@ -644,7 +642,6 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
     f.rest = static_cast<char*>(a->out_rest);
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     f.lse = a->lse; f.lse_b = a->lse_stride[0]; f.lse_h = a->lse_stride[1];
-    f.grid_tiles = (int)tiles;
     const Cut c = cut_keys(a);
     if (c.n_splits > 1 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
     if (c.units * c.n_splits > 0x7fffffffll || c.units > 0x3ffffff) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }

@@ -40,7 +40,6 @@ struct BackwardArgs {
     float *lse2, *delta;              // like lse: lse in log2 units (less the shift of p; +inf for rows without keys), g . o
     int64_t lse_b, lse_h;
     unsigned *norm_g, *norm_v;        // float16: largest squared row norms, per document and key head (bit patterns of floats >= 0)
-    int grid_tiles;
 };
 
 template <bool BF>
@@ -181,18 +180,25 @@ __device__ __forceinline__ void load_rows(u32x4 (&f)[DP / 16], const char* row, 
     }
 }
 
-// dk and dv of 128 keys (32 per wave)
+// dk and dv of 128 keys, 32 per wave.  Head sizes up to 64: 8 waves, the second four taking the second 32 rows of every tile, whose sums join
+// the first four's through LDS at the end; a block then takes half as long, and the longest one (4096 keys of a causal document,
+// three heads' rows behind it) bounds the launch: FIXME.  Head size 128 has no registers for that.
+template <int DP>
+constexpr int kKeyWaves = DP == 128 ? 4 : 8;
+
 template <bool BF, int DP>
-__global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const BackwardArgs a) {
+__global__ void __launch_bounds__(64 * kKeyWaves<DP>, 1) keys_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // 2 x [q tile][g tile][lse2][delta]
     const Problem& p = a.p;
     constexpr int kTileBytes = kTile * DP * 2;
     constexpr int kBuf = 2 * kTileBytes + 2 * kTile * 4;
+    constexpr int kW = kKeyWaves<DP>;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    const int part = wave >> 2;                                       // which of the tile's 32 rows (8 waves)
     const int kvh = blockIdx.x % p.kv_heads;
     Doc d;
     if (!find_doc<false>(p, blockIdx.x / p.kv_heads, kRows, d)) return;
-    const int key0 = d.tile * kRows, w0 = key0 + 32 * wave, key = w0 + col;
+    const int key0 = d.tile * kRows, w0 = key0 + 32 * (wave & 3), key = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
     // rows [first, nq) see key j: all of them, or those from j - off on
     auto first_row = [&](int j) { return p.causal && j >= d.prefix ? max(0, j - off) : 0; };
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
     const int t_first = block_first / kTile, t_end = block_first < nq ? (nq + kTile - 1) / kTile : t_first;
     const int per_head = t_end - t_first, steps = per_head * p.group;
 
-    Loader<DP, kTile, kWaves> lq, lg;
+    Loader<DP, kTile, kW> lq, lg;
     lq.init(p.dim, p.q.n, wave);
     lg.init(p.dim, a.g.n, wave);
     const unsigned lds0 = lds_address(smem);
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
         const float* delta = lse2 + kTile;
         const Shape sh(p, kvh * p.group + g);
 #pragma unroll 1
-        for (int b = 0; b < 2; ++b) {
+        for (int b = kW == 8 ? part : 0; b < (kW == 8 ? part + 1 : 2); ++b) {
             const int i0 = t * kTile + 32 * b;
             if (i0 + 32 <= wave_first || i0 >= nq) continue;
             f32x16 x{}, dp{};
@@ -318,6 +324,28 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
         g = gn;
         t = tn;
     }
+    if constexpr (kW == 8) {
+        wait_all();
+        block_sync();
+        float* meet = reinterpret_cast<float*>(smem) + (wave & 3) * (DP / 32) * 2 * 16 * 64 + lane;
+        if (part == 1)
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    meet[(i * 32 + r) * 64] = dk[i][r];
+                    meet[(i * 32 + 16 + r) * 64] = dv[i][r];
+                }
+        __syncthreads();
+        if (part == 1) return;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dk[i][r] += meet[(i * 32 + r) * 64];
+                dv[i][r] += meet[(i * 32 + 16 + r) * 64];
+            }
+    }
     if (key >= d.rows) return;
     const float back = __builtin_amdgcn_exp2f(-kShift<BF>);
     store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, d.k0 + key, kvh)), dk, p.dim, p.scale * back / phi, key < nk && steps > 0 && nk > 1);      // a softmax over one key is constant
@@ -332,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
     constexpr int kTileBytes = kTile * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     Doc d;
-    if (!find_doc<true>(p, a.grid_tiles - 1 - blockIdx.x / p.heads, kRows, d)) return;
+    if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
     const int head = head_of(p, blockIdx.x % p.heads), kvh = head / p.group;
     const int row0 = d.tile * kRows, w0 = row0 + 32 * wave, row = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
@@ -440,17 +468,17 @@ template <bool BF, int DP>
 int launch(BackwardArgs& b, int64_t q_rows, int64_t k_rows, hipStream_t stream) {
     Problem& p = b.p;
     int rc = MMFE_OK, blocks = 1, cus = 256;
-    const size_t tiles_lds = 4 * (size_t)kTile * DP * 2, keys_lds = tiles_lds + 4 * kTile * 4;
-    if ((rc = kernel_prepare(reinterpret_cast<const void*>(&keys_kernel<BF, DP>), kThreads, keys_lds, &blocks, &cus)) != MMFE_OK) return rc;
+    const size_t tiles_lds = 4 * (size_t)kTile * DP * 2, meet_lds = 4 * (size_t)(DP / 32) * 2 * 16 * 64 * 4;
+    const size_t keys_lds = kKeyWaves<DP> == 8 && meet_lds > tiles_lds + 4 * kTile * 4 ? meet_lds : tiles_lds + 4 * kTile * 4;
+    if ((rc = kernel_prepare(reinterpret_cast<const void*>(&keys_kernel<BF, DP>), 64 * kKeyWaves<DP>, keys_lds, &blocks, &cus)) != MMFE_OK) return rc;
     if ((rc = kernel_prepare(reinterpret_cast<const void*>(&rows_kernel<BF, DP>), kThreads, tiles_lds, &blocks, &cus)) != MMFE_OK) return rc;
     const int64_t tq = count_tiles(p, q_rows, kRows);
-    b.grid_tiles = (int)tq;
     const int q_tiles = p.tiles;
     if (tq > 0) hipLaunchKernelGGL((delta_kernel<BF, DP>), dim3((uint32_t)(tq * p.heads)), dim3(kThreads), 0, stream, b);
     const int64_t tk = count_tiles(p, k_rows, kRows);
     if (tk > 0) {
         if constexpr (!BF) hipLaunchKernelGGL((norm_kernel<DP>), dim3((uint32_t)(tk * p.kv_heads)), dim3(kThreads), 0, stream, b);
-        hipLaunchKernelGGL((keys_kernel<BF, DP>), dim3((uint32_t)(tk * p.kv_heads)), dim3(kThreads), keys_lds, stream, b);
+        hipLaunchKernelGGL((keys_kernel<BF, DP>), dim3((uint32_t)(tk * p.kv_heads)), dim3(64 * kKeyWaves<DP>), keys_lds, stream, b);
     }
     p.tiles = q_tiles;
     if (tq > 0) hipLaunchKernelGGL((rows_kernel<BF, DP>), dim3((uint32_t)(tq * p.heads)), dim3(kThreads), tiles_lds, stream, b);

@@ -67,15 +67,35 @@ struct Doc {
 __device__ __forceinline__ int clamp_int(int64_t v, int64_t lo, int64_t hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Sum over a wave's lanes, in every lane.
+__device__ __forceinline__ int wave_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);           // row_shr 1, 2, 4, 8: sums of 16 lanes in their last one
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    return __builtin_amdgcn_readlane(v, 15) + __builtin_amdgcn_readlane(v, 31) + __builtin_amdgcn_readlane(v, 47) + __builtin_amdgcn_readlane(v, 63);
+}
+
 // Document and tile of tile number t, on the query side (QSIDE) or the key side.  False: there is no such tile.
 // Packed rows that no document holds (before the first offset, behind the last) form tiles of their own, of a document without
 // partners: their results are zeros.  Offsets are clamped into the rows, so that no entry can lead out of the tensors.
+//
+// Blocks start in the order of their numbers, and a block's time goes with the partners its tile has, so tiles are numbered from the
+// longest to the shortest: under a causal mask the last row tile and the first key tile of a document have the most.  Packed
+// documents are sorted that way up to 64 of them (one lane each: under a causal mask by the tile's distance from the short end, found by
+// bisection over the counts; otherwise by the partners' number); of more documents a single one matters less, and they are taken in
+// reverse.  16 recordings of 1 to 4096 tokens, causal, forward: FIXME us sorted, 200 in reverse.
 template <bool QSIDE>
 __device__ __forceinline__ bool find_doc(const Problem& p, int t, int tile_rows, Doc& d) {
     if (!p.packed) {
-        const int b = t / p.tiles;
+        int b = t / p.tiles, tile = t - b * p.tiles;
+        if (p.causal) {                                   // all documents' longest tiles first
+            tile = t / p.n_docs;
+            b = t - tile * p.n_docs;
+            if (QSIDE) tile = p.tiles - 1 - tile;
+        }
         d.batch = d.index = b;
-        d.tile = t - b * p.tiles;
+        d.tile = tile;
         d.q0 = d.k0 = 0;
         d.nq = p.q_len ? clamp_int(uniform(p.q_len[b]), 0, p.q_rows) : (int)p.q_rows;
         d.nk = p.k_len ? clamp_int(uniform(p.k_len[b]), 0, p.k_rows) : (int)p.k_rows;
@@ -84,58 +104,107 @@ __device__ __forceinline__ bool find_doc(const Problem& p, int t, int tile_rows,
         return true;
     }
     const int32_t* off = QSIDE ? p.q_off : p.k_off;
-    const int64_t all = QSIDE ? p.q_rows : p.k_rows;
+    const int32_t* other = QSIDE ? p.k_off : p.q_off;
+    const int64_t all = QSIDE ? p.q_rows : p.k_rows, other_all = QSIDE ? p.k_rows : p.q_rows;
     const int lane = threadIdx.x & 63;
     d.batch = 0;
     d.index = -1;
     d.nq = d.nk = 0;
     d.q0 = d.k0 = 0;
     d.prefix = 0;
-    const int first = clamp_int(uniform(off[0]), 0, all);
-    const int lead = (first + tile_rows - 1) / tile_rows;
-    if (t < lead) {
-        d.tile = t;
-        d.rows = first;
+    auto found = [&](int index, int tile, int start, int rows) {
+        d.index = index;
+        d.tile = tile;
+        d.rows = rows;
+        const int os = clamp_int(uniform(other[index]), 0, other_all);
+        const int oe = clamp_int(uniform(other[index + 1]), os, other_all);
+        if (QSIDE) { d.q0 = start; d.nq = rows; d.k0 = os; d.nk = oe - os; }
+        else { d.k0 = start; d.nk = rows; d.q0 = os; d.nq = oe - os; }
+        if (p.prefix) d.prefix = uniform(p.prefix[index]);
         return true;
-    }
-    t -= lead;
+    };
+    const int first = clamp_int(uniform(off[0]), 0, all);
     int last = first;
-    for (int base = 0; base < p.n_docs; base += 64) {
-        const int i = base + lane;
-        int s = 0, e = 0;
-        if (i < p.n_docs) {
-            s = clamp_int(off[i], 0, all);
-            e = clamp_int(off[i + 1], s, all);
+    if (p.n_docs <= 64) {
+        int s = 0, e = 0, partners = 0;
+        if (lane < p.n_docs) {
+            s = clamp_int(off[lane], 0, all);
+            e = clamp_int(off[lane + 1], s, all);
+            const int os = clamp_int(other[lane], 0, other_all);
+            partners = clamp_int(other[lane + 1], os, other_all) - os;
         }
-        int sum = (e - s + tile_rows - 1) / tile_rows;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(sum, o);
-            if (lane >= o) sum += up;
-        }
-        const int total = uniform(__shfl(sum, 63));
+        if (p.n_docs > 0) last = __builtin_amdgcn_readlane(e, p.n_docs - 1);
+        const int n = (e - s + tile_rows - 1) / tile_rows;
+        const int total = wave_sum(n);
         if (t < total) {
-            const int w = uniform(__ffsll((unsigned long long)__ballot(sum > t)) - 1);
-            const int before = w ? uniform(__shfl(sum, w - 1)) : 0;
-            const int ds = uniform(__shfl(s, w)), de = uniform(__shfl(e, w));
-            d.index = base + w;
-            d.tile = t - before;
-            d.rows = de - ds;
-            const int32_t* other = QSIDE ? p.k_off : p.q_off;
-            const int64_t other_all = QSIDE ? p.k_rows : p.q_rows;
-            const int os = clamp_int(uniform(other[d.index]), 0, other_all);
-            const int oe = clamp_int(uniform(other[d.index + 1]), os, other_all);
-            if (QSIDE) { d.q0 = ds; d.nq = de - ds; d.k0 = os; d.nk = oe - os; }
-            else { d.k0 = ds; d.nk = de - ds; d.q0 = os; d.nq = oe - os; }
-            if (p.prefix) d.prefix = uniform(p.prefix[d.index]);
-            return true;
+            int w, tile;
+            if (p.causal) {
+                int lo = 0, hi = total;                   // tiles of level >= lo: more than t; of level >= hi: not more
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (wave_sum(max(0, n - mid)) > t) lo = mid;
+                    else hi = mid;
+                }
+                int rank = t - wave_sum(max(0, n - lo - 1));
+                unsigned long long has = __ballot(n > lo);
+                for (; rank > 0; --rank) has &= has - 1;
+                w = __ffsll(has) - 1;
+                tile = QSIDE ? lo : __builtin_amdgcn_readlane(n, w) - 1 - lo;
+            } else {
+                int before = 0;
+                for (int i = 0; i < p.n_docs; ++i) {
+                    const int m = __builtin_amdgcn_readlane(partners, i);
+                    if (m > partners || (m == partners && i < lane)) before += __builtin_amdgcn_readlane(n, i);
+                }
+                w = __ffsll(__ballot(before <= t && t < before + n)) - 1;
+                tile = t - __builtin_amdgcn_readlane(before, w);
+            }
+            const int ds = __builtin_amdgcn_readlane(s, w);
+            return found(w, uniform(tile), ds, __builtin_amdgcn_readlane(e, w) - ds);
         }
         t -= total;
-        const int n = p.n_docs - base < 64 ? p.n_docs - base : 64;
-        last = uniform(__shfl(e, n - 1));
+        const int lead = (first + tile_rows - 1) / tile_rows;
+        if (t < lead) {
+            d.tile = t;
+            d.rows = first;
+            return true;
+        }
+        t -= lead;
+    } else {
+        t = p.tiles - 1 - t;
+        const int lead = (first + tile_rows - 1) / tile_rows;
+        if (t < lead) {
+            d.tile = t;
+            d.rows = first;
+            return true;
+        }
+        t -= lead;
+        for (int base = 0; base < p.n_docs; base += 64) {
+            const int i = base + lane;
+            int s = 0, e = 0;
+            if (i < p.n_docs) {
+                s = clamp_int(off[i], 0, all);
+                e = clamp_int(off[i + 1], s, all);
+            }
+            int sum = (e - s + tile_rows - 1) / tile_rows;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int up = __shfl_up(sum, o);
+                if (lane >= o) sum += up;
+            }
+            const int total = __builtin_amdgcn_readlane(sum, 63);
+            if (t < total) {
+                const int w = __ffsll(__ballot(sum > t)) - 1;
+                const int before = w ? __builtin_amdgcn_readlane(sum, w - 1) : 0;
+                const int ds = __builtin_amdgcn_readlane(s, w);
+                return found(base + w, t - before, ds, __builtin_amdgcn_readlane(e, w) - ds);
+            }
+            t -= total;
+            last = __builtin_amdgcn_readlane(e, min(63, p.n_docs - 1 - base));
+        }
     }
     const int rest = (int)all - last;
-    if (rest <= 0 || t >= (rest + tile_rows - 1) / tile_rows) return false;
+    if (t >= (rest + tile_rows - 1) / tile_rows) return false;
     d.tile = t;
     d.rows = rest;
     if (QSIDE) d.q0 = last;
