@@ -346,10 +346,10 @@ typedef struct mmfe_attention_grads {
     const void* grad_out;
     void *grad_q, *grad_k, *grad_v;
     int64_t grad_out_stride[3], grad_q_stride[3], grad_k_stride[3], grad_v_stride[3];
-    float* scratch;           /* device, 2 x the size of lse, the call's own until it has run */
-    uint32_t* norms;          /* device, 2 x n_docs x kv_heads, ZEROED by the caller; float16 only (NULL otherwise) */
 } mmfe_attention_grads;
-int mmfe_attention_backward(const mmfe_attention_args* args, const mmfe_attention_grads* grads, int device, void* hip_stream);
+/* Bytes of the workspace mmfe_attention_backward needs (as mmfe_attention_workspace). */
+int64_t mmfe_attention_backward_workspace(const mmfe_attention_args* args);
+int mmfe_attention_backward(const mmfe_attention_args* args, const mmfe_attention_grads* grads, void* workspace, int device, void* hip_stream);
 
 /* ---- global norm of many tensors, and clipping by it ------------------------------------------------------------------
  * What a training step of the encoders does between backward and the optimizer (the reference's loops call the optimizer directly,

@@ -36,7 +36,7 @@ EXPORTED_SYMBOLS = (
     "mmfe_plan_kernel",
     "mmfe_patch_embed_create", "mmfe_patch_embed_destroy", "mmfe_patch_embed_shape", "mmfe_patch_embed_run", "mmfe_patch_embed_update",
     "mmfe_rotary_create", "mmfe_rotary_destroy", "mmfe_rotary_run",
-    "mmfe_attention_workspace", "mmfe_attention_forward", "mmfe_attention_backward",
+    "mmfe_attention_workspace", "mmfe_attention_forward", "mmfe_attention_backward_workspace", "mmfe_attention_backward",
     "mmfe_grad_partials", "mmfe_grad_clip",
 )
 
@@ -95,8 +95,7 @@ class AttentionArgs(ctypes.Structure):
 class AttentionGrads(ctypes.Structure):
     """mmfe_attention_grads"""
     _fields_ = [("struct_size", ctypes.c_int32), ("reserved", ctypes.c_int32)] + [(n, ctypes.c_void_p) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + [
-        (n, ctypes.c_int64 * 3) for n in ("grad_out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride")] + [
-        ("scratch", ctypes.c_void_p), ("norms", ctypes.c_void_p)]
+        (n, ctypes.c_int64 * 3) for n in ("grad_out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride")]
 
 
 def library_path() -> str:
@@ -169,7 +168,9 @@ def bind_library(path: str):
     lib.mmfe_attention_workspace.restype = c_i64
     lib.mmfe_attention_workspace.argtypes = [ctypes.POINTER(AttentionArgs)]
     lib.mmfe_attention_backward.restype = ctypes.c_int
-    lib.mmfe_attention_backward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionGrads), ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_backward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionGrads), ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_backward_workspace.restype = c_i64
+    lib.mmfe_attention_backward_workspace.argtypes = [ctypes.POINTER(AttentionArgs)]
     lib.mmfe_grad_partials.restype = c_i64
     lib.mmfe_grad_partials.argtypes = [c_i64]
     lib.mmfe_grad_clip.restype = ctypes.c_int
@@ -368,18 +369,19 @@ class RotaryHandle:
             pass
 
 
-def attention_workspace(args: AttentionArgs) -> int:
-    n = load_library().mmfe_attention_workspace(ctypes.byref(args))
-    check(0 if n >= 0 else -1, "mmfe_attention_workspace")
-    return n
-
-
 def attention_forward(args: AttentionArgs, workspace_ptr: int, device: int, stream: int) -> None:
     check(load_library().mmfe_attention_forward(ctypes.byref(args), workspace_ptr or None, device, stream or None), "mmfe_attention_forward")
 
 
-def attention_backward(args: AttentionArgs, grads: AttentionGrads, device: int, stream: int) -> None:
-    check(load_library().mmfe_attention_backward(ctypes.byref(args), ctypes.byref(grads), device, stream or None), "mmfe_attention_backward")
+def attention_workspace(args: AttentionArgs, backward: bool = False) -> int:
+    lib = load_library()
+    n = (lib.mmfe_attention_backward_workspace if backward else lib.mmfe_attention_workspace)(ctypes.byref(args))
+    check(0 if n >= 0 else -1, "mmfe_attention_workspace")
+    return n
+
+
+def attention_backward(args: AttentionArgs, grads: AttentionGrads, workspace_ptr: int, device: int, stream: int) -> None:
+    check(load_library().mmfe_attention_backward(ctypes.byref(args), ctypes.byref(grads), workspace_ptr or None, device, stream or None), "mmfe_attention_backward")
 
 
 def grad_partials(n: int) -> int:

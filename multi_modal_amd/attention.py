@@ -101,11 +101,11 @@ class _AttentionFn(torch.autograd.Function):
         call = ctx.call
         g = _rows(grad_out)
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        scratch = torch.empty((2,) + tuple(lse.shape), dtype=torch.float32, device=q.device)
-        norms = torch.zeros(2 * call.n_docs * k.shape[-2], dtype=torch.int32, device=q.device) if q.dtype == torch.float16 else None
         grads = N.AttentionGrads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _strides(g), _strides(gq), _strides(gk),
-                                 _strides(gv), scratch.data_ptr(), _ptr(norms))
-        N.attention_backward(call.args(q, k, v, out, rest, lse), grads, q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+                                 _strides(gv))
+        args = call.args(q, k, v, out, rest, lse)
+        work = torch.empty(N.attention_workspace(args, backward=True), dtype=torch.uint8, device=q.device)
+        N.attention_backward(args, grads, work.data_ptr(), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None
 

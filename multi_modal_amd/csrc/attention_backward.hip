@@ -39,99 +39,117 @@ struct BackwardArgs {
     const float* lse;
     float *lse2, *delta;              // like lse: lse in log2 units (less the shift of p; +inf for rows without keys), g . o
     int64_t lse_b, lse_h;
-    unsigned *norm_g, *norm_v;        // float16: largest squared row norms, per document and key head (bit patterns of floats >= 0)
+    float *norm_g, *norm_v;           // float16: largest squared row norm of each 128-row tile, (heads, q_slots) and (kv_heads, k_slots)
+    int q_slots, k_slots, q_tiles, k_tiles, q_blocks;
 };
 
 template <bool BF>
 constexpr float kShift = BF ? 0.f : 8.f;
 
-__device__ __forceinline__ void block_max(float v, unsigned* to) {
-    __shared__ float m[kWaves];
+// Place of a document's tile among the norms: one place per tile, in a document's order, without a table.  Packed documents may share
+// a 128-row stretch with their neighbours, one place is added per document before them.
+__device__ __forceinline__ int64_t slot(const Problem& p, const Doc& d, bool qside, int tile) {
+    if (p.packed) return ((qside ? d.q0 : d.k0) >> 7) + d.index + tile;
+    return (int64_t)d.batch * (((qside ? p.q_rows : p.k_rows) + kRows - 1) / kRows) + tile;
+}
+
+__device__ __forceinline__ float block_max(float v, float* lds) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    if ((threadIdx.x & 63) == 0) m[threadIdx.x >> 6] = v;
+    for (int o = 32; o > 0; o >>= 1) v = max2(v, __shfl_xor(v, o));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    if (threadIdx.x == 0) atomicMax(to, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));     // a maximum has no order
+    float m = lds[0];
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) m = max2(m, lds[w]);
+    __syncthreads();
+    return m;
 }
 
-// delta and lse2 of 128 rows of one head; float16: and the rows' largest gradient norm.  DP / 8 lanes share a row.
+// What both passes need of every row: delta and lse2 (blocks below q_blocks, 128 rows of one head each), and for float16 the tiles' largest
+// squared norms of g and, in the blocks behind, of v.  DP / 8 lanes share a row.
 template <bool BF, int DP>
-__global__ void __launch_bounds__(kThreads) delta_kernel(const BackwardArgs a) {
-    const Problem& p = a.p;
-    Doc d;
-    if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
-    const int head = blockIdx.x % p.heads;
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const BackwardArgs a) {
+    __shared__ float lds[kWaves];
+    Problem p = a.p;
     constexpr int kLanes = DP / 8;
     const int e = (threadIdx.x & (kLanes - 1)) * 8;
-    float biggest = 0.f;
-    for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
-        const int row = d.tile * kRows + r;
-        float dot = 0.f, sq = 0.f;
-        if (row < d.nq && e < p.dim) {
-            const int64_t at = 2 * (d.batch * a.out.b + (d.q0 + row) * a.out.n + head * a.out.h + e);
-            const u32x4 o = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.out.p) + at);
-            u32x4 rest{0, 0, 0, 0};
-            if (a.rest != nullptr) rest = *reinterpret_cast<const u32x4*>(a.rest + at);
-            const u32x4 g = *reinterpret_cast<const u32x4*>(row_base(a.g, d, d.q0 + row, head) + 2 * e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = widen<BF>(g[i >> 1], i & 1);
-                dot = fmaf(x, widen<BF>(o[i >> 1], i & 1) + widen<BF>(rest[i >> 1], i & 1), dot);
-                if constexpr (!BF) sq = fmaf(x, x, sq);
-            }
-        }
-#pragma unroll
-        for (int m = 1; m < kLanes; m <<= 1) {
-            dot += __shfl_xor(dot, m);
-            if constexpr (!BF) sq += __shfl_xor(sq, m);
-        }
-        biggest = fmaxf(biggest, sq);
-        if (row < d.nq && e == 0) {
-            const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + row;
-            const float l = a.lse[at];
-            a.lse2[at] = l == -INFINITY ? INFINITY : l * kLog2e - kShift<BF>;
-            a.delta[at] = l == -INFINITY ? 0.f : dot;
-        }
-    }
-    if constexpr (!BF)
-        if (d.index >= 0) block_max(biggest, a.norm_g + (int64_t)d.index * p.kv_heads + head / p.group);
-}
-
-// float16: largest squared norm of 128 rows of v
-template <int DP>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const BackwardArgs a) {
-    const Problem& p = a.p;
     Doc d;
-    if (!find_doc<false>(p, blockIdx.x / p.kv_heads, kRows, d) || d.index < 0) return;
-    const int head = blockIdx.x % p.kv_heads;
-    constexpr int kLanes = DP / 8;
-    const int e = (threadIdx.x & (kLanes - 1)) * 8;
     float biggest = 0.f;
-    for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
-        const int row = d.tile * kRows + r;
-        float sq = 0.f;
-        if (row < d.nk && e < p.dim) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(row_base(p.v, d, d.k0 + row, head) + 2 * e);
+    if ((int)blockIdx.x < a.q_blocks) {
+        p.tiles = a.q_tiles;
+        if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
+        const int head = blockIdx.x % p.heads;
+        for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
+            const int row = d.tile * kRows + r;
+            float dot = 0.f, sq = 0.f;
+            if (row < d.nq && e < p.dim) {
+                const int64_t at = 2 * (d.batch * a.out.b + (d.q0 + row) * a.out.n + head * a.out.h + e);
+                const u32x4 o = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.out.p) + at);
+                u32x4 rest{0, 0, 0, 0};
+                if (a.rest != nullptr) rest = *reinterpret_cast<const u32x4*>(a.rest + at);
+                const u32x4 g = *reinterpret_cast<const u32x4*>(row_base(a.g, d, d.q0 + row, head) + 2 * e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = widen<false>(v[i >> 1], i & 1);
-                sq = fmaf(x, x, sq);
+                for (int i = 0; i < 8; ++i) {
+                    const float x = widen<BF>(g[i >> 1], i & 1);
+                    dot = fmaf(x, widen<BF>(o[i >> 1], i & 1) + widen<BF>(rest[i >> 1], i & 1), dot);
+                    if constexpr (!BF) sq = fmaf(x, x, sq);
+                }
+            }
+#pragma unroll
+            for (int m = 1; m < kLanes; m <<= 1) {
+                dot += __shfl_xor(dot, m);
+                if constexpr (!BF) sq += __shfl_xor(sq, m);
+            }
+            biggest = max2(biggest, sq);
+            if (row < d.nq && e == 0) {
+                const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + row;
+                const float l = a.lse[at];
+                a.lse2[at] = l == -INFINITY ? INFINITY : l * kLog2e - kShift<BF>;
+                a.delta[at] = l == -INFINITY ? 0.f : dot;
             }
         }
+        if constexpr (!BF) {
+            biggest = block_max(biggest, lds);
+            if (d.index >= 0 && threadIdx.x == 0) a.norm_g[(int64_t)head * a.q_slots + slot(p, d, true, d.tile)] = biggest;
+        }
+    } else if constexpr (!BF) {
+        p.tiles = a.k_tiles;
+        const int block = blockIdx.x - a.q_blocks;
+        if (!find_doc<false>(p, block / p.kv_heads, kRows, d) || d.index < 0) return;
+        const int head = block % p.kv_heads;
+        for (int r = threadIdx.x / kLanes; r < kRows; r += kThreads / kLanes) {
+            const int row = d.tile * kRows + r;
+            float sq = 0.f;
+            if (row < d.nk && e < p.dim) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(row_base(p.v, d, d.k0 + row, head) + 2 * e);
 #pragma unroll
-        for (int m = 1; m < kLanes; m <<= 1) sq += __shfl_xor(sq, m);
-        biggest = fmaxf(biggest, sq);
+                for (int i = 0; i < 8; ++i) {
+                    const float x = widen<false>(v[i >> 1], i & 1);
+                    sq = fmaf(x, x, sq);
+                }
+            }
+#pragma unroll
+            for (int m = 1; m < kLanes; m <<= 1) sq += __shfl_xor(sq, m);
+            biggest = max2(biggest, sq);
+        }
+        biggest = block_max(biggest, lds);
+        if (threadIdx.x == 0) a.norm_v[(int64_t)head * a.k_slots + slot(p, d, false, d.tile)] = biggest;
     }
-    block_max(biggest, a.norm_v + (int64_t)d.index * p.kv_heads + head);
 }
 
+// phi of a document and key head, from its tiles' norms; called by the whole block.
 template <bool BF>
-__device__ __forceinline__ float find_phi(const BackwardArgs& a, const Doc& d, int kvh) {
+__device__ __forceinline__ float find_phi(const BackwardArgs& a, const Doc& d, int kvh, float* lds) {
     if constexpr (BF) return 1.f;
     else {
         if (d.index < 0) return 1.f;
-        const int64_t i = (int64_t)d.index * a.p.kv_heads + kvh;
-        const float bound = sqrtf(__uint_as_float(a.norm_g[i])) * sqrtf(__uint_as_float(a.norm_v[i]));
+        float g = 0.f, v = 0.f;
+        const int tq = (d.nq + kRows - 1) / kRows, tk = (d.nk + kRows - 1) / kRows;
+        const float* ng = a.norm_g + slot(a.p, d, true, 0) + (int64_t)kvh * a.p.group * a.q_slots;
+        for (int h = 0; h < a.p.group; ++h)
+            for (int i = threadIdx.x; i < tq; i += blockDim.x) g = max2(g, ng[(int64_t)h * a.q_slots + i]);
+        const float* nv = a.norm_v + slot(a.p, d, false, 0) + (int64_t)kvh * a.k_slots;
+        for (int i = threadIdx.x; i < tk; i += blockDim.x) v = max2(v, nv[i]);
+        const float bound = sqrtf(block_max(g, lds)) * sqrtf(block_max(v, lds));
         if (!(bound > 0.f) || !(bound < 3e38f)) return 1.f;
         int e;
         (void)frexpf(bound, &e);                       // bound < 2^e
@@ -140,16 +158,30 @@ __device__ __forceinline__ float find_phi(const BackwardArgs& a, const Doc& d, i
 }
 
 // How scores leave the linear form, in log2 units.
+template <bool CAP>
 struct Shape {
-    bool cap, bias;
+    bool bias;
     float c, slope, cap_in, cap_out;
-    __device__ __forceinline__ Shape(const Problem& p, int head) {
-        cap = p.cap > 0.f;
+    __device__ __forceinline__ void set(const Problem& p, int head) {
         bias = p.slopes != nullptr;
         c = p.scale * kLog2e;
         slope = bias ? p.slopes[head] * kLog2e : 0.f;
-        cap_in = cap ? p.scale / p.cap : 0.f;
+        cap_in = CAP ? p.scale / p.cap : 0.f;
         cap_out = p.cap * kLog2e;
+    }
+    // products to scores in log2 units; th: the tanh of capped ones.  at: distance of register row 0, step: its sign per row
+    __device__ __forceinline__ void apply(f32x16& x, f32x16& th, float at, float step) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (CAP) {
+                th[i] = tanh_fast(x[i] * cap_in);
+                x[i] = cap_out * th[i];
+            } else x[i] *= c;
+        }
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = fmaf(-slope, fabsf(at + step * (float)reg_row(i)), x[i]);
+        }
     }
 };
 
@@ -162,15 +194,13 @@ __device__ __forceinline__ void store_rows(char* to, const f32x16 (&o)[DP / 32],
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int e = 32 * i + 8 * g;
-            if (e < dim) {
-                u32x2 w{0, 0};
-                if (some) w = u32x2{pack2<BF>(o[i][4 * g] * by, o[i][4 * g + 1] * by), pack2<BF>(o[i][4 * g + 2] * by, o[i][4 * g + 3] * by)};
-                *reinterpret_cast<u32x2*>(to + 2 * (e + 4 * half)) = w;
-            }
+            if (e >= dim) continue;
+            if (some) store4<BF>(to + 2 * (e + 4 * half), nullptr, o[i][4 * g] * by, o[i][4 * g + 1] * by, o[i][4 * g + 2] * by, o[i][4 * g + 3] * by);
+            else store4<BF>(to + 2 * (e + 4 * half), nullptr, 0.f, 0.f, 0.f, 0.f);
         }
 }
 
-template <bool BF, int DP>
+template <int DP>
 __device__ __forceinline__ void load_rows(u32x4 (&f)[DP / 16], const char* row, int dim, bool some) {
     const int half = (threadIdx.x >> 5) & 1;
 #pragma unroll
@@ -180,21 +210,41 @@ __device__ __forceinline__ void load_rows(u32x4 (&f)[DP / 16], const char* row, 
     }
 }
 
-// dk and dv of 128 keys, 32 per wave.  Head sizes up to 64: 8 waves, the second four taking the second 32 rows of every tile, whose sums join
-// the first four's through LDS at the end; a block then takes half as long, and the longest one (4096 keys of a causal document,
-// three heads' rows behind it) bounds the launch: FIXME.  Head size 128 has no registers for that.
-template <int DP>
-constexpr int kKeyWaves = DP == 128 ? 4 : 8;
-
+// acc += columns of a tile's 32 rows from row0 on, times x: what the short documents' rounding lost goes in as a second product
 template <bool BF, int DP>
-__global__ void __launch_bounds__(64 * kKeyWaves<DP>, 1) keys_kernel(const BackwardArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // 2 x [q tile][g tile][lse2][delta]
+__device__ __forceinline__ void accumulate(f32x16 (&acc)[DP / 32], const char* tile, int row0, const f32x16& x, bool both) {
+    u32x4 f[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        f[s] = operand<BF>(x, s);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) acc[i] = mfma<BF>(read_cols<DP>(tile, row0 + 16 * s, 32 * i), f[s], acc[i]);
+    }
+    if (both)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const u32x4 r = operand_rest<BF>(x, s, f[s]);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) acc[i] = mfma<BF>(read_cols<DP>(tile, row0 + 16 * s, 32 * i), r, acc[i]);
+        }
+}
+
+constexpr int64_t kLongWalk = 2048;   // rows of a key head's queries from which keys_kernel has eight waves
+constexpr int kRing = 4;              // tiles in LDS: the one in use, the next one's scores, two on their way
+
+// dk and dv of 128 keys, 32 per wave, over tiles of 64 rows.  Step u turns the scores of its rows (computed a step earlier) into p and
+// ds beside the products of the next rows, then adds them to dv and dk; its tiles stay until then, and it asks for those of step u + 3.
+// W = 8 waves: the second four take the second 32 rows of every tile and their sums join the first four's through LDS at the
+// end.  A block then takes half as long and one fits a CU instead of two: better where the longest block bounds the launch (FIXME).
+template <bool BF, int DP, bool CAP, int W>
+__global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kernel(const BackwardArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][lse2][delta]
     const Problem& p = a.p;
     constexpr int kTileBytes = kTile * DP * 2;
     constexpr int kBuf = 2 * kTileBytes + 2 * kTile * 4;
-    constexpr int kW = kKeyWaves<DP>;
+    constexpr int kParts = W == 8 ? 1 : 2;                            // 32-row parts of a tile that a wave takes
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int part = wave >> 2;                                       // which of the tile's 32 rows (8 waves)
+    const int part = W == 8 ? wave >> 2 : 0;
     const int kvh = blockIdx.x % p.kv_heads;
     Doc d;
     if (!find_doc<false>(p, blockIdx.x / p.kv_heads, kRows, d)) return;
@@ -207,124 +257,105 @@ __global__ void __launch_bounds__(64 * kKeyWaves<DP>, 1) keys_kernel(const Backw
     const int wave_full = first_row(min(w0 + 31, nk - 1));            // from here on every row sees all keys of the wave
     const int my_first = first_row(key);
     const int t_first = block_first / kTile, t_end = block_first < nq ? (nq + kTile - 1) / kTile : t_first;
-    const int per_head = t_end - t_first, steps = per_head * p.group;
+    const int steps = (t_end - t_first) * p.group;
 
-    Loader<DP, kTile, kW> lq, lg;
+    typedef Loader<DP, kTile, W> Load;
+    Load lq, lg;
     lq.init(p.dim, p.q.n, wave);
     lg.init(p.dim, a.g.n, wave);
     const unsigned lds0 = lds_address(smem);
-    auto stage = [&](int g, int t, int buf) {
-        const int head = kvh * p.group + g, r0 = t * kTile;
-        const unsigned dst = uniform(lds0 + buf * kBuf);
+    int ask_g = 0, ask_t = t_first, ask = 0;                          // the next tile to ask for
+    auto stage = [&]() {
+        const int head = kvh * p.group + ask_g, r0 = ask_t * kTile;
+        const unsigned dst = uniform(lds0 + (ask % kRing) * kBuf);
         lq.load(row_base(p.q, d, d.q0 + r0, head), nq - r0, p.dim, p.q.n, dst, wave);
         lg.load(row_base(a.g, d, d.q0 + r0, head), nq - r0, p.dim, a.g.n, dst + kTileBytes, wave);
         const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + r0;
         const unsigned mine = 4 * min(lane, nq - 1 - r0);
         if (wave == 0) dma4(a.lse2 + at, mine, dst + 2 * kTileBytes);
         if (wave == 1) dma4(a.delta + at, mine, dst + 2 * kTileBytes + kTile * 4);
+        ++ask;
+        if (++ask_t == t_end) { ask_t = t_first; ++ask_g; }
     };
-    if (steps > 0) stage(0, t_first, 0);
     u32x4 kf[DP / 16], vf[DP / 16];
     {
         const int r = max(0, min(key, nk - 1));
-        load_rows<BF, DP>(kf, row_base(p.k, d, d.k0 + r, kvh), p.dim, nk > 0);
-        load_rows<BF, DP>(vf, row_base(p.v, d, d.k0 + r, kvh), p.dim, nk > 0);
+        load_rows<DP>(kf, row_base(p.k, d, d.k0 + r, kvh), p.dim, nk > 0);
+        load_rows<DP>(vf, row_base(p.v, d, d.k0 + r, kvh), p.dim, nk > 0);
     }
-    const float phi = find_phi<BF>(a, d, kvh);
-    f32x16 dk[DP / 32], dv[DP / 32];
+    const float phi = find_phi<BF>(a, d, kvh, reinterpret_cast<float*>(smem));
+    for (int i = 0; i < kRing - 1 && i < steps; ++i) stage();
+    f32x16 dk[DP / 32], dv[DP / 32], x{}, dp{};
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
-
+    // scores and dp of 32 rows: register rows are rows, a lane has one key
+    auto products = [&](const char* qt, int b, f32x16& sx, f32x16& sd) {
+        sx = f32x16{};
+        sd = f32x16{};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sx = mfma<BF>(read_rows<DP>(qt, 32 * b, s), kf[s], sx);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sd = mfma<BF>(read_rows<DP>(qt + kTileBytes, 32 * b, s), vf[s], sd);
+    };
     wait_all();
+    block_sync();
     arrived(kf);
     arrived(vf);
+    if (steps > 0) products(smem, part, x, dp);
+    Shape<CAP> sh;
+    sh.set(p, kvh * p.group);
     int g = 0, t = t_first;
     for (int step = 0; step < steps; ++step) {
-        wait_all();
+        if (step + kRing - 2 < steps) wait_but<2 * Load::kCount>();   // tile step + 1 is there; what step - 1 asked for may be on its way
+        else wait_all();
         block_sync();
-        int gn = g, tn = t + 1;
-        if (tn == t_end) { tn = t_first; ++gn; }
-        if (step + 1 < steps) stage(gn, tn, (step + 1) & 1);
-        const char* qt = smem + (step & 1) * kBuf;
+        if (step + kRing - 1 < steps) stage();
+        const char* qt = smem + (step % kRing) * kBuf;
+        const char* next = smem + ((step + 1) % kRing) * kBuf;
         const char* gt = qt + kTileBytes;
         const float* lse2 = reinterpret_cast<const float*>(gt + kTileBytes);
         const float* delta = lse2 + kTile;
-        const Shape sh(p, kvh * p.group + g);
-#pragma unroll 1
-        for (int b = kW == 8 ? part : 0; b < (kW == 8 ? part + 1 : 2); ++b) {
-            const int i0 = t * kTile + 32 * b;
-            if (i0 + 32 <= wave_first || i0 >= nq) continue;
-            f32x16 x{}, dp{};
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) x = mfma<BF>(read_rows<DP>(qt, 32 * b, s), kf[s], x);
+        for (int b0 = 0; b0 < kParts; ++b0) {
+            const int b = part + b0, i0 = t * kTile + 32 * b;
+            const bool live = i0 + 32 > wave_first && i0 < nq;
+            f32x16 th;
+            if (live) {
+                sh.apply(x, th, (float)(i0 + 4 * half + off - key), 1.f);
+                if (i0 < wave_full || i0 + 32 > nq) {
+                    const int lo = my_first - i0 - 4 * half, hi = nq - i0 - 4 * half;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) dp = mfma<BF>(read_rows<DP>(gt, 32 * b, s), vf[s], dp);
-            f32x16 th{};
-            if (sh.cap) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    th[i] = tanh_fast(x[i] * sh.cap_in);
-                    x[i] = sh.cap_out * th[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] *= sh.c;
-            }
-            if (sh.bias) {
-                const float at = (float)(i0 + 4 * half + off - key);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] -= sh.slope * fabsf(at + (float)reg_row(i));
-            }
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const float4 l4 = *reinterpret_cast<const float4*>(lse2 + 32 * b + 8 * q4 + 4 * half);
-                const float4 d4 = *reinterpret_cast<const float4*>(delta + 32 * b + 8 * q4 + 4 * half);
-                const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 4 * q4 + r;
-                    x[i] = exp2_fast(x[i] - l[r]);
-                    dp[i] = fmaf(dp[i], phi, -de[r] * phi);
+                    for (int i = 0; i < 16; ++i) x[i] = reg_row(i) >= lo && reg_row(i) < hi ? x[i] : -INFINITY;
                 }
             }
-            if (i0 < wave_full || i0 + 32 > nq) {
-                const int lo = my_first - i0 - 4 * half, hi = nq - i0 - 4 * half;
+            f32x16 nx, nd;
+            products(b0 + 1 < kParts ? qt : next, b0 + 1 < kParts ? b + 1 : part, nx, nd);
+            if (live) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = reg_row(i) >= lo && reg_row(i) < hi ? x[i] : 0.f;
-            }
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const float4 l4 = *reinterpret_cast<const float4*>(lse2 + 32 * b + 8 * q4 + 4 * half);
+                    const float4 d4 = *reinterpret_cast<const float4*>(delta + 32 * b + 8 * q4 + 4 * half);
+                    const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u32x4 pf = operand<BF>(x, s);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dv[i] = mfma<BF>(read_cols<DP>(gt, 32 * b + 16 * s, 32 * i), pf, dv[i]);
-                if (nk <= kShortKeys) {
-                    const u32x4 rf = operand_rest<BF>(x, s, pf);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) dv[i] = mfma<BF>(read_cols<DP>(gt, 32 * b + 16 * s, 32 * i), rf, dv[i]);
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 4 * q4 + r;
+                        x[i] = exp2_fast(x[i] - l[r]);
+                        dp[i] = fmaf(dp[i], phi, -de[r] * phi) * x[i];
+                        if constexpr (CAP) dp[i] *= 1.f - th[i] * th[i];
+                    }
                 }
+                accumulate<BF, DP>(dv, gt, 32 * b, x, nk <= kShortKeys);
+                accumulate<BF, DP>(dk, qt, 32 * b, dp, nk <= kShortKeys);
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] *= dp[i];
-            if (sh.cap) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] *= 1.f - th[i] * th[i];
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u32x4 df = operand<BF>(x, s);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dk[i] = mfma<BF>(read_cols<DP>(qt, 32 * b + 16 * s, 32 * i), df, dk[i]);
-                if (nk <= kShortKeys) {
-                    const u32x4 rf = operand_rest<BF>(x, s, df);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) dk[i] = mfma<BF>(read_cols<DP>(qt, 32 * b + 16 * s, 32 * i), rf, dk[i]);
-                }
-            }
+            x = nx;
+            dp = nd;
         }
-        g = gn;
-        t = tn;
+        if (++t == t_end) {
+            t = t_first;
+            if (++g < p.group) sh.set(p, kvh * p.group + g);
+        }
     }
-    if constexpr (kW == 8) {
+    if constexpr (W == 8) {
         wait_all();
         block_sync();
         float* meet = reinterpret_cast<float*>(smem) + (wave & 3) * (DP / 32) * 2 * 16 * 64 + lane;
@@ -352,12 +383,13 @@ __global__ void __launch_bounds__(64 * kKeyWaves<DP>, 1) keys_kernel(const Backw
     store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, d.k0 + key, kvh)), dv, p.dim, back, key < nk && steps > 0);
 }
 
-// dq of 128 rows (32 per wave)
-template <bool BF, int DP>
+// dq of 128 rows, 32 per wave, over tiles of 32 keys; steps overlap as in keys_kernel.
+template <bool BF, int DP, bool CAP>
 __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // 2 x [k tile][v tile]
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [k tile][v tile]
     const Problem& p = a.p;
-    constexpr int kTileBytes = kTile * DP * 2;
+    constexpr int kKeys = 32;
+    constexpr int kTileBytes = kKeys * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     Doc d;
     if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
@@ -372,118 +404,122 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
     const int wave_lim = w0 < nq ? limit(w0 + 31) : 0;
     const int full_lim = w0 < nq ? limit(w0) : 0;
     const int lim = row < nq ? limit(row) : 0;
-    const int n_tiles = block_lim > 0 ? (block_lim + kTile - 1) / kTile : 0;
+    const int n = block_lim > 0 ? (block_lim + kKeys - 1) / kKeys : 0;
 
-    Loader<DP, kTile, kWaves> lk, lv;
+    typedef Loader<DP, kKeys, kWaves> Load;
+    Load lk, lv;
     lk.init(p.dim, p.k.n, wave);
     lv.init(p.dim, p.v.n, wave);
     const unsigned lds0 = lds_address(smem);
-    auto stage = [&](int t, int buf) {
-        const unsigned dst = uniform(lds0 + buf * 2 * kTileBytes);
-        lk.load(row_base(p.k, d, d.k0 + (int64_t)t * kTile, kvh), nk - t * kTile, p.dim, p.k.n, dst, wave);
-        lv.load(row_base(p.v, d, d.k0 + (int64_t)t * kTile, kvh), nk - t * kTile, p.dim, p.v.n, dst + kTileBytes, wave);
+    auto stage = [&](int t) {
+        const unsigned dst = uniform(lds0 + (t % kRing) * 2 * kTileBytes);
+        lk.load(row_base(p.k, d, d.k0 + (int64_t)t * kKeys, kvh), nk - t * kKeys, p.dim, p.k.n, dst, wave);
+        lv.load(row_base(p.v, d, d.k0 + (int64_t)t * kKeys, kvh), nk - t * kKeys, p.dim, p.v.n, dst + kTileBytes, wave);
     };
-    if (n_tiles > 0) stage(0, 0);
     u32x4 qf[DP / 16], gf[DP / 16];
     const int r = max(0, min(row, nq - 1));
-    load_rows<BF, DP>(qf, row_base(p.q, d, d.q0 + r, head), p.dim, nq > 0);
-    load_rows<BF, DP>(gf, row_base(a.g, d, d.q0 + r, head), p.dim, nq > 0);
+    load_rows<DP>(qf, row_base(p.q, d, d.q0 + r, head), p.dim, nq > 0);
+    load_rows<DP>(gf, row_base(a.g, d, d.q0 + r, head), p.dim, nq > 0);
     const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + r;
-    const float phi = find_phi<BF>(a, d, kvh);
-    const float lse2 = nq > 0 ? a.lse2[at] : 0.f;
-    const float delta = nq > 0 ? -a.delta[at] * phi : 0.f;
-    const Shape sh(p, head);
-    f32x16 dq[DP / 32];
+    const float phi = find_phi<BF>(a, d, kvh, reinterpret_cast<float*>(smem));
+    float lse2 = nq > 0 ? a.lse2[at] : 0.f;
+    float delta = nq > 0 ? -a.delta[at] * phi : 0.f;
+    Shape<CAP> sh;
+    sh.set(p, head);
+    for (int i = 0; i < kRing - 1 && i < n; ++i) stage(i);
+    f32x16 dq[DP / 32], x{}, dp{};
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dq[i] = f32x16{};
-
+    auto products = [&](const char* kt, f32x16& sx, f32x16& sd) {
+        sx = f32x16{};
+        sd = f32x16{};
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sx = mfma<BF>(read_rows<DP>(kt, 0, s), qf[s], sx);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sd = mfma<BF>(read_rows<DP>(kt + kTileBytes, 0, s), gf[s], sd);
+    };
     wait_all();
+    block_sync();
     arrived(qf);
     arrived(gf);
-    for (int t = 0; t < n_tiles; ++t) {
-        wait_all();
+    asm volatile("" : "+v"(lse2), "+v"(delta));
+    if (wave_lim > 0) products(smem, x, dp);
+    for (int t = 0; t < n; ++t) {
+        if (t + kRing - 2 < n) wait_but<2 * Load::kCount>();
+        else wait_all();
         block_sync();
-        if (t + 1 < n_tiles) stage(t + 1, (t + 1) & 1);
-        const char* kt = smem + (t & 1) * 2 * kTileBytes;
-        const char* vt = kt + kTileBytes;
-#pragma unroll 1
-        for (int b = 0; b < 2; ++b) {
-            const int j0 = t * kTile + 32 * b;
-            if (j0 >= wave_lim) break;
-            f32x16 x{}, dp{};
+        if (t + kRing - 1 < n) stage(t + kRing - 1);
+        const int j0 = t * kKeys;
+        if (j0 >= wave_lim) continue;
+        const char* kt = smem + (t % kRing) * 2 * kTileBytes;
+        f32x16 th;
+        sh.apply(x, th, (float)(row + off - j0 - 4 * half), -1.f);
+        if (j0 + kKeys > full_lim) {
+            const int left = lim - j0 - 4 * half;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) x = mfma<BF>(read_rows<DP>(kt, 32 * b, s), qf[s], x);
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) dp = mfma<BF>(read_rows<DP>(vt, 32 * b, s), gf[s], dp);
-            f32x16 th{};
-            if (sh.cap) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    th[i] = tanh_fast(x[i] * sh.cap_in);
-                    x[i] = sh.cap_out * th[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] *= sh.c;
-            }
-            if (sh.bias) {
-                const float far = (float)(row + off - j0 - 4 * half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] -= sh.slope * fabsf(far - (float)reg_row(i));
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = exp2_fast(x[i] - lse2);
-                dp[i] = fmaf(dp[i], phi, delta);
-            }
-            if (j0 + 32 > full_lim) {
-                const int left = lim - j0 - 4 * half;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = reg_row(i) < left ? x[i] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] *= dp[i];
-            if (sh.cap) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] *= 1.f - th[i] * th[i];
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u32x4 df = operand<BF>(x, s);
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) dq[i] = mfma<BF>(read_cols<DP>(kt, 32 * b + 16 * s, 32 * i), df, dq[i]);
-                if (nk <= kShortKeys) {
-                    const u32x4 rf = operand_rest<BF>(x, s, df);
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) dq[i] = mfma<BF>(read_cols<DP>(kt, 32 * b + 16 * s, 32 * i), rf, dq[i]);
-                }
-            }
+            for (int i = 0; i < 16; ++i) x[i] = reg_row(i) < left ? x[i] : -INFINITY;
         }
+        f32x16 nx, nd;
+        products(smem + ((t + 1) % kRing) * 2 * kTileBytes, nx, nd);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            dp[i] = fmaf(dp[i], phi, delta) * exp2_fast(x[i] - lse2);
+            if constexpr (CAP) dp[i] *= 1.f - th[i] * th[i];
+        }
+        accumulate<BF, DP>(dq, kt, 0, dp, nk <= kShortKeys);
+        x = nx;
+        dp = nd;
     }
+    wait_all();
     if (row >= d.rows) return;
     store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi, lim > 1);       // a softmax over one key is constant
 }
 
-template <bool BF, int DP>
-int launch(BackwardArgs& b, int64_t q_rows, int64_t k_rows, hipStream_t stream) {
+template <bool BF, int DP, bool CAP>
+int launch(BackwardArgs& b, hipStream_t stream) {
     Problem& p = b.p;
     int rc = MMFE_OK, blocks = 1, cus = 256;
-    const size_t tiles_lds = 4 * (size_t)kTile * DP * 2, meet_lds = 4 * (size_t)(DP / 32) * 2 * 16 * 64 * 4;
-    const size_t keys_lds = kKeyWaves<DP> == 8 && meet_lds > tiles_lds + 4 * kTile * 4 ? meet_lds : tiles_lds + 4 * kTile * 4;
-    if ((rc = kernel_prepare(reinterpret_cast<const void*>(&keys_kernel<BF, DP>), 64 * kKeyWaves<DP>, keys_lds, &blocks, &cus)) != MMFE_OK) return rc;
-    if ((rc = kernel_prepare(reinterpret_cast<const void*>(&rows_kernel<BF, DP>), kThreads, tiles_lds, &blocks, &cus)) != MMFE_OK) return rc;
-    const int64_t tq = count_tiles(p, q_rows, kRows);
-    const int q_tiles = p.tiles;
-    if (tq > 0) hipLaunchKernelGGL((delta_kernel<BF, DP>), dim3((uint32_t)(tq * p.heads)), dim3(kThreads), 0, stream, b);
-    const int64_t tk = count_tiles(p, k_rows, kRows);
+    const int64_t tk = count_tiles(p, p.k_rows, kRows);
+    b.k_tiles = p.tiles;
+    const int64_t tq = count_tiles(p, p.q_rows, kRows);
+    b.q_tiles = p.tiles;
+    b.q_blocks = (int)(tq * p.heads);
+    const int64_t norms = BF ? 0 : tk * p.kv_heads;
+    if (b.q_blocks + norms > 0) hipLaunchKernelGGL((prepare_kernel<BF, DP>), dim3((uint32_t)(b.q_blocks + norms)), dim3(kThreads), 0, stream, b);
     if (tk > 0) {
-        if constexpr (!BF) hipLaunchKernelGGL((norm_kernel<DP>), dim3((uint32_t)(tk * p.kv_heads)), dim3(kThreads), 0, stream, b);
-        hipLaunchKernelGGL((keys_kernel<BF, DP>), dim3((uint32_t)(tk * p.kv_heads)), dim3(64 * kKeyWaves<DP>), keys_lds, stream, b);
+        // eight waves where a block's walk over the rows is long and its length, not the number of blocks, bounds the launch
+        p.tiles = b.k_tiles;
+        const bool wide = DP < 128 && p.q_rows * p.group >= kLongWalk;
+        constexpr int W = DP < 128 ? 8 : 4;
+        const auto fn = wide ? &keys_kernel<BF, DP, CAP, W> : &keys_kernel<BF, DP, CAP, 4>;
+        const size_t tiles = kRing * (2 * (size_t)kTile * DP * 2 + 2 * kTile * 4), meet = 4 * (size_t)(DP / 32) * 2 * 16 * 64 * 4;
+        const size_t lds = wide && meet > tiles ? meet : tiles;
+        const int threads = 64 * (wide ? W : 4);
+        if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), threads, lds, &blocks, &cus)) != MMFE_OK) return rc;
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads)), dim3(threads), lds, stream, b);
     }
-    p.tiles = q_tiles;
-    if (tq > 0) hipLaunchKernelGGL((rows_kernel<BF, DP>), dim3((uint32_t)(tq * p.heads)), dim3(kThreads), tiles_lds, stream, b);
+    if (tq > 0) {
+        p.tiles = b.q_tiles;
+        const auto fn = &rows_kernel<BF, DP, CAP>;
+        const size_t lds = kRing * 2 * (size_t)32 * DP * 2;
+        if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(tq * p.heads)), dim3(kThreads), lds, stream, b);
+    }
     return launched("attention backward");
 }
+
+template <bool BF, bool CAP>
+int launch_dim(BackwardArgs& b, hipStream_t stream) {
+    const int dp = padded_dim(b.p.dim);
+    return dp == 32 ? launch<BF, 32, CAP>(b, stream) : dp == 64 ? launch<BF, 64, CAP>(b, stream) : launch<BF, 128, CAP>(b, stream);
+}
+
+// places of the norms' tiles (see slot)
+int64_t slots(const mmfe_attention_args* a, int64_t rows) {
+    const int64_t tiles = (rows + kRows - 1) / kRows;
+    return a->packed ? tiles + a->n_docs + 1 : tiles * a->n_docs;
+}
+int64_t lse_size(const mmfe_attention_args* a) { return (a->packed ? 1 : (int64_t)a->n_docs) * a->heads * a->q_rows; }
 
 }  // namespace
 }  // namespace mmfe
@@ -492,34 +528,41 @@ using namespace mmfe;
 
 extern "C" {
 
-int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_grads* g, int device, void* hip_stream) {
+int64_t mmfe_attention_backward_workspace(const mmfe_attention_args* a) {
+    Problem p{};
+    if (make_problem(a, p)) return -1;
+    const int64_t norms = a->dtype == MMFE_OUT_F16 ? a->heads * slots(a, a->q_rows) + a->kv_heads * slots(a, a->k_rows) : 0;
+    return (2 * lse_size(a) + norms) * (int64_t)sizeof(float);
+}
+
+int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_grads* g, void* workspace, int device, void* hip_stream) {
     BackwardArgs b{};
     int rc = make_problem(a, b.p);
     if (rc) return rc;
     if (g == nullptr || g->struct_size != (int32_t)sizeof(mmfe_attention_grads)) { set_error("attention: gradients NULL or of another version"); return MMFE_EINVAL; }
     const bool any_q = a->q_rows > 0 && (a->packed || a->n_docs > 0), any_k = a->k_rows > 0 && (a->packed || a->n_docs > 0);
-    if (any_q && (a->out == nullptr || a->lse == nullptr || g->grad_out == nullptr || g->grad_q == nullptr || g->scratch == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
+    if (any_q && (a->out == nullptr || a->lse == nullptr || g->grad_out == nullptr || g->grad_q == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
     if (any_k && (g->grad_k == nullptr || g->grad_v == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
-    if (a->dtype == MMFE_OUT_F16 && (any_q || any_k) && a->n_docs > 0 && g->norms == nullptr) { set_error("attention: NULL norms"); return MMFE_EINVAL; }
+    if ((any_q || any_k) && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride) || bad_rows("grad_out", g->grad_out, g->grad_out_stride) || bad_rows("grad_q", g->grad_q, g->grad_q_stride) ||
         bad_rows("grad_k", g->grad_k, g->grad_k_stride) || bad_rows("grad_v", g->grad_v, g->grad_v_stride)) return MMFE_EINVAL;
-    if (count_tiles(b.p, a->q_rows, kRows) * a->heads > 0x7fffffffll || count_tiles(b.p, a->k_rows, kRows) * a->kv_heads > 0x7fffffffll) {
+    if (count_tiles(b.p, a->q_rows, kRows) * a->heads + count_tiles(b.p, a->k_rows, kRows) * a->kv_heads > 0x7fffffffll) {
         set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL;
     }
     auto rows = [](const void* ptr, const int64_t* s) { return Rows{ptr, s[0], s[1], s[2]}; };
     b.out = rows(a->out, a->out_stride); b.rest = static_cast<const char*>(a->out_rest); b.g = rows(g->grad_out, g->grad_out_stride);
     b.dq = rows(g->grad_q, g->grad_q_stride); b.dk = rows(g->grad_k, g->grad_k_stride); b.dv = rows(g->grad_v, g->grad_v_stride);
     b.lse = a->lse; b.lse_b = a->lse_stride[0]; b.lse_h = a->lse_stride[1];
-    const int64_t n = (a->packed ? 1 : (int64_t)a->n_docs) * a->heads * a->q_rows;
-    b.lse2 = g->scratch; b.delta = g->scratch + n;
-    b.norm_g = g->norms; b.norm_v = g->norms ? g->norms + (int64_t)a->n_docs * a->kv_heads : nullptr;
+    b.lse2 = static_cast<float*>(workspace); b.delta = b.lse2 + lse_size(a);
+    b.q_slots = (int)slots(a, a->q_rows); b.k_slots = (int)slots(a, a->k_rows);
+    b.norm_g = b.delta + lse_size(a); b.norm_v = b.norm_g + (int64_t)a->heads * b.q_slots;
     OnDevice on(device);
     if (on.rc) return on.rc;
     hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
-    const int dp = padded_dim(a->dim);
-    if (a->dtype == MMFE_OUT_BF16) return dp == 32 ? launch<true, 32>(b, a->q_rows, a->k_rows, stream) : dp == 64 ? launch<true, 64>(b, a->q_rows, a->k_rows, stream) : launch<true, 128>(b, a->q_rows, a->k_rows, stream);
-    return dp == 32 ? launch<false, 32>(b, a->q_rows, a->k_rows, stream) : dp == 64 ? launch<false, 64>(b, a->q_rows, a->k_rows, stream) : launch<false, 128>(b, a->q_rows, a->k_rows, stream);
+    const bool cap = a->cap > 0.f;
+    if (a->dtype == MMFE_OUT_BF16) return cap ? launch_dim<true, true>(b, stream) : launch_dim<true, false>(b, stream);
+    return cap ? launch_dim<false, true>(b, stream) : launch_dim<false, false>(b, stream);
 }
 
 }  // extern "C"

@@ -178,13 +178,13 @@ def test_attention_entries_refuse(N):
     def forward(**kw):
         return lib.mmfe_attention_forward(ctypes.byref(args(**kw)), A, 99, None)
 
-    def backward(grads=None, **kw):
-        g = dict(struct_size=ctypes.sizeof(N.AttentionGrads), grad_out=A, grad_q=A, grad_k=A, grad_v=A, scratch=A, norms=A)
+    def backward(grads=None, work=A, **kw):
+        g = dict(struct_size=ctypes.sizeof(N.AttentionGrads), grad_out=A, grad_q=A, grad_k=A, grad_v=A)
         g.update(grads or {})
         s = N.AttentionGrads(**{n: v for n, v in g.items() if "stride" not in n})
         for n in ("grad_out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride"):
             setattr(s, n, (ctypes.c_int64 * 3)(*g.get(n, (2560, 256, 64))))
-        return lib.mmfe_attention_backward(ctypes.byref(args(**kw)), ctypes.byref(s), 99, None)
+        return lib.mmfe_attention_backward(ctypes.byref(args(**kw)), ctypes.byref(s), work, 99, None)
     good = forward()
     assert good not in (0, -1) and backward() == good
     wrong = [dict(struct_size=8), dict(dtype=0), dict(dim=12), dict(dim=136), dict(dim=0), dict(n_docs=-1), dict(q_rows=-1), dict(k_rows=1 << 31), dict(heads=3),
@@ -199,9 +199,10 @@ def test_attention_entries_refuse(N):
     for kw in wrong:
         assert forward(**kw) == -1, kw
         assert backward(**kw) == -1, kw
-    for kw in (dict(struct_size=4), dict(grad_out=None), dict(grad_q=None), dict(grad_k=None), dict(grad_v=None), dict(scratch=None), dict(grad_q=A + 2),
+    for kw in (dict(struct_size=4), dict(grad_out=None), dict(grad_q=None), dict(grad_k=None), dict(grad_v=None), dict(grad_q=A + 2),
                dict(grad_k_stride=(2560, 256, 4))):
         assert backward(grads=kw) == -1, kw
-    assert backward(lse=None) == -1 and backward(grads=dict(norms=None), dtype=1) == -1 and backward(grads=dict(norms=None)) == good
-    assert lib.mmfe_attention_forward(None, None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, 0, None) == -1
+    assert backward(lse=None) == -1 and backward(work=None) == -1 and backward(work=A + 4) == -1
+    assert lib.mmfe_attention_backward_workspace(ctypes.byref(args())) > 0 and lib.mmfe_attention_backward_workspace(ctypes.byref(args(dim=9))) == -1
+    assert lib.mmfe_attention_forward(None, None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, None, 0, None) == -1
     assert forward(n_docs=0, q=None, k=None, v=None, out=None) == 0 and forward(q_rows=0, q=None, out=None) == 0
