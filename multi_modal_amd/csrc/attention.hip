@@ -223,36 +223,42 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
         constexpr int kAhead = (kRing - 2) * 2 * Load::kCount;
         u32x4 pf[2];
         if (wave_lim > 0) x = scores(0);
-        for (int t = 0; t < n; ++t) {
+        auto step = [&](int t) {           // every wave's parts have arrived, and its reads of the buffers that are asked for now are done
             if (t - 1 + kRing < n) wait_but<kAhead>();     // the last kRing - 2 steps asked for a whole tile of each
             else wait_all();
-            block_sync();              // every wave's parts have arrived, and its reads of the buffers that are asked for now are done
+            block_sync();
             if (t + kRing < n) load_k(t + kRing);
             if (t + kRing - 2 < n) load_v(t + kRing - 2);
-            const int j0 = t * kStepKeys;
-            if (j0 < wave_lim) {
-                shape_and_hide(t);
-                const float mx = State::largest(x);
-                if (t > 0) {
-                    values(t - 1, 0, pf[0]);
-                    values(t - 1, 1, pf[1]);
-                }
-                rescale(mx);
-                const f32x16 y = scores(t + 1);      // past the last step: of whatever the buffer holds, and dropped
-                st.exponentials(x, unit);
-                pf[0] = operand<BF>(x, 0);
-                pf[1] = operand<BF>(x, 1);
-                x = y;
-            } else if (t > 0 && j0 - kStepKeys < wave_lim) {
+        };
+        const int mine = (wave_lim + kStepKeys - 1) / kStepKeys;       // steps of this wave; it only keeps step with the others behind them
+        for (int t = 0; t < mine; ++t) {
+            step(t);
+            shape_and_hide(t);
+            const float mx = State::largest(x);
+            if (t > 0) {
                 values(t - 1, 0, pf[0]);
                 values(t - 1, 1, pf[1]);
             }
+            rescale(mx);
+            const f32x16 y = scores(t + 1);          // past the last step: of whatever the buffer holds, and dropped
+            st.exponentials(x, unit);
+            pf[0] = operand<BF>(x, 0);
+            pf[1] = operand<BF>(x, 1);
+            x = y;
         }
-        wait_all();
-        block_sync();
-        if ((n - 1) * kStepKeys < wave_lim) {
-            values(n - 1, 0, pf[0]);
-            values(n - 1, 1, pf[1]);
+        if (mine < n) step(mine);
+        else {
+            wait_all();
+            block_sync();
+        }
+        if (mine > 0) {
+            values(mine - 1, 0, pf[0]);
+            values(mine - 1, 1, pf[1]);
+        }
+        for (int t = mine + 1; t < n; ++t) step(t);
+        if (mine < n) {
+            wait_all();
+            block_sync();
         }
     }
     const float l = both_sum(st.l);

@@ -232,6 +232,13 @@ __device__ __forceinline__ void dma16(const void* base, unsigned voff, unsigned 
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(voff), "s"(base), "s"(lds_dst) : "memory");
 }
+// two of them
+__device__ __forceinline__ void dma16x2(const void* base0, unsigned voff0, unsigned dst0, const void* base1, unsigned voff1, unsigned dst1) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %3, %4\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff0), "s"(base0), "v"(voff1), "s"(base1), "s"(dst0), "s"(dst1) : "memory");
+}
 __device__ __forceinline__ void dma4(const void* base, unsigned voff, unsigned lds_dst) {
     unsigned keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
@@ -267,7 +274,12 @@ struct Loader {
     }
     // base: the tile's first row; rows >= 1: valid rows from there on
     __device__ __forceinline__ void load(const char* base, int rows, int dim, int64_t stride, unsigned lds, int wave) const {
-        if (rows >= ROWS) {
+        if (rows >= ROWS && kCount % 2 == 0) {
+#pragma unroll
+            for (int i = 0; i + 1 < kCount; i += 2)
+                dma16x2(kKept == 1 ? base + i * kStep * 2 * stride : base, off[kKept == 1 ? 0 : i], lds + number(i, wave) * 1024,
+                        kKept == 1 ? base + (i + 1) * kStep * 2 * stride : base, off[kKept == 1 ? 0 : i + 1], lds + number(i + 1, wave) * 1024);
+        } else if (rows >= ROWS) {
 #pragma unroll
             for (int i = 0; i < kCount; ++i)
                 dma16(kKept == 1 ? base + i * kStep * 2 * stride : base, off[kKept == 1 ? 0 : i], lds + number(i, wave) * 1024);
