@@ -38,6 +38,9 @@ struct BackwardArgs {
     const char* rest;                 // like out: what its rounding lost, or NULL
     const float* lse;
     float *lse2, *delta;              // like lse: lse in log2 units (less the shift of p; +inf for rows without keys), g . o
+    u32x4* aux;                       // like lse, 16 bytes: both again in the form keys_kernel takes (see there)
+    float *part_k, *part_v;           // keys_kernel, one block per query head: (heads, keys, dim) gradients to be summed over the heads that share
+    int sub;                          // ... and how many blocks a key head's query heads are spread over (1 or group)
     int64_t lse_b, lse_h;
     float *norm_g, *norm_v;           // float16: largest squared row norm of each 128-row tile, (heads, q_slots) and (kv_heads, k_slots)
     int q_slots, k_slots, q_tiles, k_tiles, q_blocks;
@@ -62,6 +65,15 @@ __device__ __forceinline__ float block_max(float v, float* lds) {
     for (int w = 1; w < (int)(blockDim.x >> 6); ++w) m = max2(m, lds[w]);
     __syncthreads();
     return m;
+}
+
+// A float32 as three bfloat16 values that add up to it (8 bits each; a fourth place is zero).
+__device__ __forceinline__ u32x2 thirds(float v) {
+    const unsigned a = pack2<true>(v, 0.f);
+    const float r = v - widen<true>(a, 0);
+    const unsigned b = pack2<true>(r, 0.f);
+    const unsigned c = pack2<true>(r - widen<true>(b, 0), 0.f);
+    return u32x2{(a & 0xffffu) | b << 16, c & 0xffffu};
 }
 
 // What both passes need of every row: delta and lse2 (blocks below q_blocks, 128 rows of one head each), and for float16 the tiles' largest
@@ -103,8 +115,14 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const BackwardArgs a)
             if (row < d.nq && e == 0) {
                 const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + row;
                 const float l = a.lse[at];
-                a.lse2[at] = l == -INFINITY ? INFINITY : l * kLog2e - kShift<BF>;
-                a.delta[at] = l == -INFINITY ? 0.f : dot;
+                const float l2 = l == -INFINITY ? INFINITY : l * kLog2e - kShift<BF>;
+                if (l == -INFINITY) dot = 0.f;
+                a.lse2[at] = l2;
+                a.delta[at] = dot;
+                // keys_kernel adds these to its products: in log2 units beside a capped score, in the products' own otherwise.  -1e30: p = 0
+                const float add = p.cap > 0.f ? p.cap * kLog2e - l2 : -l2 / (p.scale * kLog2e);
+                const u32x2 x = thirds(add < -1e30f ? -1e30f : add), y = thirds(-dot);
+                a.aux[at] = u32x4{x.x, x.y, y.x, y.y};
             }
         }
         if constexpr (!BF) {
@@ -157,7 +175,9 @@ __device__ __forceinline__ float find_phi(const BackwardArgs& a, const Doc& d, i
     }
 }
 
-// How scores leave the linear form, in log2 units.
+// Scores in log2 units from the products, and the factor that a capped score's gradient has.  A capped score is
+// cap tanh(z) = cap (1 - 2 r) with r = 1 / (e^(2 z) + 1), and 1 - tanh^2 = 4 (r - r^2): one exponential and one reciprocal; the 4
+// is left to the gradients' final factor.
 template <bool CAP>
 struct Shape {
     bool bias;
@@ -166,23 +186,27 @@ struct Shape {
         bias = p.slopes != nullptr;
         c = p.scale * kLog2e;
         slope = bias ? p.slopes[head] * kLog2e : 0.f;
-        cap_in = CAP ? p.scale / p.cap : 0.f;
-        cap_out = p.cap * kLog2e;
+        cap_in = CAP ? 2.f * kLog2e * p.scale / p.cap : 0.f;
+        cap_out = 2.f * p.cap * kLog2e;
     }
-    // products to scores in log2 units; th: the tanh of capped ones.  at: distance of register row 0, step: its sign per row
-    __device__ __forceinline__ void apply(f32x16& x, f32x16& th, float at, float step) const {
+    // x -> score + add, w -> the factor.  at: distance of register row 0, step: its sign per row.  FOLDED: the products hold `add` already
+    template <bool FOLDED, typename ADD>
+    __device__ __forceinline__ void apply(f32x16& x, f32x16& w, ADD add, float at, float step) const {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if constexpr (CAP) {
-                th[i] = tanh_fast(x[i] * cap_in);
-                x[i] = cap_out * th[i];
-            } else x[i] *= c;
+                const float r = __builtin_amdgcn_rcpf(exp2_fast(x[i] * cap_in) + 1.f);
+                x[i] = fmaf(-cap_out, r, add(i));
+                w[i] = fmaf(-r, r, r);
+            } else if constexpr (FOLDED) x[i] *= c;
+            else x[i] = fmaf(x[i], c, add(i));
         }
         if (bias) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = fmaf(-slope, fabsf(at + step * (float)reg_row(i)), x[i]);
         }
     }
+    __device__ __forceinline__ float factor() const { return CAP ? 4.f : 1.f; }
 };
 
 // rows [0, dim) of result registers to 16-bit memory, times `by`
@@ -232,22 +256,28 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[DP / 32], const char* t
 constexpr int64_t kLongWalk = 2048;   // rows of a key head's queries from which keys_kernel has eight waves
 constexpr int kRing = 4;              // tiles in LDS: the one in use, the next one's scores, two on their way
 
+// Row statistics come as a third kind of operand: prepare_kernel leaves -lse and -delta of each row as three bfloat16 values that add
+// up to the float32, and a product with ones adds them to a row's scores and dp, over all keys at once.  Read as numbers they
+// would be 8 broadcast reads of 1 KB per 32 rows and wave, a third of all LDS traffic, which is what bounds this kernel; so
+// they are one read of 16 bytes a row and two products more (16 to 18, head size 64).
+//
 // dk and dv of 128 keys, 32 per wave, over tiles of 64 rows.  Step u turns the scores of its rows (computed a step earlier) into p and
 // ds beside the products of the next rows, then adds them to dv and dk; its tiles stay until then, and it asks for those of step u + 3.
 // W = 8 waves: the second four take the second 32 rows of every tile and their sums join the first four's through LDS at the
 // end.  A block then takes half as long and one fits a CU instead of two: better where the longest block bounds the launch (FIXME).
 template <bool BF, int DP, bool CAP, int W>
 __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kernel(const BackwardArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][lse2][delta]
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][row statistics]
     const Problem& p = a.p;
     constexpr int kTileBytes = kTile * DP * 2;
-    constexpr int kBuf = 2 * kTileBytes + 2 * kTile * 4;
+    constexpr int kBuf = 2 * kTileBytes + kTile * 16;
     constexpr int kParts = W == 8 ? 1 : 2;                            // 32-row parts of a tile that a wave takes
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int part = W == 8 ? wave >> 2 : 0;
-    const int kvh = blockIdx.x % p.kv_heads;
+    const int lot = blockIdx.x % (p.kv_heads * a.sub), kvh = lot % p.kv_heads;
     Doc d;
-    if (!find_doc<false>(p, blockIdx.x / p.kv_heads, kRows, d)) return;
+    if (!find_doc<false>(p, blockIdx.x / (p.kv_heads * a.sub), kRows, d)) return;
+    const int heads = p.group / a.sub, head0 = kvh * p.group + lot / p.kv_heads * heads;         // query heads of this block
     const int key0 = d.tile * kRows, w0 = key0 + 32 * (wave & 3), key = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
     // rows [first, nq) see key j: all of them, or those from j - off on
@@ -257,7 +287,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
     const int wave_full = first_row(min(w0 + 31, nk - 1));            // from here on every row sees all keys of the wave
     const int my_first = first_row(key);
     const int t_first = block_first / kTile, t_end = block_first < nq ? (nq + kTile - 1) / kTile : t_first;
-    const int steps = (t_end - t_first) * p.group;
+    const int steps = (t_end - t_first) * heads;
 
     typedef Loader<DP, kTile, W> Load;
     Load lq, lg;
@@ -266,14 +296,12 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
     const unsigned lds0 = lds_address(smem);
     int ask_g = 0, ask_t = t_first, ask = 0;                          // the next tile to ask for
     auto stage = [&]() {
-        const int head = kvh * p.group + ask_g, r0 = ask_t * kTile;
+        const int head = head0 + ask_g, r0 = ask_t * kTile;
         const unsigned dst = uniform(lds0 + (ask % kRing) * kBuf);
         lq.load(row_base(p.q, d, d.q0 + r0, head), nq - r0, p.dim, p.q.n, dst, wave);
         lg.load(row_base(a.g, d, d.q0 + r0, head), nq - r0, p.dim, a.g.n, dst + kTileBytes, wave);
         const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + r0;
-        const unsigned mine = 4 * min(lane, nq - 1 - r0);
-        if (wave == 0) dma4(a.lse2 + at, mine, dst + 2 * kTileBytes);
-        if (wave == 1) dma4(a.delta + at, mine, dst + 2 * kTileBytes + kTile * 4);
+        if (wave == 0) dma16(a.aux + at, 16 * min(lane, nq - 1 - r0), dst + 2 * kTileBytes);
         ++ask;
         if (++ask_t == t_end) { ask_t = t_first; ++ask_g; }
     };
@@ -288,10 +316,14 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
     f32x16 dk[DP / 32], dv[DP / 32], x{}, dp{};
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
-    // scores and dp of 32 rows: register rows are rows, a lane has one key
+    const u32x4 ones = half == 0 ? u32x4{0x3f803f80u, 0x00003f80u, 0u, 0u} : u32x4{0u, 0u, 0u, 0u};       // of the three places
+    auto statistics = [&](const char* qt, int b) { return *reinterpret_cast<const u32x4*>(qt + 2 * kTileBytes + (32 * b + col) * 16); };
+    // scores and dp - delta of 32 rows: register rows are rows, a lane has one key
     auto products = [&](const char* qt, int b, f32x16& sx, f32x16& sd) {
-        sx = f32x16{};
-        sd = f32x16{};
+        const u32x4 st = statistics(qt, b);
+        if constexpr (CAP) sx = f32x16{};
+        else sx = mfma<true>(u32x4{st.x, st.y, 0u, 0u}, ones, f32x16{});
+        sd = mfma<true>(u32x4{st.z, st.w, 0u, 0u}, ones, f32x16{});
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) sx = mfma<BF>(read_rows<DP>(qt, 32 * b, s), kf[s], sx);
 #pragma unroll
@@ -303,7 +335,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
     arrived(vf);
     if (steps > 0) products(smem, part, x, dp);
     Shape<CAP> sh;
-    sh.set(p, kvh * p.group);
+    sh.set(p, head0);
     int g = 0, t = t_first;
     for (int step = 0; step < steps; ++step) {
         if (step + kRing - 2 < steps) wait_but<2 * Load::kCount>();   // tile step + 1 is there; what step - 1 asked for may be on its way
@@ -313,15 +345,18 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
         const char* qt = smem + (step % kRing) * kBuf;
         const char* next = smem + ((step + 1) % kRing) * kBuf;
         const char* gt = qt + kTileBytes;
-        const float* lse2 = reinterpret_cast<const float*>(gt + kTileBytes);
-        const float* delta = lse2 + kTile;
 #pragma unroll
         for (int b0 = 0; b0 < kParts; ++b0) {
             const int b = part + b0, i0 = t * kTile + 32 * b;
             const bool live = i0 + 32 > wave_first && i0 < nq;
-            f32x16 th;
+            f32x16 w;
             if (live) {
-                sh.apply(x, th, (float)(i0 + 4 * half + off - key), 1.f);
+                f32x16 add;
+                if constexpr (CAP) {
+                    const u32x4 st = statistics(qt, b);
+                    add = mfma<true>(u32x4{st.x, st.y, 0u, 0u}, ones, f32x16{});
+                }
+                sh.template apply<true>(x, w, [&](int i) { return add[i]; }, (float)(i0 + 4 * half + off - key), 1.f);
                 if (i0 < wave_full || i0 + 32 > nq) {
                     const int lo = my_first - i0 - 4 * half, hi = nq - i0 - 4 * half;
 #pragma unroll
@@ -332,17 +367,11 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
             products(b0 + 1 < kParts ? qt : next, b0 + 1 < kParts ? b + 1 : part, nx, nd);
             if (live) {
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const float4 l4 = *reinterpret_cast<const float4*>(lse2 + 32 * b + 8 * q4 + 4 * half);
-                    const float4 d4 = *reinterpret_cast<const float4*>(delta + 32 * b + 8 * q4 + 4 * half);
-                    const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 4 * q4 + r;
-                        x[i] = exp2_fast(x[i] - l[r]);
-                        dp[i] = fmaf(dp[i], phi, -de[r] * phi) * x[i];
-                        if constexpr (CAP) dp[i] *= 1.f - th[i] * th[i];
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = exp2_fast(x[i]);
+                    dp[i] *= x[i];
+                    if constexpr (!BF) dp[i] *= phi;
+                    if constexpr (CAP) dp[i] *= w[i];
                 }
                 accumulate<BF, DP>(dv, gt, 32 * b, x, nk <= kShortKeys);
                 accumulate<BF, DP>(dk, qt, 32 * b, dp, nk <= kShortKeys);
@@ -352,7 +381,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
         }
         if (++t == t_end) {
             t = t_first;
-            if (++g < p.group) sh.set(p, kvh * p.group + g);
+            if (++g < heads) sh.set(p, head0 + g);
         }
     }
     if constexpr (W == 8) {
@@ -378,9 +407,47 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
             }
     }
     if (key >= d.rows) return;
-    const float back = __builtin_amdgcn_exp2f(-kShift<BF>);
-    store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, d.k0 + key, kvh)), dk, p.dim, p.scale * back / phi, key < nk && steps > 0 && nk > 1);      // a softmax over one key is constant
-    store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, d.k0 + key, kvh)), dv, p.dim, back, key < nk && steps > 0);
+    const float back = __builtin_amdgcn_exp2f(-kShift<BF>), fk = p.scale * back / phi * sh.factor();
+    const bool any = key < nk && steps > 0, any_k = any && nk > 1;    // a softmax over one key is constant
+    if (a.sub == 1) {
+        store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, d.k0 + key, kvh)), dk, p.dim, fk, any_k);
+        store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, d.k0 + key, kvh)), dv, p.dim, back, any);
+        return;
+    }
+    const int64_t rows = p.packed ? p.k_rows : p.k_rows * p.n_docs;
+    const int64_t at = (head0 * rows + (p.packed ? d.k0 : d.batch * p.k_rows) + key) * p.dim;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int e = 32 * i + 2 * r;
+            if (e >= p.dim) continue;
+            *reinterpret_cast<float4*>(a.part_k + at + e + 4 * half) = any_k ? make_float4(dk[i][r] * fk, dk[i][r + 1] * fk, dk[i][r + 2] * fk, dk[i][r + 3] * fk) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(a.part_v + at + e + 4 * half) = any ? make_float4(dv[i][r] * back, dv[i][r + 1] * back, dv[i][r + 2] * back, dv[i][r + 3] * back) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+}
+
+// Sums of the query heads' parts, 4 elements a thread.
+template <bool BF>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const BackwardArgs a, int64_t n) {
+    const Problem& p = a.p;
+    const int64_t rows = p.packed ? p.k_rows : p.k_rows * p.n_docs;
+    const int pieces = p.dim / 4;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t which = i >= n / 2, j = i - which * (n / 2);
+        const int64_t hr = j / pieces;
+        const int e = 4 * (int)(j - hr * pieces), kvh = (int)(hr / rows);
+        const int64_t row = hr - kvh * rows;
+        const float* part = (which ? a.part_v : a.part_k) + ((int64_t)kvh * p.group * rows + row) * p.dim + e;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int h = 0; h < p.group; ++h) {
+            const float4 v = *reinterpret_cast<const float4*>(part + h * rows * p.dim);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        const Rows& to = which ? a.dv : a.dk;
+        const int64_t b = p.packed ? 0 : row / p.k_rows;
+        store4<BF>(static_cast<char*>(const_cast<void*>(to.p)) + 2 * (b * to.b + (row - b * p.k_rows) * to.n + kvh * to.h + e), nullptr, s.x, s.y, s.z, s.w);
+    }
 }
 
 // dq of 128 rows, 32 per wave, over tiles of 32 keys; steps overlap as in keys_kernel.
@@ -422,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
     load_rows<DP>(gf, row_base(a.g, d, d.q0 + r, head), p.dim, nq > 0);
     const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + r;
     const float phi = find_phi<BF>(a, d, kvh, reinterpret_cast<float*>(smem));
-    float lse2 = nq > 0 ? a.lse2[at] : 0.f;
+    float add = nq > 0 ? (CAP ? p.cap * kLog2e : 0.f) - a.lse2[at] : 0.f;       // what the scores' log2 form lacks to log2 p
     float delta = nq > 0 ? -a.delta[at] * phi : 0.f;
     Shape<CAP> sh;
     sh.set(p, head);
@@ -442,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
     block_sync();
     arrived(qf);
     arrived(gf);
-    asm volatile("" : "+v"(lse2), "+v"(delta));
+    asm volatile("" : "+v"(add), "+v"(delta));
     if (wave_lim > 0) products(smem, x, dp);
     for (int t = 0; t < n; ++t) {
         if (t + kRing - 2 < n) wait_but<2 * Load::kCount>();
@@ -452,8 +519,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
         const int j0 = t * kKeys;
         if (j0 >= wave_lim) continue;
         const char* kt = smem + (t % kRing) * 2 * kTileBytes;
-        f32x16 th;
-        sh.apply(x, th, (float)(row + off - j0 - 4 * half), -1.f);
+        f32x16 w;
+        sh.template apply<false>(x, w, [&](int) { return add; }, (float)(row + off - j0 - 4 * half), -1.f);
         if (j0 + kKeys > full_lim) {
             const int left = lim - j0 - 4 * half;
 #pragma unroll
@@ -463,8 +530,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
         products(smem + ((t + 1) % kRing) * 2 * kTileBytes, nx, nd);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            dp[i] = fmaf(dp[i], phi, delta) * exp2_fast(x[i] - lse2);
-            if constexpr (CAP) dp[i] *= 1.f - th[i] * th[i];
+            dp[i] = (BF ? dp[i] + delta : fmaf(dp[i], phi, delta)) * exp2_fast(x[i]);
+            if constexpr (CAP) dp[i] *= w[i];
         }
         accumulate<BF, DP>(dq, kt, 0, dp, nk <= kShortKeys);
         x = nx;
@@ -472,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
     }
     wait_all();
     if (row >= d.rows) return;
-    store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi, lim > 1);       // a softmax over one key is constant
+    store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi * sh.factor(), lim > 1);       // a softmax over one key is constant
 }
 
 template <bool BF, int DP, bool CAP>
@@ -489,14 +556,18 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     if (tk > 0) {
         // eight waves where a block's walk over the rows is long and its length, not the number of blocks, bounds the launch
         p.tiles = b.k_tiles;
-        const bool wide = DP < 128 && p.q_rows * p.group >= kLongWalk;
+        const bool wide = DP < 128 && p.q_rows * (p.group / b.sub) >= kLongWalk;
         constexpr int W = DP < 128 ? 8 : 4;
         const auto fn = wide ? &keys_kernel<BF, DP, CAP, W> : &keys_kernel<BF, DP, CAP, 4>;
-        const size_t tiles = kRing * (2 * (size_t)kTile * DP * 2 + 2 * kTile * 4), meet = 4 * (size_t)(DP / 32) * 2 * 16 * 64 * 4;
+        const size_t tiles = kRing * (2 * (size_t)kTile * DP * 2 + kTile * 16), meet = 4 * (size_t)(DP / 32) * 2 * 16 * 64 * 4;
         const size_t lds = wide && meet > tiles ? meet : tiles;
         const int threads = 64 * (wide ? W : 4);
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), threads, lds, &blocks, &cus)) != MMFE_OK) return rc;
-        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads)), dim3(threads), lds, stream, b);
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.sub)), dim3(threads), lds, stream, b);
+        if (b.sub > 1) {
+            const int64_t n = 2 * (p.packed ? p.k_rows : p.k_rows * p.n_docs) * p.kv_heads * (p.dim / 4), need = (n + kThreads - 1) / kThreads;
+            hipLaunchKernelGGL(sum_kernel<BF>, dim3((uint32_t)(need < 8192 ? need : 8192)), dim3(kThreads), 0, stream, b, n);
+        }
     }
     if (tq > 0) {
         p.tiles = b.q_tiles;
@@ -519,6 +590,13 @@ int64_t slots(const mmfe_attention_args* a, int64_t rows) {
     const int64_t tiles = (rows + kRows - 1) / kRows;
     return a->packed ? tiles + a->n_docs + 1 : tiles * a->n_docs;
 }
+// Blocks that a key head's query heads are spread over: one, or one per query head (whose parts a second launch sums in float32)
+// where one would leave fewer than 1024 blocks, 4 a CU: FIXME
+int spread(const mmfe_attention_args* a) {
+    const int64_t rows = a->packed ? a->k_rows : a->k_rows * a->n_docs;
+    return a->heads > a->kv_heads && (rows + kRows - 1) / kRows * a->kv_heads < 1024 && a->q_rows * (a->heads / a->kv_heads) >= kLongWalk ? a->heads / a->kv_heads : 1;
+}
+int64_t part_size(const mmfe_attention_args* a) { return spread(a) > 1 ? (a->packed ? a->k_rows : a->k_rows * a->n_docs) * a->heads * a->dim : 0; }
 int64_t lse_size(const mmfe_attention_args* a) { return (a->packed ? 1 : (int64_t)a->n_docs) * a->heads * a->q_rows; }
 
 }  // namespace
@@ -532,7 +610,7 @@ int64_t mmfe_attention_backward_workspace(const mmfe_attention_args* a) {
     Problem p{};
     if (make_problem(a, p)) return -1;
     const int64_t norms = a->dtype == MMFE_OUT_F16 ? a->heads * slots(a, a->q_rows) + a->kv_heads * slots(a, a->k_rows) : 0;
-    return (2 * lse_size(a) + norms) * (int64_t)sizeof(float);
+    return (6 * lse_size(a) + 2 * part_size(a) + norms + 4) * (int64_t)sizeof(float);
 }
 
 int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_grads* g, void* workspace, int device, void* hip_stream) {
@@ -547,14 +625,17 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride) || bad_rows("grad_out", g->grad_out, g->grad_out_stride) || bad_rows("grad_q", g->grad_q, g->grad_q_stride) ||
         bad_rows("grad_k", g->grad_k, g->grad_k_stride) || bad_rows("grad_v", g->grad_v, g->grad_v_stride)) return MMFE_EINVAL;
-    if (count_tiles(b.p, a->q_rows, kRows) * a->heads + count_tiles(b.p, a->k_rows, kRows) * a->kv_heads > 0x7fffffffll) {
+    if (count_tiles(b.p, a->q_rows, kRows) * a->heads + count_tiles(b.p, a->k_rows, kRows) * a->heads > 0x7fffffffll) {
         set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL;
     }
     auto rows = [](const void* ptr, const int64_t* s) { return Rows{ptr, s[0], s[1], s[2]}; };
     b.out = rows(a->out, a->out_stride); b.rest = static_cast<const char*>(a->out_rest); b.g = rows(g->grad_out, g->grad_out_stride);
     b.dq = rows(g->grad_q, g->grad_q_stride); b.dk = rows(g->grad_k, g->grad_k_stride); b.dv = rows(g->grad_v, g->grad_v_stride);
     b.lse = a->lse; b.lse_b = a->lse_stride[0]; b.lse_h = a->lse_stride[1];
-    b.lse2 = static_cast<float*>(workspace); b.delta = b.lse2 + lse_size(a);
+    b.sub = spread(a);
+    b.aux = static_cast<u32x4*>(workspace);
+    b.part_k = reinterpret_cast<float*>(b.aux + lse_size(a)); b.part_v = b.part_k + part_size(a);
+    b.lse2 = b.part_v + part_size(a); b.delta = b.lse2 + lse_size(a);
     b.q_slots = (int)slots(a, a->q_rows); b.k_slots = (int)slots(a, a->k_rows);
     b.norm_g = b.delta + lse_size(a); b.norm_v = b.norm_g + (int64_t)a->heads * b.q_slots;
     OnDevice on(device);

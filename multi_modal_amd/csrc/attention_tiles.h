@@ -239,12 +239,6 @@ __device__ __forceinline__ void dma16x2(const void* base0, unsigned voff0, unsig
                  "global_load_lds_dwordx4 %3, %4\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(voff0), "s"(base0), "v"(voff1), "s"(base1), "s"(dst0), "s"(dst1) : "memory");
 }
-__device__ __forceinline__ void dma4(const void* base, unsigned voff, unsigned lds_dst) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(voff), "s"(base), "s"(lds_dst) : "memory");
-}
-
 __device__ __forceinline__ unsigned lds_address(const void* p) {
     return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
