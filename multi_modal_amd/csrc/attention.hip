@@ -47,18 +47,36 @@ struct Shape {
     float c, slope, cap_in, cap_out;
     __device__ __forceinline__ Shape(const Problem& p, int head) {
         c = p.scale * kLog2e;
-        slope = SHAPE & kBias ? p.slopes[head] * kLog2e : 0.f;
-        cap_in = SHAPE & kCap ? p.scale / p.cap : 0.f;
-        cap_out = SHAPE & kCap ? p.cap * kLog2e : 0.f;
+        slope = SHAPE & kBias ? __uint_as_float(uniform(__float_as_uint(p.slopes[head] * kLog2e))) : 0.f;
+        cap_in = SHAPE & kCap ? 2.f * kLog2e * p.scale / p.cap : 0.f;
+        cap_out = SHAPE & kCap ? 2.f * p.cap * kLog2e : 0.f;
     }
-    // x: products of 32 keys from j0 on; at = row + off - j0 - 4 * half: distance to the lane's first key
-    __device__ __forceinline__ void apply(f32x16& x, float at) const {
+    // x: products of 32 keys; at: distance from the lane's row back to its first key (row + off - j0 - 4 * half); side 1: all keys stand at
+    // or before all rows of the wave, -1: all behind them, 0: some of each.  Returns what the scores lack: on one side, -slope * |at - r|
+    // is a number of the row's plus a number that all lanes share, and only the shared one is added here (one instruction a score, not three).
+    // A capped score is cap tanh(z) = cap - 2 cap / (e^(2 z) + 1).
+    __device__ __forceinline__ float apply(f32x16& x, float at, int side) const {
+        if constexpr (SHAPE & kCap)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if constexpr (SHAPE & kCap) x[i] = cap_out * tanh_fast(x[i] * cap_in);
-            if constexpr (SHAPE == kBias) x[i] = fmaf(x[i], c, -slope * fabsf(at - (float)reg_row(i)));
-            if constexpr (SHAPE == (kBias | kCap)) x[i] = fmaf(-slope, fabsf(at - (float)reg_row(i)), x[i]);
+            for (int i = 0; i < 16; ++i) x[i] = fmaf(-cap_out, __builtin_amdgcn_rcpf(exp2_fast(x[i] * cap_in) + 1.f), 0.5f * cap_out);
+        if constexpr (SHAPE & kBias) {
+            if (side == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float far = slope * fabsf(at - (float)reg_row(i));
+                    x[i] = SHAPE & kCap ? x[i] - far : fmaf(x[i], c, -far);
+                }
+                return 0.f;
+            }
+            const float s = side > 0 ? slope : -slope;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float shared = __uint_as_float(uniform(__float_as_uint(s * (float)reg_row(i))));
+                x[i] = SHAPE & kCap ? x[i] + shared : fmaf(x[i], c, shared);
+            }
+            return -s * at;
         }
+        return 0.f;
     }
     // factor from the units the maximum is kept in to log2 units
     __device__ __forceinline__ float unit() const { return SHAPE == kPlain ? c : 1.f; }
@@ -67,14 +85,14 @@ struct Shape {
 // Softmax state of a lane's row, and what 32 keys do to it.
 struct State {
     float m = -INFINITY, l = 0.f;
-    __device__ __forceinline__ static float largest(const f32x16& a) {
+    __device__ __forceinline__ static float largest(const f32x16& a, float lack) {      // lack: the lane's own, before the halves meet
         float m = a[0], k = a[1];
 #pragma unroll
         for (int i = 2; i < 16; i += 4) {
             m = max2(max2(m, a[i]), a[i + 1]);
             if (i + 2 < 16) k = max2(max2(k, a[i + 2]), a[i + 3]);
         }
-        return both_max(max2(m, k));
+        return both_max(max2(m, k) + lack);
     }
     // raises the running maximum when scores exceed it by more than 8 log2 units; true: o and l have to be scaled by alpha
     __device__ __forceinline__ bool raise(float mx, float unit, float& alpha) {
@@ -85,8 +103,9 @@ struct State {
         l *= alpha;
         return true;
     }
-    __device__ __forceinline__ void exponentials(f32x16& x, float unit) {
-        const float mc = m == -INFINITY ? 0.f : m * unit;
+    // lack: what the scores lack, in log2 units
+    __device__ __forceinline__ void exponentials(f32x16& x, float unit, float lack) {
+        const float mc = (m == -INFINITY ? 0.f : m * unit) - lack;
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
@@ -183,8 +202,10 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     };
     auto shape_and_hide = [&](int t) {
         const int j0 = t * kStepKeys;
-        if constexpr (SHAPE != kPlain) sh.apply(x, (float)(row + off - j0 - 4 * half));
+        float lack = 0.f;
+        if constexpr (SHAPE != kPlain) lack = sh.apply(x, (float)(row + off - j0 - 4 * half), j0 + kStepKeys - 1 <= w0 + off ? 1 : j0 >= w0 + 31 + off ? -1 : 0);
         if (j0 + kStepKeys > full_lim) hide(x, lim - j0 - 4 * half);
+        return lack;
     };
     auto rescale = [&](float mx) {
         float alpha;
@@ -205,9 +226,9 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     if (at_once) {
         for (int t = 0; t < n && t * kStepKeys < wave_lim; ++t) {
             x = scores(t);
-            shape_and_hide(t);
-            rescale(State::largest(x));
-            st.exponentials(x, unit);
+            const float lack = shape_and_hide(t);
+            rescale(State::largest(x, lack));
+            st.exponentials(x, unit, lack);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const u32x4 pf = operand<BF>(x, s);
@@ -233,15 +254,15 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
         const int mine = (wave_lim + kStepKeys - 1) / kStepKeys;       // steps of this wave; it only keeps step with the others behind them
         for (int t = 0; t < mine; ++t) {
             step(t);
-            shape_and_hide(t);
-            const float mx = State::largest(x);
+            const float lack = shape_and_hide(t);
+            const float mx = State::largest(x, lack);
             if (t > 0) {
                 values(t - 1, 0, pf[0]);
                 values(t - 1, 1, pf[1]);
             }
             rescale(mx);
             const f32x16 y = scores(t + 1);          // past the last step: of whatever the buffer holds, and dropped
-            st.exponentials(x, unit);
+            st.exponentials(x, unit, lack);
             pf[0] = operand<BF>(x, 0);
             pf[1] = operand<BF>(x, 1);
             x = y;

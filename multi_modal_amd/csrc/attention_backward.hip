@@ -253,7 +253,6 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[DP / 32], const char* t
         }
 }
 
-constexpr int64_t kLongWalk = 2048;   // rows of a key head's queries from which keys_kernel has eight waves
 constexpr int kRing = 4;              // tiles in LDS: the one in use, the next one's scores, two on their way
 
 // Row statistics come as a third kind of operand: prepare_kernel leaves -lse and -delta of each row as three bfloat16 values that add
@@ -263,22 +262,19 @@ constexpr int kRing = 4;              // tiles in LDS: the one in use, the next 
 //
 // dk and dv of 128 keys, 32 per wave, over tiles of 64 rows.  Step u turns the scores of its rows (computed a step earlier) into p and
 // ds beside the products of the next rows, then adds them to dv and dk; its tiles stay until then, and it asks for those of step u + 3.
-// W = 8 waves: the second four take the second 32 rows of every tile and their sums join the first four's through LDS at the
-// end.  A block then takes half as long and one fits a CU instead of two: better where the longest block bounds the launch (FIXME).
-template <bool BF, int DP, bool CAP, int W>
-__global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kernel(const BackwardArgs a) {
+// Head size 128 has one wave per SIMD (357 registers), the smaller ones two.
+template <bool BF, int DP, bool CAP>
+__global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][row statistics]
     const Problem& p = a.p;
     constexpr int kTileBytes = kTile * DP * 2;
     constexpr int kBuf = 2 * kTileBytes + kTile * 16;
-    constexpr int kParts = W == 8 ? 1 : 2;                            // 32-row parts of a tile that a wave takes
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int part = W == 8 ? wave >> 2 : 0;
     const int lot = blockIdx.x % (p.kv_heads * a.sub), kvh = lot % p.kv_heads;
     Doc d;
     if (!find_doc<false>(p, blockIdx.x / (p.kv_heads * a.sub), kRows, d)) return;
     const int heads = p.group / a.sub, head0 = kvh * p.group + lot / p.kv_heads * heads;         // query heads of this block
-    const int key0 = d.tile * kRows, w0 = key0 + 32 * (wave & 3), key = w0 + col;
+    const int key0 = d.tile * kRows, w0 = key0 + 32 * wave, key = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
     // rows [first, nq) see key j: all of them, or those from j - off on
     auto first_row = [&](int j) { return p.causal && j >= d.prefix ? max(0, j - off) : 0; };
@@ -289,7 +285,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
     const int t_first = block_first / kTile, t_end = block_first < nq ? (nq + kTile - 1) / kTile : t_first;
     const int steps = (t_end - t_first) * heads;
 
-    typedef Loader<DP, kTile, W> Load;
+    typedef Loader<DP, kTile, kWaves> Load;
     Load lq, lg;
     lq.init(p.dim, p.q.n, wave);
     lg.init(p.dim, a.g.n, wave);
@@ -333,7 +329,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
     block_sync();
     arrived(kf);
     arrived(vf);
-    if (steps > 0) products(smem, part, x, dp);
+    if (steps > 0) products(smem, 0, x, dp);
     Shape<CAP> sh;
     sh.set(p, head0);
     int g = 0, t = t_first;
@@ -346,8 +342,8 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
         const char* next = smem + ((step + 1) % kRing) * kBuf;
         const char* gt = qt + kTileBytes;
 #pragma unroll
-        for (int b0 = 0; b0 < kParts; ++b0) {
-            const int b = part + b0, i0 = t * kTile + 32 * b;
+        for (int b = 0; b < 2; ++b) {
+            const int i0 = t * kTile + 32 * b;
             const bool live = i0 + 32 > wave_first && i0 < nq;
             f32x16 w;
             if (live) {
@@ -364,7 +360,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
                 }
             }
             f32x16 nx, nd;
-            products(b0 + 1 < kParts ? qt : next, b0 + 1 < kParts ? b + 1 : part, nx, nd);
+            products(b == 0 ? qt : next, 1 - b, nx, nd);
             if (live) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -383,28 +379,6 @@ __global__ void __launch_bounds__(64 * W, DP == 128 || W == 8 ? 1 : 2) keys_kern
             t = t_first;
             if (++g < heads) sh.set(p, head0 + g);
         }
-    }
-    if constexpr (W == 8) {
-        wait_all();
-        block_sync();
-        float* meet = reinterpret_cast<float*>(smem) + (wave & 3) * (DP / 32) * 2 * 16 * 64 + lane;
-        if (part == 1)
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    meet[(i * 32 + r) * 64] = dk[i][r];
-                    meet[(i * 32 + 16 + r) * 64] = dv[i][r];
-                }
-        __syncthreads();
-        if (part == 1) return;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                dk[i][r] += meet[(i * 32 + r) * 64];
-                dv[i][r] += meet[(i * 32 + 16 + r) * 64];
-            }
     }
     if (key >= d.rows) return;
     const float back = __builtin_amdgcn_exp2f(-kShift<BF>), fk = p.scale * back / phi * sh.factor();
@@ -554,16 +528,11 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     const int64_t norms = BF ? 0 : tk * p.kv_heads;
     if (b.q_blocks + norms > 0) hipLaunchKernelGGL((prepare_kernel<BF, DP>), dim3((uint32_t)(b.q_blocks + norms)), dim3(kThreads), 0, stream, b);
     if (tk > 0) {
-        // eight waves where a block's walk over the rows is long and its length, not the number of blocks, bounds the launch
         p.tiles = b.k_tiles;
-        const bool wide = DP < 128 && p.q_rows * (p.group / b.sub) >= kLongWalk;
-        constexpr int W = DP < 128 ? 8 : 4;
-        const auto fn = wide ? &keys_kernel<BF, DP, CAP, W> : &keys_kernel<BF, DP, CAP, 4>;
-        const size_t tiles = kRing * (2 * (size_t)kTile * DP * 2 + kTile * 16), meet = 4 * (size_t)(DP / 32) * 2 * 16 * 64 * 4;
-        const size_t lds = wide && meet > tiles ? meet : tiles;
-        const int threads = 64 * (wide ? W : 4);
-        if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), threads, lds, &blocks, &cus)) != MMFE_OK) return rc;
-        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.sub)), dim3(threads), lds, stream, b);
+        const auto fn = &keys_kernel<BF, DP, CAP>;
+        const size_t lds = kRing * (2 * (size_t)kTile * DP * 2 + kTile * 16);
+        if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.sub)), dim3(kThreads), lds, stream, b);
         if (b.sub > 1) {
             const int64_t n = 2 * (p.packed ? p.k_rows : p.k_rows * p.n_docs) * p.kv_heads * (p.dim / 4), need = (n + kThreads - 1) / kThreads;
             hipLaunchKernelGGL(sum_kernel<BF>, dim3((uint32_t)(need < 8192 ? need : 8192)), dim3(kThreads), 0, stream, b, n);
@@ -591,10 +560,11 @@ int64_t slots(const mmfe_attention_args* a, int64_t rows) {
     return a->packed ? tiles + a->n_docs + 1 : tiles * a->n_docs;
 }
 // Blocks that a key head's query heads are spread over: one, or one per query head (whose parts a second launch sums in float32)
-// where one would leave fewer than 1024 blocks, 4 a CU: FIXME
+// where one would leave fewer than 1024 blocks, 4 a CU, and walk over 2048 rows at least.  4096 rows, 16 heads on 4 of 128: 766 us in 128
+// blocks, 405 in 512 and the sums; at 1024 blocks and more both take the same and the parts' traffic is saved.
 int spread(const mmfe_attention_args* a) {
     const int64_t rows = a->packed ? a->k_rows : a->k_rows * a->n_docs;
-    return a->heads > a->kv_heads && (rows + kRows - 1) / kRows * a->kv_heads < 1024 && a->q_rows * (a->heads / a->kv_heads) >= kLongWalk ? a->heads / a->kv_heads : 1;
+    return a->heads > a->kv_heads && (rows + kRows - 1) / kRows * a->kv_heads < 1024 && a->q_rows * (a->heads / a->kv_heads) >= 2048 ? a->heads / a->kv_heads : 1;
 }
 int64_t part_size(const mmfe_attention_args* a) { return spread(a) > 1 ? (a->packed ? a->k_rows : a->k_rows * a->n_docs) * a->heads * a->dim : 0; }
 int64_t lse_size(const mmfe_attention_args* a) { return (a->packed ? 1 : (int64_t)a->n_docs) * a->heads * a->q_rows; }
