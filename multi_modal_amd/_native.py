@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import Optional, Sequence
 
@@ -98,6 +99,12 @@ class AttentionGrads(ctypes.Structure):
         (n, ctypes.c_int64 * 3) for n in ("grad_out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride")]
 
 
+# The same as bytes (struct.pack is several times faster than filling a ctypes structure field by field)
+pack_rotary = struct.Struct("<8i2q4Q12qQ3q").pack
+pack_attention = struct.Struct("<8i2f2q12Q12q2q").pack
+pack_attention_grads = struct.Struct("<2i4Q12q").pack
+
+
 def library_path() -> str:
     """libmmfe.so next to this file; MMFE_LIBRARY_PATH selects another build of the same ABI (kernel tuning)."""
     override = os.environ.get("MMFE_LIBRARY_PATH")
@@ -162,15 +169,15 @@ def bind_library(path: str):
     lib.mmfe_rotary_destroy.restype = ctypes.c_int
     lib.mmfe_rotary_destroy.argtypes = [ctypes.c_void_p]
     lib.mmfe_rotary_run.restype = ctypes.c_int
-    lib.mmfe_rotary_run.argtypes = [ctypes.c_void_p, ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
+    lib.mmfe_rotary_run.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     lib.mmfe_attention_forward.restype = ctypes.c_int
-    lib.mmfe_attention_forward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_forward.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.mmfe_attention_workspace.restype = c_i64
-    lib.mmfe_attention_workspace.argtypes = [ctypes.POINTER(AttentionArgs)]
+    lib.mmfe_attention_workspace.argtypes = [ctypes.c_void_p]
     lib.mmfe_attention_backward.restype = ctypes.c_int
-    lib.mmfe_attention_backward.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionGrads), ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
+    lib.mmfe_attention_backward.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
     lib.mmfe_attention_backward_workspace.restype = c_i64
-    lib.mmfe_attention_backward_workspace.argtypes = [ctypes.POINTER(AttentionArgs)]
+    lib.mmfe_attention_backward_workspace.argtypes = [ctypes.c_void_p]
     lib.mmfe_grad_partials.restype = c_i64
     lib.mmfe_grad_partials.argtypes = [c_i64]
     lib.mmfe_grad_clip.restype = ctypes.c_int
@@ -354,8 +361,11 @@ class RotaryHandle:
         check(self._lib.mmfe_rotary_create(len(sections), s, ladder, pairing, float(base), int(device), ctypes.byref(handle)), "mmfe_rotary_create")
         self._handle = handle
 
-    def run(self, args: RotaryArgs, stream: int) -> None:
-        check(self._lib.mmfe_rotary_run(self._handle, ctypes.byref(args), stream or None), "mmfe_rotary_run")
+    def run(self, args: bytes, stream: int) -> None:
+        """args: pack_rotary of the fields of RotaryArgs"""
+        rc = self._lib.mmfe_rotary_run(self._handle, args, stream)
+        if rc:
+            check(rc, "mmfe_rotary_run")
 
     def close(self) -> None:
         if getattr(self, "_handle", None):
@@ -369,28 +379,37 @@ class RotaryHandle:
             pass
 
 
-def attention_forward(args: AttentionArgs, workspace_ptr: int, device: int, stream: int) -> None:
-    check(load_library().mmfe_attention_forward(ctypes.byref(args), workspace_ptr or None, device, stream or None), "mmfe_attention_forward")
+# args, grads: pack_attention / pack_attention_grads of the fields of AttentionArgs / AttentionGrads
 
-
-def attention_workspace(args: AttentionArgs, backward: bool = False) -> int:
-    lib = load_library()
-    n = (lib.mmfe_attention_backward_workspace if backward else lib.mmfe_attention_workspace)(ctypes.byref(args))
-    check(0 if n >= 0 else -1, "mmfe_attention_workspace")
+def attention_workspace(args: bytes, backward: bool = False) -> int:
+    lib = _lib or load_library()
+    n = (lib.mmfe_attention_backward_workspace if backward else lib.mmfe_attention_workspace)(args)
+    if n < 0:
+        check(-1, "mmfe_attention_workspace")
     return n
 
 
-def attention_backward(args: AttentionArgs, grads: AttentionGrads, workspace_ptr: int, device: int, stream: int) -> None:
-    check(load_library().mmfe_attention_backward(ctypes.byref(args), ctypes.byref(grads), workspace_ptr or None, device, stream or None), "mmfe_attention_backward")
+def attention_forward(args: bytes, workspace_ptr: int, device: int, stream: int) -> None:
+    rc = (_lib or load_library()).mmfe_attention_forward(args, workspace_ptr, device, stream)
+    if rc:
+        check(rc, "mmfe_attention_forward")
+
+
+def attention_backward(args: bytes, grads: bytes, workspace_ptr: int, device: int, stream: int) -> None:
+    rc = (_lib or load_library()).mmfe_attention_backward(args, grads, workspace_ptr, device, stream)
+    if rc:
+        check(rc, "mmfe_attention_backward")
 
 
 def grad_partials(n: int) -> int:
-    return int(load_library().mmfe_grad_partials(n))
+    return int((_lib or load_library()).mmfe_grad_partials(n))
 
 
 def grad_clip(ptrs, numels, dtypes, out_ptrs, out_dtypes, kind: int, max_norm: float, partials_ptr: int, norm_ptr: int, device: int, stream: int = 0) -> None:
     n = len(ptrs)
-    check(load_library().mmfe_grad_clip(n, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*numels), (ctypes.c_int32 * n)(*dtypes),
-                                        None if out_ptrs is None else (ctypes.c_void_p * n)(*out_ptrs),
-                                        None if out_ptrs is None else (ctypes.c_int32 * n)(*out_dtypes),
-                                        kind, max_norm, partials_ptr, norm_ptr, device, stream or None), "mmfe_grad_clip")
+    words, codes = struct.Struct(f"{n}q").pack, struct.Struct(f"{n}i").pack
+    rc = (_lib or load_library()).mmfe_grad_clip(
+        n, words(*ptrs), words(*numels), codes(*dtypes), None if out_ptrs is None else words(*out_ptrs),
+        None if out_dtypes is None else codes(*out_dtypes), kind, max_norm, partials_ptr, norm_ptr, device, stream)
+    if rc:
+        check(rc, "mmfe_grad_clip")

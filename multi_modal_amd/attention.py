@@ -14,26 +14,34 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, require_gpu
+from .plans import OUT_CODES, raw_stream, require_gpu
 
 _ARGS_SIZE = ctypes.sizeof(N.AttentionArgs)
 _GRADS_SIZE = ctypes.sizeof(N.AttentionGrads)
 _DTYPES = (torch.float16, torch.bfloat16)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t itself when the kernels can read it where it is (unit stride inside the heads, 16-byte pieces), else a packed copy."""
-    s = t.stride()
-    if s[-1] == 1 and t.data_ptr() % 16 == 0 and all(v % 8 == 0 for v, m in zip(s[:-1], t.shape) if m > 1) and s[-3] <= 1 << 24:
-        return t
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    """t itself when the kernels can read it where it is (unit stride inside the heads, 16-byte pieces), else a packed copy; and its
+    (batch, row, head) strides, 0 where there is one entry."""
+    if t.dim() == 4:
+        b, n, h, e = t.stride()
+        m = t.shape
+        s = (b if m[0] > 1 else 0, n if m[1] > 1 else 0, h if m[2] > 1 else 0)
+    else:
+        n, h, e = t.stride()
+        m = t.shape
+        s = (0, n if m[0] > 1 else 0, h if m[1] > 1 else 0)
+    if e == 1 and t.data_ptr() % 16 == 0 and (s[0] | s[1] | s[2]) % 8 == 0 and s[1] <= 1 << 24:
+        return t, s
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return _rows(t if t.data_ptr() % 16 == 0 else t.clone())
 
 
-def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
-    """(batch, row, head) strides, 0 where there is one entry."""
-    s = tuple(v if m > 1 else 0 for v, m in zip(t.stride()[:-1], t.shape))
-    return s if len(s) == 3 else (0,) + s
+def _packed_strides(t: torch.Tensor) -> Tuple[int, int, int]:
+    """Strides of a contiguous tensor of t's shape."""
+    h, d = t.shape[-2], t.shape[-1]
+    return (t.shape[-3] * h * d if t.dim() == 4 else 0, h * d, d)
 
 
 def _counts(x, name: str, n: int, device, limit: Optional[int] = None, rising: bool = False) -> Optional[torch.Tensor]:
@@ -41,6 +49,8 @@ def _counts(x, name: str, n: int, device, limit: Optional[int] = None, rising: b
     clamped by the kernels."""
     if x is None:
         return None
+    if type(x) is torch.Tensor and x.dtype == torch.int32 and x.is_cuda and x.device == device and x.shape == (n,) and x.is_contiguous():
+        return x
     t = torch.as_tensor(x)
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise TypeError(f"{name} must be integers")
@@ -63,26 +73,27 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 class _Call:
     """One checked call: what does not depend on the outputs."""
 
-    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes")
+    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "device", "q_stride", "k_stride", "v_stride")
 
-    def args(self, q, k, v, out, rest, lse) -> N.AttentionArgs:
-        return N.AttentionArgs(
-            _ARGS_SIZE, OUT_CODES[q.dtype], self.n_docs, q.shape[-2], k.shape[-2], q.shape[-1], self.packed, self.causal, self.scale, self.cap,
-            q.shape[-3], k.shape[-3], q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(self.q_len), _ptr(self.k_len), _ptr(self.q_off), _ptr(self.k_off),
-            _ptr(self.prefix), _ptr(self.slopes), out.data_ptr(), _ptr(rest), _ptr(lse), _strides(q), _strides(k), _strides(v), _strides(out),
-            (0, 0) if lse is None else (lse.stride(0), lse.stride(1)) if lse.dim() == 3 else (0, lse.stride(0)))
+    def args(self, q, k, v, out, rest, lse) -> bytes:
+        H, n = q.shape[-2], q.shape[-3]
+        return N.pack_attention(
+            _ARGS_SIZE, OUT_CODES[q.dtype], self.n_docs, H, k.shape[-2], q.shape[-1], self.packed, self.causal, self.scale, self.cap, n, k.shape[-3],
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(self.q_len), _ptr(self.k_len), _ptr(self.q_off), _ptr(self.k_off), _ptr(self.prefix),
+            _ptr(self.slopes), out.data_ptr(), _ptr(rest), _ptr(lse), *self.q_stride, *self.k_stride, *self.v_stride, *_packed_strides(out), H * n, n)
 
     def forward(self, q, k, v, want_lse: bool, want_rest: bool = False):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        rest = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_rest else None
+        device = q.device
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        rest = torch.empty(q.shape, dtype=q.dtype, device=device) if want_rest else None
         lse = None
         if want_lse:
             shape = (q.shape[-2], q.shape[-3])
-            lse = torch.empty(shape if self.packed else (q.shape[0],) + shape, dtype=torch.float32, device=q.device)
+            lse = torch.empty(shape if self.packed else (q.shape[0],) + shape, dtype=torch.float32, device=device)
         args = self.args(q, k, v, out, rest, lse)
         need = N.attention_workspace(args) if q.shape[-3] <= 64 and not self.packed else 0
-        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        N.attention_forward(args, _ptr(work), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        N.attention_forward(args, _ptr(work), self.device, raw_stream(self.device))
         return out, rest, lse
 
 
@@ -99,13 +110,13 @@ class _AttentionFn(torch.autograd.Function):
     def backward(ctx, grad_out, _):
         q, k, v, out, rest, lse = ctx.saved_tensors
         call = ctx.call
-        g = _rows(grad_out)
+        g, g_stride = _rows(grad_out)
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        grads = N.AttentionGrads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _strides(g), _strides(gq), _strides(gk),
-                                 _strides(gv))
+        kv_stride = _packed_strides(gk)
+        grads = N.pack_attention_grads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *g_stride, *_packed_strides(gq), *kv_stride, *kv_stride)
         args = call.args(q, k, v, out, rest, lse)
         work = torch.empty(N.attention_workspace(args, backward=True), dtype=torch.uint8, device=q.device)
-        N.attention_backward(args, grads, work.data_ptr(), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+        N.attention_backward(args, grads, work.data_ptr(), call.device, raw_stream(call.device))
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None
 
@@ -129,20 +140,23 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
     `lengths`, `offsets` and `prefix` may be integer tensors on the GPU (not read back; entries out of range are clamped) or on the
     host (checked).  return_lse=True also returns the float32 log-sum-exp of each row's scores, (B, H, N) or (H, T), without gradient.
     Tensors on the CPU are copied over and the result is copied back."""
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in _DTYPES or k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"attention takes float16 or bfloat16 tensors of one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     packed = offsets is not None
+    qs, ks = q.shape, k.shape
     dims = 3 if packed else 4
-    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+    if len(qs) != dims or len(ks) != dims or v.dim() != dims:
         raise ValueError("attention takes (batch, tokens, heads, head size) tensors, or (tokens, heads, head size) with offsets")
-    if k.shape != v.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
+    if ks != v.shape or ks[-1] != qs[-1] or (not packed and ks[0] != qs[0]):
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-    H, D, K = q.shape[-2], q.shape[-1], k.shape[-2]
+    H, D, K = qs[-2], qs[-1], ks[-2]
     if K < 1 or H < 1 or H % K != 0:
         raise ValueError(f"{H} query heads cannot share {K} key heads")
     if D < 8 or D > 128 or D % 8 != 0:
         raise ValueError(f"head size {D}: a multiple of 8 up to 128")
-    if k.device != q.device or v.device != q.device:
+    device = origin = q.device
+    if k.device != device or v.device != device:
         raise ValueError("q, k and v must be on one device")
     call = _Call()
     call.cap = float(cap)
@@ -155,7 +169,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
         raise ValueError("lengths belong to the padded form: documents that are packed have offsets")
     if not packed and kv_offsets is not None:
         raise ValueError("kv_offsets needs offsets")
-    n, s = q.shape[-3], k.shape[-3]
+    n, s = qs[-3], ks[-3]
     if packed:
         m = len(offsets) - 1
         if m < 0:
@@ -163,14 +177,14 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
         if kv_offsets is None and s != n:
             raise ValueError(f"{n} rows and {s} keys: kv_offsets says how the keys are cut")
     else:
-        m = q.shape[0]
+        m = qs[0]
         if kv_lengths is None and s == n:
             kv_lengths = lengths
-    require_gpu()
-    origin = q.device
     if not q.is_cuda:
+        require_gpu()
         q, k, v = q.cuda(), k.cuda(), v.cuda()
-    device = q.device
+        device = q.device
+    call.device = device.index
     call.packed, call.causal, call.n_docs = packed, bool(causal), m
     call.q_len = call.k_len = call.q_off = call.k_off = None
     if packed:
@@ -188,11 +202,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
         if t.requires_grad:
             raise ValueError("slopes have no gradient: detach them")
         call.slopes = t.to(device=device, dtype=torch.float32).contiguous()
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, call.q_stride = _rows(q)
+    k, call.k_stride = _rows(k)
+    v, call.v_stride = _rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _AttentionFn.apply(q, k, v, call)
     else:
         out, _, lse = call.forward(q, k, v, return_lse)
-    if origin.type != "cuda":
+    if device != origin:
         out, lse = out.to(origin), None if lse is None else lse.to(origin)
     return (out, lse) if return_lse else out

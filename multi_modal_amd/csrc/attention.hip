@@ -30,6 +30,7 @@ using namespace attn;
 namespace {
 
 constexpr int kSplitTile = 32;         // keys of a wave's tile in split_kernel
+constexpr int kSplitWaves = 2;
 
 struct ForwardArgs {
     Problem p;
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
 
 struct SplitArgs {
     ForwardArgs f;
-    int chunk, n_splits, row_tiles;
+    int chunk, n_splits, n_units, row_tiles;
     float* part;                      // (unit, split, 32, dim) partial results over their own maximum; (unit, split, 32, 2) maximum and sum behind them
     float* part_ml;
 };
@@ -340,12 +341,16 @@ __device__ __forceinline__ void finish_row(const ForwardArgs& f, int doc, const 
 }
 
 template <bool BF, int DP>
-__global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
+__global__ void __launch_bounds__(64 * kSplitWaves, 1) split_kernel(const SplitArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // per wave: 2 x [k tile][v tile]
     const Problem& p = a.f.p;
     constexpr int kTileBytes = kSplitTile * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int unit = blockIdx.x / a.n_splits, split = blockIdx.x - unit * a.n_splits;
+    // Chunk by chunk, the units of a chunk turned by the chunk's number: neighbouring blocks go to different XCDs, and a document's chunks
+    // (long documents have many, short ones one) then spread over all of them, while the key heads of a chunk's keys, which lie
+    // interleaved in memory, are read at the same time.
+    const int split = blockIdx.x / a.n_units, place = blockIdx.x - split * a.n_units;
+    const int unit = (place + split) % a.n_units, part = unit * a.n_splits + split;
     const int kvh = unit % p.kv_heads, rt = (unit / p.kv_heads) % a.row_tiles;
     const int b = unit / p.kv_heads / a.row_tiles;
     Doc d;
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
     const int max_lim = last_token >= 0 && 32 * rt / p.group < nq ? limit(last_token) : 0;
     const int full_lim = limit(32 * rt / p.group);
     const int s0 = split * a.chunk, s1 = min(s0 + a.chunk, max_lim);
-    float2* ml = reinterpret_cast<float2*>(a.part_ml) + (int64_t)blockIdx.x * 32;
+    float2* ml = reinterpret_cast<float2*>(a.part_ml) + (int64_t)part * 32;
     if (s0 >= s1 && a.n_splits > 1) {                                 // nothing of this chunk is visible to these rows
         if (threadIdx.x < n_rows) ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
         return;
@@ -399,10 +404,10 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
     int buf = 0;
     wait_all();
     arrived(qf);
-    for (int t = wave; t < n_tiles; t += kWaves, buf ^= 1) {
-        if (t + kWaves < n_tiles) {
+    for (int t = wave; t < n_tiles; t += kSplitWaves, buf ^= 1) {
+        if (t + kSplitWaves < n_tiles) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the other buffer has been read
-            stage(t + kWaves, buf ^ 1);
+            stage(t + kSplitWaves, buf ^ 1);
             asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * Loader<DP, kSplitTile, 1>::kCount) : "memory");      // all but the tile just asked for
         } else wait_all();
         const int j0 = s0 + t * kSplitTile;
@@ -463,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
     block_sync();
     constexpr int kPitch = DP + 4;
     float* wo = reinterpret_cast<float*>(smem);
-    float2* wml = reinterpret_cast<float2*>(wo + kWaves * 32 * kPitch);
+    float2* wml = reinterpret_cast<float2*>(wo + kSplitWaves * 32 * kPitch);
     if (col < n_rows) {
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
@@ -474,15 +479,15 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
     }
     __syncthreads();
     const int pieces = p.dim / 4;
-    for (int i = threadIdx.x; i < n_rows * pieces; i += kThreads) {
+    for (int i = threadIdx.x; i < n_rows * pieces; i += 64 * kSplitWaves) {
         const int r = i / pieces, e = 4 * (i - r * pieces);
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wml[w * 32 + r].x);
+        for (int w = 0; w < kSplitWaves; ++w) top = fmaxf(top, wml[w * 32 + r].x);
         float total = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < kSplitWaves; ++w) {
             const float2 s = wml[w * 32 + r];
             if (s.y == 0.f) continue;                                 // saw no key
             const float k = exp2_fast(s.x - top);
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) split_kernel(const SplitArgs a) {
         const SplitRow row(p, 32 * rt + r, kvh, nq);
         if (a.n_splits == 1) finish_row<BF>(a.f, b, row, e, limit(row.token) > 0, top, total, v);
         else {
-            *reinterpret_cast<float4*>(a.part + ((int64_t)blockIdx.x * 32 + r) * p.dim + e) = v;
+            *reinterpret_cast<float4*>(a.part + ((int64_t)part * 32 + r) * p.dim + e) = v;
             if (e == 0) ml[r] = make_float2(top, total);
         }
     }
@@ -575,11 +580,14 @@ Cut cut_keys(const mmfe_attention_args* a) {
     if (a->q_rows > 64 || rows > 1024 || a->k_rows <= kShortKeys) return c;
     c.row_tiles = (int)((rows + 31) / 32);
     c.units = (int64_t)a->n_docs * c.row_tiles * a->kv_heads;
-    // About 2048 blocks if every document fills its room, in chunks of 256 keys at least; up to 512 keys stay in one block (a wave then has 4 tiles,
-    // less than the second launch takes)
-    int64_t chunk = (a->k_rows * c.units + 2047) / 2048;
-    chunk = (chunk + 127) / 128 * 128;
-    if (chunk < 256) chunk = 256;
+    // About 2048 blocks if every document fills its room (two or more on each CU, so that one's start and end run beside another's reads; and
+    // documents shorter than their room leave chunks empty), but 512 keys where 1024 blocks have them and 256 otherwise: every chunk
+    // costs its block's start and a part to join.  16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 111 / 97 / 104 us with 512 / 1024 /
+    // 2048 keys; 64 streams of 2048: 70 / 61 us with 256 / 512.  Up to 512 keys stay in one block: 8 tiles a wave take less than a second launch.
+    const int64_t all = a->k_rows * c.units;
+    int64_t chunk = ((all + 2047) / 2048 + 127) / 128 * 128;
+    const int64_t least = all >= 512 * 1024 ? 512 : 256;
+    if (chunk < least) chunk = least;
     if (a->k_rows <= 512) chunk = 512;
     c.chunk = (int)chunk;
     c.n_splits = (int)((a->k_rows + chunk - 1) / chunk);
@@ -679,17 +687,17 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
         SplitArgs s{};
         s.f = f;
         s.f.p.tiles = 1;
-        s.chunk = c.chunk; s.n_splits = c.n_splits; s.row_tiles = c.row_tiles;
+        s.chunk = c.chunk; s.n_splits = c.n_splits; s.n_units = (int)c.units; s.row_tiles = c.row_tiles;
         s.part = static_cast<float*>(workspace);
         s.part_ml = c.n_splits > 1 ? s.part + c.units * c.n_splits * 32 * a->dim : nullptr;
         const split_fn fn = bf ? pick_split<true>(a->dim) : pick_split<false>(a->dim);
         const int dp = padded_dim(a->dim);
-        const size_t tiles = (size_t)kWaves * 4 * kSplitTile * dp * 2, meet = (size_t)kWaves * 32 * ((dp + 4) * 4 + 8);
+        const size_t tiles = (size_t)kSplitWaves * 4 * kSplitTile * dp * 2, meet = (size_t)kSplitWaves * 32 * ((dp + 4) * 4 + 8);
         const size_t lds = tiles > meet ? tiles : meet;
         int blocks = 1, cus = 256;
-        rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);
+        rc = kernel_prepare(reinterpret_cast<const void*>(fn), 64 * kSplitWaves, lds, &blocks, &cus);
         if (rc) return rc;
-        hipLaunchKernelGGL(fn, dim3((uint32_t)(c.units * c.n_splits)), dim3(kThreads), lds, reinterpret_cast<hipStream_t>(hip_stream), s);
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(c.units * c.n_splits)), dim3(64 * kSplitWaves), lds, reinterpret_cast<hipStream_t>(hip_stream), s);
         if (c.n_splits > 1) hipLaunchKernelGGL(bf ? &join_kernel<true> : &join_kernel<false>, dim3((uint32_t)(c.units * 32)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(hip_stream), s);
         return launched("attention");
     }

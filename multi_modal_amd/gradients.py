@@ -7,28 +7,38 @@ another type, e.g. the float32 gradients an optimizer takes) that the clipped gr
 """
 from __future__ import annotations
 
-import ctypes
 import math
-from typing import Iterable, List, Optional, Sequence, Union
+from operator import attrgetter
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, require_gpu
+from .plans import OUT_CODES, raw_stream, require_gpu
 
 _KINDS = {2.0: N.NORM_2, math.inf: N.NORM_MAX}
 
 
 def _gradients(tensors: Union[torch.Tensor, Iterable[torch.Tensor]]) -> List[torch.Tensor]:
     """Gradients of a list of parameters (those that have one), or the tensors of the list themselves."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    kinds = set(map(type, tensors))
+    if kinds == _PLAIN and not any(map(_requires_grad, tensors)):        # the two usual lists, walked in C
+        return tensors
+    if kinds == _PARAMETERS:
+        return [g for g in map(_grad, tensors) if g is not None]
     found = []
-    for t in [tensors] if isinstance(tensors, torch.Tensor) else tensors:
-        if isinstance(t, torch.nn.Parameter) or (t.requires_grad and t.is_leaf):
+    for t in tensors:
+        if (t.requires_grad and t.is_leaf) or isinstance(t, torch.nn.Parameter):
             t = t.grad
             if t is None:
                 continue
         found.append(t)
     return found
+
+
+_PLAIN, _PARAMETERS = {torch.Tensor}, {torch.nn.Parameter}
+_dtype, _grad, _requires_grad = attrgetter("dtype"), attrgetter("grad"), attrgetter("requires_grad")
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -43,27 +53,30 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _check(grads: Sequence[torch.Tensor], what: str) -> torch.device:
-    device = grads[0].device
-    for t in grads:
-        if t.layout != torch.strided:
-            raise TypeError(f"{what}: sparse gradients are not supported")
-        if t.dtype not in OUT_CODES:
-            raise TypeError(f"{what}: float32, float16 or bfloat16 tensors, got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{what}: the tensors are on {device} and {t.device}: clip each device's by itself")
-    if device.type != "cuda":
+def _check(tensors: Sequence[torch.Tensor], what: str) -> Tuple[int, List[int], bool]:
+    """(device index, type codes, all contiguous)"""
+    codes = list(map(OUT_CODES.get, map(_dtype, tensors)))
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if None in codes:
+        raise TypeError(f"{what}: float32, float16 or bfloat16 tensors, got {tensors[codes.index(None)].dtype}")
+    if -1 in devices:
         raise ValueError(f"{what}: the tensors must be on the GPU (there is no CPU path)")
-    return device
+    if len(devices) > 1:
+        raise ValueError(f"{what}: the tensors are on GPUs {sorted(devices)}: clip each device's by itself")
+    contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+    if not contiguous and any(t.layout != torch.strided for t in tensors):           # a sparse tensor is not contiguous
+        raise TypeError(f"{what}: sparse gradients are not supported")
+    return devices.pop(), codes, contiguous
 
 
-def _run(grads, outs, kind, max_norm, device) -> torch.Tensor:
-    norm = torch.empty((), dtype=torch.float32, device=device)
+def _run(grads, codes, outs, out_codes, kind, max_norm, device: int) -> torch.Tensor:
     n = len(grads)
-    partials = torch.empty(N.grad_partials(n), dtype=torch.float64, device=device)
-    N.grad_clip([t.data_ptr() for t in grads], [t.numel() for t in grads], [OUT_CODES[t.dtype] for t in grads],
-                None if outs is None else [t.data_ptr() for t in outs], None if outs is None else [OUT_CODES[t.dtype] for t in outs],
-                kind, max_norm, partials.data_ptr(), norm.data_ptr(), device.index, torch.cuda.current_stream(device).cuda_stream)
+    # the float32 norm stands behind the call's float64 partial sums
+    work = torch.empty(N.grad_partials(n) + 1, dtype=torch.float64, device=grads[0].device)
+    norm = work[-1:].view(torch.float32)[0]
+    ptrs = list(map(torch.Tensor.data_ptr, grads))
+    N.grad_clip(ptrs, list(map(torch.Tensor.numel, grads)), codes, None if outs is None else ptrs if outs is grads else list(map(torch.Tensor.data_ptr, outs)),
+                out_codes, kind, max_norm, work.data_ptr(), norm.data_ptr(), device, raw_stream(device))
     return norm
 
 
@@ -79,12 +92,12 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: f
     """Norm over all values of all tensors (of their gradients, where they are parameters): a float32 scalar on their device.
     float32, float16 and bfloat16 tensors of any shape on one GPU; norm_type 2 or inf.  Nothing given: 0."""
     kind = _kind(norm_type)
-    require_gpu()
     grads = _gradients(tensors)
     if not grads:
+        require_gpu()
         return torch.zeros((), device="cuda")
-    device = _check(grads, "grad_norm")
-    return _run([t if _dense(t) else t.contiguous() for t in grads], None, kind, 0.0, device)
+    device, codes, contiguous = _check(grads, "grad_norm")
+    return _run(grads if contiguous else [t if _dense(t) else t.contiguous() for t in grads], codes, None, None, kind, 0.0, device)
 
 
 @torch.no_grad()
@@ -99,33 +112,32 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must be a number >= 0")
-    require_gpu()
     grads = _gradients(parameters)
     if out is not None:
         out = list(out)
         if len(out) != len(grads):
             raise ValueError(f"out holds {len(out)} tensors for {len(grads)} gradients")
     if not grads:
+        require_gpu()
         return torch.zeros((), device="cuda")
-    device = _check(grads, "clip_grad_norm")
+    device, codes, contiguous = _check(grads, "clip_grad_norm")
     if error_if_nonfinite:
         norm = grad_norm(grads, norm_type)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"the norm of the gradients is {float(norm)}: nothing was scaled")
     if out is not None:
-        _check(out, "clip_grad_norm: out")
-        for g, o in zip(grads, out):
-            if o.device != device or o.numel() != g.numel() or not o.is_contiguous():
-                raise ValueError(f"out: contiguous tensors on {device} with their gradient's number of elements")
-        return _run([t.contiguous() for t in grads], out, kind, max_norm, device)
-    if all(t.is_contiguous() or _dense(t) for t in grads):
-        return _run(grads, grads, kind, max_norm, device)
+        out_device, out_codes, packed = _check(out, "clip_grad_norm: out")
+        if out_device != device or not packed or list(map(torch.Tensor.numel, out)) != list(map(torch.Tensor.numel, grads)):
+            raise ValueError(f"out: contiguous tensors on GPU {device} with their gradient's number of elements")
+        return _run(grads if contiguous else [t.contiguous() for t in grads], codes, out, out_codes, kind, max_norm, device)
+    if contiguous or all(map(_dense, grads)):
+        return _run(grads, codes, grads, codes, kind, max_norm, device)
     # views with gaps: their values pass through a packed copy
     for t in grads:
         if any(s == 0 and m > 1 for s, m in zip(t.stride(), t.shape)):
             raise ValueError("clip_grad_norm cannot write an expanded gradient")
     packed = [t if _dense(t) else t.contiguous() for t in grads]
-    norm = _run(packed, packed, kind, max_norm, device)
+    norm = _run(packed, codes, packed, codes, kind, max_norm, device)
     for t, p in zip(grads, packed):
         if p is not t:
             t.copy_(p)

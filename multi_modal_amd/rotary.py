@@ -16,7 +16,9 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, require_gpu
+from .plans import OUT_CODES, raw_stream, require_gpu
+
+_ARGS_SIZE = ctypes.sizeof(N.RotaryArgs)
 
 _LADDERS = {"shared": N.ROTARY_SHARED, "axis": N.ROTARY_PER_AXIS}
 _PAIRINGS = {"halves": N.ROTARY_HALVES, "adjacent": N.ROTARY_ADJACENT}
@@ -49,6 +51,7 @@ class Rotary:
             raise ValueError("base must be a positive number")
         require_gpu()
         self.base, self.ladder, self.pairing = float(base), ladder, pairing
+        self._pairs2 = 2 * sum(self.sections)
         self.device = torch.cuda.current_device() if device is None else torch.device("cuda", device).index if isinstance(device, int) else torch.device(device).index
         self._h = N.RotaryHandle(self.sections, _LADDERS[ladder], _PAIRINGS[pairing], self.base, self.device)
 
@@ -61,21 +64,25 @@ class Rotary:
         inplace=True writes the result over q and k (no gradients; the two must not share elements) and returns them.
         Tensors on the CPU are copied over and the results copied back."""
         origin = q.device
-        given = [t for t in (q, k) if t is not None]
-        if any(t.dim() != 4 for t in given):
+        dtype, shape = q.dtype, q.shape
+        if len(shape) != 4 or (k is not None and k.dim() != 4):
             raise ValueError("q and k are (batch, tokens, heads, head size) tensors")
-        if any(t.dtype != q.dtype or t.device != q.device for t in given) or q.dtype not in OUT_CODES:
+        if dtype not in OUT_CODES or (k is not None and (k.dtype != dtype or k.device != origin)):
             raise ValueError("q and k must both be float32, float16 or bfloat16 on one device")
-        B, n, _, D = q.shape
+        B, n, _, D = shape
         if k is not None and (k.shape[0] != B or k.shape[1] != n or k.shape[3] != D):
             raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or head size")
-        if D < 2 * sum(self.sections) or D > 1024:
-            raise ValueError(f"head size {D}: the sections {self.sections} need {2 * sum(self.sections)} elements (1024 at most)")
-        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
-            raise TypeError("positions must be integers")
+        if not self._pairs2 <= D <= 1024:
+            raise ValueError(f"head size {D}: the sections {self.sections} need {self._pairs2} elements (1024 at most)")
+        kind = positions.dtype
+        if kind != torch.int32 and kind != torch.int64:
+            if kind.is_floating_point or kind.is_complex or kind == torch.bool:
+                raise TypeError("positions must be integers")
+            positions = positions.to(torch.int64)
         A = len(self.sections)
         if tuple(positions.shape) not in ((A, n), (A, B, n)):
             raise ValueError(f"positions must be ({A}, {n}) or ({A}, {B}, {n}), got {tuple(positions.shape)}")
+        given = (q,) if k is None else (q, k)
         if inplace:
             if torch.is_grad_enabled() and any(t.requires_grad for t in given):
                 raise RuntimeError("inplace=True has no gradient: use it under torch.no_grad()")
@@ -89,18 +96,16 @@ class Rotary:
                 raise ValueError("inplace=True needs a unit stride inside the heads")
         if not q.is_cuda:
             q, k = q.cuda(self.device), None if k is None else k.cuda(self.device)
-        if q.device.index != self.device:
+        if q.get_device() != self.device:
             raise ValueError(f"tensors on {q.device} but the frequency table is on cuda:{self.device}")
-        if positions.dtype not in (torch.int32, torch.int64):
-            positions = positions.to(torch.int64)
-        if positions.device != q.device:
+        if positions.get_device() != self.device:
             positions = positions.to(q.device)
         if not inplace and torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             out = _RotaryFn.apply(q, k, positions, self)
             yq, yk = out if k is not None else (out, None)
         else:
             yq, yk = self._run(q, k, positions, False, inplace)
-        if origin.type != "cuda":
+        if q.device != origin:
             yq, yk = yq.to(origin), None if yk is None else yk.to(origin)
         return yq if yk is None else (yq, yk)
 
@@ -119,13 +124,10 @@ class Rotary:
             return yq, yk
         zero = (0, 0, 0)
         ps = positions.stride()
-        self._h.run(N.RotaryArgs(
-            ctypes.sizeof(N.RotaryArgs), OUT_CODES[some.dtype], positions.dtype == torch.int64, inverse,
-            0 if q is None else q.shape[2], 0 if k is None else k.shape[2], D, 0, B, n,
-            0 if q is None else q.data_ptr(), 0 if q is None else yq.data_ptr(), 0 if k is None else k.data_ptr(), 0 if k is None else yk.data_ptr(),
-            zero if q is None else q.stride()[:3], zero if q is None else yq.stride()[:3], zero if k is None else k.stride()[:3],
-            zero if k is None else yk.stride()[:3], positions.data_ptr(), (ps[0], 0, ps[1]) if len(ps) == 2 else ps),
-            torch.cuda.current_stream(some.device).cuda_stream)
+        qh, qp, yqp, qs, yqs = (0, 0, 0, zero, zero) if q is None else (q.shape[2], q.data_ptr(), yq.data_ptr(), q.stride()[:3], yq.stride()[:3])
+        kh, kp, ykp, ks, yks = (0, 0, 0, zero, zero) if k is None else (k.shape[2], k.data_ptr(), yk.data_ptr(), k.stride()[:3], yk.stride()[:3])
+        self._h.run(N.pack_rotary(_ARGS_SIZE, OUT_CODES[some.dtype], positions.dtype == torch.int64, inverse, qh, kh, D, 0, B, n, qp, yqp, kp, ykp,
+                                  *qs, *yqs, *ks, *yks, positions.data_ptr(), *((ps[0], 0, ps[1]) if len(ps) == 2 else ps)), raw_stream(self.device))
         return yq, yk
 
     def close(self) -> None:

@@ -50,6 +50,15 @@ def test_rotary_entries_refuse(N):
 def test_struct_sizes_match_header(N):
     """The ctypes structures have the C layout (8-byte members on 8-byte boundaries, no padding inside)."""
     assert ctypes.sizeof(N.RotaryArgs) == 8 * 4 + 2 * 8 + 4 * 8 + 12 * 8 + 8 + 3 * 8
+    # ... and the packed bytes are those of the structures
+    for cls, pack in ((N.RotaryArgs, N.pack_rotary), (N.AttentionArgs, N.pack_attention), (N.AttentionGrads, N.pack_attention_grads)):
+        s, values = cls(), []
+        for i, (name, kind) in enumerate(cls._fields_):
+            n = getattr(kind, "_length_", 1)
+            v = [float(i) + 0.5] if kind is ctypes.c_float else [1000 * i + j + 1 for j in range(n)]
+            setattr(s, name, kind(*v) if n > 1 else v[0])
+            values += v
+        assert bytes(s) == pack(*values), cls.__name__
 
 
 def clip(N, ptrs, numels, dtypes, outs=None, out_dtypes=None, kind=2, max_norm=1.0, partials=64, norm=64):
@@ -98,9 +107,11 @@ def test_wrappers_refuse(N):
     for bad in (-1.0, math.nan):
         with pytest.raises(ValueError, match="max_norm"):
             clip_grad_norm([x], bad)
+    with pytest.raises(ValueError, match="no CPU path"):
+        clip_grad_norm([x], 1.0)
     if not torch.cuda.is_available():
         with pytest.raises(N.MmfeError):
-            clip_grad_norm([x], 1.0)
+            clip_grad_norm([], 1.0)
 
 
 def test_share_of_views():
