@@ -9,6 +9,7 @@ import ctypes
 import os
 import struct
 import threading
+from array import array
 from typing import Optional, Sequence
 
 import numpy as np
@@ -405,11 +406,13 @@ def grad_partials(n: int) -> int:
     return int((_lib or load_library()).mmfe_grad_partials(n))
 
 
-def grad_clip(ptrs, numels, dtypes, out_ptrs, out_dtypes, kind: int, max_norm: float, partials_ptr: int, norm_ptr: int, device: int, stream: int = 0) -> None:
-    n = len(ptrs)
-    words, codes = struct.Struct(f"{n}q").pack, struct.Struct(f"{n}i").pack
+def grad_clip(ptrs, numels, codes, out_ptrs, out_codes, kind: int, max_norm: float, partials_ptr: int, norm_ptr: int, device: int, stream: int = 0) -> None:
+    """ptrs, numels, out_ptrs: iterables of integers; codes, out_codes: lists of MMFE_OUT_*; out_ptrs is ptrs: in place"""
+    at, n, types = array("q", ptrs), array("q", numels), array("i", codes)
+    to = None if out_ptrs is None else at if out_ptrs is ptrs else array("q", out_ptrs)
+    to_types = None if out_ptrs is None else types if out_codes is codes else array("i", out_codes)
     rc = (_lib or load_library()).mmfe_grad_clip(
-        n, words(*ptrs), words(*numels), codes(*dtypes), None if out_ptrs is None else words(*out_ptrs),
-        None if out_dtypes is None else codes(*out_dtypes), kind, max_norm, partials_ptr, norm_ptr, device, stream)
+        len(n), at.buffer_info()[0], n.buffer_info()[0], types.buffer_info()[0], None if to is None else to.buffer_info()[0],
+        None if to_types is None else to_types.buffer_info()[0], kind, max_norm, partials_ptr, norm_ptr, device, stream)
     if rc:
         check(rc, "mmfe_grad_clip")

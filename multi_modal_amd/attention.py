@@ -14,7 +14,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, raw_stream, require_gpu
+from .plans import OUT_CODES, once_differentiable, raw_stream, require_gpu
 
 _ARGS_SIZE = ctypes.sizeof(N.AttentionArgs)
 _GRADS_SIZE = ctypes.sizeof(N.AttentionGrads)
@@ -102,13 +102,15 @@ class _AttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, call):
         out, rest, lse = call.forward(q, k, v, True, True)
         ctx.call = call
-        ctx.save_for_backward(q, k, v, out, rest, lse)
+        # the counts too: autograd then notices when one of them has been changed before the backward pass
+        ctx.save_for_backward(q, k, v, out, rest, lse, call.q_len, call.k_len, call.q_off, call.k_off, call.prefix, call.slopes)
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out, _):
-        q, k, v, out, rest, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors[:6]
         call = ctx.call
         g, g_stride = _rows(grad_out)
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))

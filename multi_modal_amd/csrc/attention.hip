@@ -620,6 +620,7 @@ int make_problem(const mmfe_attention_args* a, Problem& p) {
     if (a->q_rows > (1 << 30) || a->k_rows > (1 << 30) || a->n_docs > (1 << 24)) { set_error("attention: too many rows"); return MMFE_EINVAL; }
     if (a->slopes != nullptr && (a->q_rows > (1 << 24) || a->k_rows > (1 << 24))) { set_error("attention: distances are float32: at most 2^24 rows with slopes"); return MMFE_EINVAL; }
     if (!(a->scale > 0.f) || !std::isfinite(a->scale) || !(a->cap >= 0.f) || !std::isfinite(a->cap)) { set_error("attention: scale > 0 and cap >= 0 must be finite"); return MMFE_EINVAL; }
+    if (a->cap > 0.f && !std::isfinite(4.f * a->scale / a->cap)) { set_error("attention: cap is too small against scale"); return MMFE_EINVAL; }
     if (a->packed && (a->q_off == nullptr || a->k_off == nullptr)) { set_error("attention: packed documents need offsets"); return MMFE_EINVAL; }
     if (a->prefix != nullptr && !a->causal) { set_error("attention: a prefix belongs to a causal mask"); return MMFE_EINVAL; }
     const bool any_q = a->q_rows > 0 && (a->packed || a->n_docs > 0), any_k = a->k_rows > 0 && (a->packed || a->n_docs > 0);

@@ -14,7 +14,7 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, raw_stream, require_gpu
+from .plans import OUT_CODES, mark_written, raw_stream, require_gpu
 
 _KINDS = {2.0: N.NORM_2, math.inf: N.NORM_MAX}
 
@@ -74,8 +74,8 @@ def _run(grads, codes, outs, out_codes, kind, max_norm, device: int) -> torch.Te
     # the float32 norm stands behind the call's float64 partial sums
     work = torch.empty(N.grad_partials(n) + 1, dtype=torch.float64, device=grads[0].device)
     norm = work[-1:].view(torch.float32)[0]
-    ptrs = list(map(torch.Tensor.data_ptr, grads))
-    N.grad_clip(ptrs, list(map(torch.Tensor.numel, grads)), codes, None if outs is None else ptrs if outs is grads else list(map(torch.Tensor.data_ptr, outs)),
+    ptrs = map(torch.Tensor.data_ptr, grads)
+    N.grad_clip(ptrs, map(torch.Tensor.numel, grads), codes, None if outs is None else ptrs if outs is grads else map(torch.Tensor.data_ptr, outs),
                 out_codes, kind, max_norm, work.data_ptr(), norm.data_ptr(), device, raw_stream(device))
     return norm
 
@@ -129,15 +129,20 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
         out_device, out_codes, packed = _check(out, "clip_grad_norm: out")
         if out_device != device or not packed or list(map(torch.Tensor.numel, out)) != list(map(torch.Tensor.numel, grads)):
             raise ValueError(f"out: contiguous tensors on GPU {device} with their gradient's number of elements")
-        return _run(grads if contiguous else [t.contiguous() for t in grads], codes, out, out_codes, kind, max_norm, device)
+        norm = _run(grads if contiguous else [t.contiguous() for t in grads], codes, out, out_codes, kind, max_norm, device)
+        mark_written(out)
+        return norm
     if contiguous or all(map(_dense, grads)):
-        return _run(grads, codes, grads, codes, kind, max_norm, device)
+        norm = _run(grads, codes, grads, codes, kind, max_norm, device)
+        mark_written(grads)
+        return norm
     # views with gaps: their values pass through a packed copy
     for t in grads:
         if any(s == 0 and m > 1 for s, m in zip(t.stride(), t.shape)):
             raise ValueError("clip_grad_norm cannot write an expanded gradient")
     packed = [t if _dense(t) else t.contiguous() for t in grads]
     norm = _run(packed, codes, packed, codes, kind, max_norm, device)
+    mark_written(packed)
     for t, p in zip(grads, packed):
         if p is not t:
             t.copy_(p)

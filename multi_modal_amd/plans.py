@@ -11,6 +11,7 @@ from collections import OrderedDict
 from typing import Callable, Dict, Hashable, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable as _once_differentiable
 
 from . import _native as N
 
@@ -42,6 +43,26 @@ def raw_stream(device_index: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def mark_written(tensors) -> None:
+    """Tells autograd that a kernel has overwritten these tensors (it tracks that of its own operations only): a graph that has saved
+    one of them then refuses its backward pass instead of using the new values."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                       # inference tensors are not tracked
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
+def once_differentiable(backward):
+    """torch.autograd.function.once_differentiable where a second derivative is being recorded; the plain function, which takes 10 us
+    less, where none is."""
+    recorded = _once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
 
 # Plans whose key holds caller data (a frame_signal window, a stream handle) form bounded families: the least recently
 # used plan of a full family is dropped from the cache; its device tables are freed when the last reference to it goes (a

@@ -16,7 +16,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, raw_stream, require_gpu
+from .plans import OUT_CODES, mark_written, once_differentiable, raw_stream, require_gpu
 
 _ARGS_SIZE = ctypes.sizeof(N.RotaryArgs)
 
@@ -105,6 +105,8 @@ class Rotary:
             yq, yk = out if k is not None else (out, None)
         else:
             yq, yk = self._run(q, k, positions, False, inplace)
+            if inplace:
+                mark_written(given)
         if q.device != origin:
             yq, yk = yq.to(origin), None if yk is None else yk.to(origin)
         return yq if yk is None else (yq, yk)
@@ -163,6 +165,7 @@ class _RotaryFn(torch.autograd.Function):
         return yq if k is None else (yq, yk)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         gq = grads[0] if ctx.needs_input_grad[0] else None
         gk = grads[1] if len(grads) > 1 and ctx.needs_input_grad[1] else None

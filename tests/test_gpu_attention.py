@@ -134,6 +134,11 @@ PACKED = [
     ([100, 0, 128, 300], 131, 140, 2, 1, 128, HF, False, False, True, 0.0),
     ([7] * 150, 3, 0, 2, 2, 32, BF, True, True, False, 0.0),
     ([0, 0], 4, 9, 2, 1, 64, HF, True, False, False, 0.0),
+    ([], 0, 130, 2, 1, 64, BF, True, False, False, 0.0),
+    ([3, 0, 130] * 60 + [257], 0, 300, 2, 1, 64, HF, True, False, False, 0.0),
+    ([0, 200, 1, 0] * 40, 200, 0, 2, 2, 32, BF, False, False, True, 0.0),
+    ([60, 61, 300, 2, 0, 128, 129], 1, 1, 12, 2, 128, BF, True, True, True, 9.0),
+    ([700, 40], 0, 0, 8, 2, 64, HF, True, False, True, 0.0),          # a key head's query heads on blocks of their own
 ]
 
 
@@ -380,3 +385,74 @@ def test_refusals(mm):
     assert (fn(q, k[:, :0], v[:, :0]) == 0).all()
     c = fn(q.cpu(), k.cpu(), v.cpu())
     assert not c.is_cuda and torch.equal(c, fn(q, k, v).cpu())
+
+
+def test_empty_calls_and_their_gradients(mm):
+    fn = mm.attention.attention
+    for B, N, S in ((0, 5, 5), (2, 0, 7), (2, 7, 0), (2, 0, 0)):
+        for dtype in (BF, HF):
+            q = torch.randn(B, N, 4, 64, device="cuda", dtype=dtype).requires_grad_()
+            k, v = (torch.randn(B, S, 2, 64, device="cuda", dtype=dtype).requires_grad_() for _ in "kv")
+            o, lse = fn(q, k, v, return_lse=True)
+            assert o.shape == q.shape and (o == 0).all() and lse.shape == (B, 4, N) and (S > 0 or (lse == -math.inf).all())
+            for t, x in zip(torch.autograd.grad(o, [q, k, v], torch.ones_like(o)), (q, k, v)):
+                assert t.shape == x.shape and (t == 0).all()
+
+
+def test_changed_inputs_are_noticed(mm):
+    """What the backward pass reads must be what the forward pass read; a second derivative is refused."""
+    fn = mm.attention.attention
+    lengths = torch.tensor([5, 9], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 9, 2, 64, device="cuda", dtype=BF).requires_grad_()
+    o = fn(q, q, q, lengths=lengths)
+    lengths.fill_(3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o.sum(), [q])
+    o = fn(q, q, q)
+    (g,) = torch.autograd.grad(o.float().square().sum(), [q], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [q])
+    x = torch.randn(2, 9, 2, 64, device="cuda", dtype=BF).requires_grad_()
+    y = x * 1.0
+    z = (y * y).sum()
+    rot = mm.Rotary([8])
+    with torch.no_grad():
+        rot(y, None, mm.grid_positions(9, device="cuda"), inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+def test_cache_past_32_bits(mm):
+    """Keys and values of 2.6e9 elements each: the last head of the last rows lies past 2^32 bytes and past 2^31 elements."""
+    fn = mm.attention.attention
+    S, K, D = 640_000, 32, 128
+    k, v = (torch.empty(1, S, K, D, dtype=BF, device="cuda").normal_() for _ in "kv")
+    q = torch.randn(1, 3, K, D, device="cuda").to(BF)
+    o = fn(q, k, v, causal=True)
+    far = fn(q[:, :1], k[:, -200:], v[:, -200:])                     # the end alone
+    for h in (0, 31):
+        for kk, vv, n, got in ((k[0, :, h], v[0, :, h], 3, o), (k[0, -200:, h], v[0, -200:, h], 1, far)):
+            s = (q[0, :n, h].double() @ kk.double().T) * D ** -0.5
+            if n == 3:
+                s[0, -2:] = s[1, -1] = -math.inf
+            p = torch.softmax(s, 1)
+            ref, size = p @ vv.double(), p @ vv.double().abs()
+            assert ((got[0, :n, h].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -14 * size + 2.0 ** -8 * (p * p @ vv.double().square()).sqrt() * 6).all()
+    del k, v
+
+
+def test_many_documents(mm):
+    """70 000 documents of 0 to 3 tokens: each one is what it is in a batch of its own."""
+    fn = mm.attention.attention
+    gen = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 4, (70000,), generator=gen)
+    off = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).to(torch.int32).cuda()
+    T = int(off[-1])
+    q, k, v = (torch.randn(T, 1, 64, generator=gen).to(BF).cuda() for _ in "qkv")
+    o = fn(q, k, v, offsets=off, causal=True)
+    first = torch.zeros(T, dtype=torch.bool, device="cuda")
+    first[off[:-1][lens.cuda() > 0].long()] = True
+    assert torch.equal(o[first], v[first])                            # a document's first row sees itself alone
+    d = int((lens == 3).nonzero()[-1])
+    s = slice(int(off[d]), int(off[d]) + 3)
+    assert torch.equal(o[s], fn(q[None, s], k[None, s], v[None, s], causal=True)[0])

@@ -199,7 +199,7 @@ def test_attention_entries_refuse(N):
     good = forward()
     assert good not in (0, -1) and backward() == good
     wrong = [dict(struct_size=8), dict(dtype=0), dict(dim=12), dict(dim=136), dict(dim=0), dict(n_docs=-1), dict(q_rows=-1), dict(k_rows=1 << 31), dict(heads=3),
-             dict(kv_heads=0), dict(scale=0.0), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(packed=1), dict(packed=1, n_docs=0), dict(prefix=A), dict(q=None), dict(k=None),
+             dict(kv_heads=0), dict(scale=0.0), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.nan), dict(cap=1e-39), dict(packed=1), dict(packed=1, n_docs=0), dict(prefix=A), dict(q=None), dict(k=None),
              dict(v=None), dict(out=None), dict(q=A + 8), dict(k_stride=(2560, 260, 64)), dict(v_stride=(2560, 256, 65)), dict(out_stride=(4, 256, 64)),
              dict(k_stride=(0, 1 << 25, 64)), dict(q_stride=(-8, 256, 64)), dict(slopes=A, k_rows=1 << 25)]
     assert lib.mmfe_attention_forward(ctypes.byref(args(k_rows=10 ** 6)), None, 99, None) == -1          # 10 rows over many keys: a workspace
