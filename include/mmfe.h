@@ -347,7 +347,8 @@ typedef struct mmfe_attention_grads {
     void *grad_q, *grad_k, *grad_v;
     int64_t grad_out_stride[3], grad_q_stride[3], grad_k_stride[3], grad_v_stride[3];
 } mmfe_attention_grads;
-/* Bytes of the workspace mmfe_attention_backward needs (as mmfe_attention_workspace). */
+/* Bytes of the workspace mmfe_attention_backward needs (as mmfe_attention_workspace).  0: none, and neither out nor out_rest is read
+ * (documents of up to 256 rows and keys, a key head per query head, head size up to 64). */
 int64_t mmfe_attention_backward_workspace(const mmfe_attention_args* args);
 int mmfe_attention_backward(const mmfe_attention_args* args, const mmfe_attention_grads* grads, void* workspace, int device, void* hip_stream);
 

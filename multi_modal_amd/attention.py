@@ -73,24 +73,28 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 class _Call:
     """One checked call: what does not depend on the outputs."""
 
-    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "device", "q_stride", "k_stride", "v_stride")
+    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "device", "q_stride", "k_stride", "v_stride", "backward_bytes")
 
     def args(self, q, k, v, out, rest, lse) -> bytes:
         H, n = q.shape[-2], q.shape[-3]
         return N.pack_attention(
             _ARGS_SIZE, OUT_CODES[q.dtype], self.n_docs, H, k.shape[-2], q.shape[-1], self.packed, self.causal, self.scale, self.cap, n, k.shape[-3],
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(self.q_len), _ptr(self.k_len), _ptr(self.q_off), _ptr(self.k_off), _ptr(self.prefix),
-            _ptr(self.slopes), out.data_ptr(), _ptr(rest), _ptr(lse), *self.q_stride, *self.k_stride, *self.v_stride, *_packed_strides(out), H * n, n)
+            _ptr(self.slopes), _ptr(out), _ptr(rest), _ptr(lse), *self.q_stride, *self.k_stride, *self.v_stride, *_packed_strides(q), H * n, n)
 
-    def forward(self, q, k, v, want_lse: bool, want_rest: bool = False):
+    def forward(self, q, k, v, want_lse: bool, gradients: bool = False):
         device = q.device
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        rest = torch.empty(q.shape, dtype=q.dtype, device=device) if want_rest else None
-        lse = None
+        rest = lse = None
         if want_lse:
             shape = (q.shape[-2], q.shape[-3])
             lse = torch.empty(shape if self.packed else (q.shape[0],) + shape, dtype=torch.float32, device=device)
-        args = self.args(q, k, v, out, rest, lse)
+        args = self.args(q, k, v, out, None, lse)
+        if gradients:
+            self.backward_bytes = N.attention_workspace(args, backward=True)
+            if self.backward_bytes:            # 0: the backward pass reads neither out nor its rest
+                rest = torch.empty(q.shape, dtype=q.dtype, device=device)
+                args = self.args(q, k, v, out, rest, lse)
         need = N.attention_workspace(args) if q.shape[-3] <= 64 and not self.packed else 0
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         N.attention_forward(args, _ptr(work), self.device, raw_stream(self.device))
@@ -103,7 +107,7 @@ class _AttentionFn(torch.autograd.Function):
         out, rest, lse = call.forward(q, k, v, True, True)
         ctx.call = call
         # the counts too: autograd then notices when one of them has been changed before the backward pass
-        ctx.save_for_backward(q, k, v, out, rest, lse, call.q_len, call.k_len, call.q_off, call.k_off, call.prefix, call.slopes)
+        ctx.save_for_backward(q, k, v, out if call.backward_bytes else None, rest, lse, call.q_len, call.k_len, call.q_off, call.k_off, call.prefix, call.slopes)
         ctx.mark_non_differentiable(lse)
         return out, lse
 
@@ -116,9 +120,8 @@ class _AttentionFn(torch.autograd.Function):
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         kv_stride = _packed_strides(gk)
         grads = N.pack_attention_grads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *g_stride, *_packed_strides(gq), *kv_stride, *kv_stride)
-        args = call.args(q, k, v, out, rest, lse)
-        work = torch.empty(N.attention_workspace(args, backward=True), dtype=torch.uint8, device=q.device)
-        N.attention_backward(args, grads, work.data_ptr(), call.device, raw_stream(call.device))
+        work = torch.empty(call.backward_bytes, dtype=torch.uint8, device=q.device) if call.backward_bytes else None
+        N.attention_backward(call.args(q, k, v, out, rest, lse), grads, _ptr(work), call.device, raw_stream(call.device))
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None
 

@@ -40,6 +40,7 @@ struct BackwardArgs {
     float *lse2, *delta;              // like lse: lse in log2 units (less the shift of p; +inf for rows without keys), g . o
     u32x4* aux;                       // like lse, 16 bytes: both again in the form keys_kernel takes (see there)
     float *part_k, *part_v;           // keys_kernel, one block per query head: (heads, keys, dim) gradients to be summed over the heads that share
+    bool whole;                       // whole_kernel serves the call
     int sub;                          // ... and how many blocks a key head's query heads are spread over (1 or group)
     int64_t lse_b, lse_h;
     float *norm_g, *norm_v;           // float16: largest squared row norm of each 128-row tile, (heads, q_slots) and (kv_heads, k_slots)
@@ -74,6 +75,20 @@ __device__ __forceinline__ u32x2 thirds(float v) {
     const unsigned b = pack2<true>(r, 0.f);
     const unsigned c = pack2<true>(r - widen<true>(b, 0), 0.f);
     return u32x2{(a & 0xffffu) | b << 16, c & 0xffffu};
+}
+
+// What keys_kernel adds to a row's products: in log2 units beside a capped score, in the products' own otherwise.  -1e30: p = 0
+__device__ __forceinline__ float row_add(const Problem& p, float lse2) {
+    const float add = p.cap > 0.f ? p.cap * kLog2e - lse2 : -lse2 / (p.scale * kLog2e);
+    return add < -1e30f ? -1e30f : add;                // a NaN stays one
+}
+
+// 2^(6 - ceil(log2(bound)))
+__device__ __forceinline__ float phi_of(float bound) {
+    if (!(bound > 0.f) || !(bound < 3e38f)) return 1.f;
+    int e;
+    (void)frexpf(bound, &e);                           // bound < 2^e
+    return ldexpf(1.f, 6 - e);
 }
 
 // What both passes need of every row: delta and lse2 (blocks below q_blocks, 128 rows of one head each), and for float16 the tiles' largest
@@ -119,9 +134,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const BackwardArgs a)
                 if (l == -INFINITY) dot = 0.f;
                 a.lse2[at] = l2;
                 a.delta[at] = dot;
-                // keys_kernel adds these to its products: in log2 units beside a capped score, in the products' own otherwise.  -1e30: p = 0
-                const float add = p.cap > 0.f ? p.cap * kLog2e - l2 : -l2 / (p.scale * kLog2e);
-                const u32x2 x = thirds(add < -1e30f ? -1e30f : add), y = thirds(-dot);
+                const u32x2 x = thirds(row_add(p, l2)), y = thirds(-dot);
                 a.aux[at] = u32x4{x.x, x.y, y.x, y.y};
             }
         }
@@ -167,11 +180,7 @@ __device__ __forceinline__ float find_phi(const BackwardArgs& a, const Doc& d, i
             for (int i = threadIdx.x; i < tq; i += blockDim.x) g = max2(g, ng[(int64_t)h * a.q_slots + i]);
         const float* nv = a.norm_v + slot(a.p, d, false, 0) + (int64_t)kvh * a.k_slots;
         for (int i = threadIdx.x; i < tk; i += blockDim.x) v = max2(v, nv[i]);
-        const float bound = sqrtf(block_max(g, lds)) * sqrtf(block_max(v, lds));
-        if (!(bound > 0.f) || !(bound < 3e38f)) return 1.f;
-        int e;
-        (void)frexpf(bound, &e);                       // bound < 2^e
-        return ldexpf(1.f, 6 - e);
+        return phi_of(sqrtf(block_max(g, lds)) * sqrtf(block_max(v, lds)));
     }
 }
 
@@ -424,9 +433,10 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const BackwardArgs a, int
     }
 }
 
-// dq of 128 rows, 32 per wave, over tiles of 32 keys; steps overlap as in keys_kernel.
+// dq of 128 rows, 32 per wave, over tiles of 32 keys; steps overlap as in keys_kernel.  Head size 64 is held to 168 registers for three waves
+// a SIMD (6 of them spilled): 8192 rows, 12 heads, 840 -> 954 TFLOP/s without a mask, 871 -> 830 under a causal one.
 template <bool BF, int DP, bool CAP>
-__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a) {
+__global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [k tile][v tile]
     const Problem& p = a.p;
     constexpr int kKeys = 32;
@@ -516,10 +526,218 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const BackwardArgs a)
     store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi * sh.factor(), lim > 1);       // a softmax over one key is constant
 }
 
+// ---- short documents ----
+//
+// Documents of up to 256 rows and keys (a clip's 192 patches and class token) with a key head per query head and a head size up to 64: one block
+// does all of a head's gradients, with all keys and values in LDS for dq, then all queries and g for dk and dv.  Two such blocks share a CU, so
+// that one's loads run beside the other's products.  The tensors are read from memory once (the second time from L2), delta is
+// the sum of p dp over the keys, taken in a first walk over them, and neither o nor what its rounding lost is read, or has to be stored by the
+// forward pass.  Bound by memory and by the products about equally.  64 clips of 193 rows, 12 heads of 64: FIXME us; the two passes
+// above and the launch before them take 105, their blocks waiting for their first tiles most of the time.
+constexpr int kWholeRows = 256;
+
+template <bool BF, int DP, bool CAP>
+__global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a, int padded_rows) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // [k or q][v or g] of padded_rows rows, statistics of the rows, kWaves floats
+    const Problem& p = a.p;
+    constexpr int kTileBytes = 32 * DP * 2;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    const int head = blockIdx.x % p.heads;
+    Doc d;
+    (void)find_doc<true>(p, blockIdx.x / p.heads, kWholeRows, d);     // one tile per document
+    const int nq = d.nq, nk = d.nk, off = nk - nq;
+    const int tq = (nq + 31) / 32, tk = (nk + 31) / 32;
+    const bool any = nq > 0 && nk > 0;
+    char* second = smem + padded_rows * DP * 2;
+    u32x4* stats = reinterpret_cast<u32x4*>(second + padded_rows * DP * 2);
+    float* scratch = reinterpret_cast<float*>(stats + padded_rows);
+    const unsigned lds0 = lds_address(smem), lds1 = lds0 + padded_rows * DP * 2;
+    auto limit = [&](int r) { return p.causal ? min(nk, max(d.prefix, min(r, nq - 1) + off + 1)) : nk; };
+    auto first_row = [&](int j) { return p.causal && j >= d.prefix ? max(0, j - off) : 0; };
+    typedef Loader<DP, 32, kWaves> Load;
+    auto load_all = [&](const Rows& x, const Rows& y, int tiles, int rows) {
+        Load lx, ly;
+        lx.init(p.dim, x.n, wave);
+        ly.init(p.dim, y.n, wave);
+        for (int t = 0; t < tiles; ++t) {
+            lx.load(row_base(x, d, t * 32, head), rows - t * 32, p.dim, x.n, uniform(lds0 + t * kTileBytes), wave);
+            ly.load(row_base(y, d, t * 32, head), rows - t * 32, p.dim, y.n, uniform(lds1 + t * kTileBytes), wave);
+        }
+    };
+    Shape<CAP> sh;
+    sh.set(p, head);
+    const float back = __builtin_amdgcn_exp2f(-kShift<BF>);
+
+    // dq: a wave has rows 32 wave .. and 128 + 32 wave ..
+    if (any) load_all(p.k, p.v, tk, nk);
+    u32x4 qf[2][DP / 16], gf[2][DP / 16];
+    float lse[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = max(0, min(32 * (wave + 4 * i) + col, nq - 1));
+        load_rows<DP>(qf[i], row_base(p.q, d, r, head), p.dim, any);
+        load_rows<DP>(gf[i], row_base(a.g, d, r, head), p.dim, any);
+        lse[i] = any ? a.lse[d.batch * a.lse_b + head * a.lse_h + r] : 0.f;
+    }
+    wait_all();
+    block_sync();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        arrived(qf[i]);
+        arrived(gf[i]);
+        asm volatile("" : "+v"(lse[i]));
+    }
+    float phi = 1.f;
+    if constexpr (!BF) {
+        float g = 0.f, v = 0.f;
+        if (any)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float sg = 0.f, sv = 0.f;
+                const int t = min(wave + 4 * i, tk - 1);
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) {
+                    const u32x4 vf = read_rows<DP>(second + t * kTileBytes, 0, s);       // rows past the last repeat it; pieces past the head
+                    const bool in = 16 * s + 8 * half < p.dim;                           // size repeat the first, and are left out
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = widen<BF>(gf[i][s][e >> 1], e & 1), y = in ? widen<BF>(vf[e >> 1], e & 1) : 0.f;
+                        sg = fmaf(x, x, sg);
+                        sv = fmaf(y, y, sv);
+                    }
+                }
+                g = max2(g, both_sum(sg));
+                v = max2(v, both_sum(sv));
+            }
+        phi = phi_of(sqrtf(block_max(g, scratch)) * sqrtf(block_max(v, scratch)));
+    }
+    auto products = [&](const u32x4 (&f)[DP / 16], const u32x4 (&h)[DP / 16], int t, f32x16& sx, f32x16& sd) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sx = mfma<BF>(read_rows<DP>(smem + t * kTileBytes, 0, s), f[s], sx);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sd = mfma<BF>(read_rows<DP>(second + t * kTileBytes, 0, s), h[s], sd);
+    };
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        const int w0 = 32 * (wave + 4 * i), row = w0 + col;
+        if (w0 >= p.q_rows) break;
+        const int lim = any && row < nq ? limit(row) : 0, wave_lim = any && w0 < nq ? limit(w0 + 31) : 0, full_lim = any && w0 < nq ? limit(w0) : 0;
+        const float l2 = lse[i] == -INFINITY ? INFINITY : lse[i] * kLog2e - kShift<BF>;
+        const float add = (CAP ? p.cap * kLog2e : 0.f) - l2;
+        f32x16 dq[DP / 32];
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) dq[e] = f32x16{};
+        auto probabilities = [&](int t, f32x16& x, f32x16& dp, f32x16& w) {
+            const int j0 = 32 * t;
+            x = dp = f32x16{};
+            if (i == 0) products(qf[0], gf[0], t, x, dp);
+            else products(qf[1], gf[1], t, x, dp);
+            sh.template apply<false>(x, w, [&](int) { return add; }, (float)(row + off - j0 - 4 * half), -1.f);
+            if (j0 + 32 > full_lim) {
+                const int left = lim - j0 - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = reg_row(e) < left ? x[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = exp2_fast(x[e]);
+        };
+        float sum = 0.f;
+        for (int t = 0; 32 * t < wave_lim; ++t) {
+            f32x16 x, dp, w;
+            probabilities(t, x, dp, w);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum = fmaf(x[e], dp[e], sum);
+        }
+        const float delta = lim > 0 ? both_sum(sum) * back : 0.f;
+        for (int t = 0; 32 * t < wave_lim; ++t) {
+            f32x16 x, dp, w;
+            probabilities(t, x, dp, w);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                dp[e] = (dp[e] - delta) * x[e];
+                if constexpr (!BF) dp[e] *= phi;
+                if constexpr (CAP) dp[e] *= w[e];
+            }
+            accumulate<BF, DP>(dq, smem + t * kTileBytes, 0, dp, nk <= kShortKeys);
+        }
+        if (row < p.q_rows)
+            store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, row, head)), dq, p.dim, p.scale * back / phi * sh.factor(), lim > 1);      // a softmax over one key is constant
+        if (half == 0 && row < nq) {
+            const u32x2 u = thirds(row_add(p, l2)), v = thirds(-delta);
+            stats[row] = u32x4{u.x, u.y, v.x, v.y};
+        }
+    }
+    wait_all();
+    block_sync();                                                     // k and v have been read, the statistics are there
+
+    // dk and dv: a wave has keys 32 wave .. and 128 + 32 wave ..
+    if (any) load_all(p.q, a.g, tq, nq);
+    u32x4 kf[DP / 16], vf[DP / 16];
+    auto load_keys = [&](int i) {
+        const int r = max(0, min(32 * (wave + 4 * i) + col, nk - 1));
+        load_rows<DP>(kf, row_base(p.k, d, r, head), p.dim, any);
+        load_rows<DP>(vf, row_base(p.v, d, r, head), p.dim, any);
+    };
+    load_keys(0);
+    wait_all();
+    block_sync();
+    const u32x4 ones = half == 0 ? u32x4{0x3f803f80u, 0x00003f80u, 0u, 0u} : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        const int w0 = 32 * (wave + 4 * i), key = w0 + col;
+        if (w0 >= p.k_rows) break;
+        if (i == 1) load_keys(1);
+        const int wave_first = any && w0 < nk ? first_row(w0) : nq, wave_full = first_row(min(w0 + 31, nk - 1)), my_first = first_row(key);
+        f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) dk[e] = dv[e] = f32x16{};
+        for (int t = wave_first / 32; t < tq && wave_first < nq; ++t) {
+            const int i0 = 32 * t;
+            const u32x4 st = stats[min(i0 + col, nq - 1)];
+            f32x16 x{}, dp, w, add;
+            const f32x16 lo = mfma<true>(u32x4{st.x, st.y, 0u, 0u}, ones, f32x16{});
+            if constexpr (CAP) add = lo;
+            else x = lo;
+            dp = mfma<true>(u32x4{st.z, st.w, 0u, 0u}, ones, f32x16{});
+            products(kf, vf, t, x, dp);
+            sh.template apply<true>(x, w, [&](int e) { return add[e]; }, (float)(i0 + 4 * half + off - key), 1.f);
+            if (i0 < wave_full || i0 + 32 > nq) {
+                const int from = my_first - i0 - 4 * half, to = nq - i0 - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = reg_row(e) >= from && reg_row(e) < to ? x[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x[e] = exp2_fast(x[e]);
+                dp[e] *= x[e];
+                if constexpr (!BF) dp[e] *= phi;
+                if constexpr (CAP) dp[e] *= w[e];
+            }
+            accumulate<BF, DP>(dv, second + t * kTileBytes, 0, x, nk <= kShortKeys);
+            accumulate<BF, DP>(dk, smem + t * kTileBytes, 0, dp, nk <= kShortKeys);
+        }
+        if (key < p.k_rows) {
+            const bool some = key < nk && wave_first < nq;
+            store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, key, head)), dk, p.dim, p.scale * back / phi * sh.factor(), some && nk > 1);
+            store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, key, head)), dv, p.dim, back, some);
+        }
+    }
+}
+
 template <bool BF, int DP, bool CAP>
 int launch(BackwardArgs& b, hipStream_t stream) {
     Problem& p = b.p;
     int rc = MMFE_OK, blocks = 1, cus = 256;
+    if constexpr (DP <= 64)
+        if (b.whole) {
+            const int rows = (int)((p.q_rows > p.k_rows ? p.q_rows : p.k_rows) + 31) / 32 * 32;
+            const auto fn = &whole_kernel<BF, DP, CAP>;
+            const size_t lds = (size_t)rows * (2 * DP * 2 + 16) + kWaves * 4;
+            if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
+            p.tiles = 1;
+            hipLaunchKernelGGL(fn, dim3((uint32_t)(p.n_docs * p.heads)), dim3(kThreads), lds, stream, b, rows);
+            return launched("attention backward");
+        }
     const int64_t tk = count_tiles(p, p.k_rows, kRows);
     b.k_tiles = p.tiles;
     const int64_t tq = count_tiles(p, p.q_rows, kRows);
@@ -559,6 +777,10 @@ int64_t slots(const mmfe_attention_args* a, int64_t rows) {
     const int64_t tiles = (rows + kRows - 1) / kRows;
     return a->packed ? tiles + a->n_docs + 1 : tiles * a->n_docs;
 }
+bool is_whole(const mmfe_attention_args* a) {
+    return !a->packed && a->n_docs > 0 && a->heads == a->kv_heads && a->dim <= 64 && a->q_rows <= kWholeRows && a->k_rows <= kWholeRows && a->q_rows + a->k_rows > 0;
+}
+
 // Blocks that a key head's query heads are spread over: one, or one per query head (whose parts a second launch sums in float32)
 // where one would leave fewer than 1024 blocks, 4 a CU, and walk over 2048 rows at least.  4096 rows, 16 heads on 4 of 128: 766 us in 128
 // blocks, 405 in 512 and the sums; at 1024 blocks and more both take the same and the parts' traffic is saved.
@@ -579,6 +801,7 @@ extern "C" {
 int64_t mmfe_attention_backward_workspace(const mmfe_attention_args* a) {
     Problem p{};
     if (make_problem(a, p)) return -1;
+    if (is_whole(a)) return 0;
     const int64_t norms = a->dtype == MMFE_OUT_F16 ? a->heads * slots(a, a->q_rows) + a->kv_heads * slots(a, a->k_rows) : 0;
     return (6 * lse_size(a) + 2 * part_size(a) + norms + 4) * (int64_t)sizeof(float);
 }
@@ -589,9 +812,10 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     if (rc) return rc;
     if (g == nullptr || g->struct_size != (int32_t)sizeof(mmfe_attention_grads)) { set_error("attention: gradients NULL or of another version"); return MMFE_EINVAL; }
     const bool any_q = a->q_rows > 0 && (a->packed || a->n_docs > 0), any_k = a->k_rows > 0 && (a->packed || a->n_docs > 0);
-    if (any_q && (a->out == nullptr || a->lse == nullptr || g->grad_out == nullptr || g->grad_q == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
+    const bool whole = is_whole(a);
+    if (any_q && ((a->out == nullptr && !whole) || a->lse == nullptr || g->grad_out == nullptr || g->grad_q == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
     if (any_k && (g->grad_k == nullptr || g->grad_v == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
-    if ((any_q || any_k) && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
+    if ((any_q || any_k) && !whole && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride) || bad_rows("grad_out", g->grad_out, g->grad_out_stride) || bad_rows("grad_q", g->grad_q, g->grad_q_stride) ||
         bad_rows("grad_k", g->grad_k, g->grad_k_stride) || bad_rows("grad_v", g->grad_v, g->grad_v_stride)) return MMFE_EINVAL;
@@ -602,6 +826,7 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     b.out = rows(a->out, a->out_stride); b.rest = static_cast<const char*>(a->out_rest); b.g = rows(g->grad_out, g->grad_out_stride);
     b.dq = rows(g->grad_q, g->grad_q_stride); b.dk = rows(g->grad_k, g->grad_k_stride); b.dv = rows(g->grad_v, g->grad_v_stride);
     b.lse = a->lse; b.lse_b = a->lse_stride[0]; b.lse_h = a->lse_stride[1];
+    b.whole = whole;
     b.sub = spread(a);
     b.aux = static_cast<u32x4*>(workspace);
     b.part_k = reinterpret_cast<float*>(b.aux + lse_size(a)); b.part_v = b.part_k + part_size(a);

@@ -214,6 +214,8 @@ def test_attention_entries_refuse(N):
                dict(grad_k_stride=(2560, 256, 4))):
         assert backward(grads=kw) == -1, kw
     assert backward(lse=None) == -1 and backward(work=None) == -1 and backward(work=A + 4) == -1
+    assert lib.mmfe_attention_backward_workspace(ctypes.byref(args(kv_heads=4))) == 0                     # short documents: no workspace, no out
+    assert backward(kv_heads=4, work=None, out=None) == good and backward(kv_heads=4, lse=None) == -1
     assert lib.mmfe_attention_backward_workspace(ctypes.byref(args())) > 0 and lib.mmfe_attention_backward_workspace(ctypes.byref(args(dim=9))) == -1
     assert lib.mmfe_attention_forward(None, None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, None, 0, None) == -1
     assert forward(n_docs=0, q=None, k=None, v=None, out=None) == 0 and forward(q_rows=0, q=None, out=None) == 0
