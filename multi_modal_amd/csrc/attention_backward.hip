@@ -529,16 +529,20 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
 // ---- short documents ----
 //
 // Documents of up to 256 rows and keys (a clip's 192 patches and class token) with a key head per query head and a head size up to 64: one block
-// does all of a head's gradients, with all keys and values in LDS for dq, then all queries and g for dk and dv.  Two such blocks share a CU, so
-// that one's loads run beside the other's products.  The tensors are read from memory once (the second time from L2), delta is
+// does all of a head's gradients, with q, k, v and g in LDS, a wave for every 32 rows and then for the 32 keys of the same numbers.  Eight
+// waves and one block per CU; documents of up to 128 take four, and two blocks share a CU.  The tensors are read from memory once, delta is
 // the sum of p dp over the keys, taken in a first walk over them, and neither o nor what its rounding lost is read, or has to be stored by the
-// forward pass.  Bound by memory and by the products about equally.  64 clips of 193 rows, 12 heads of 64: FIXME us; the two passes
-// above and the launch before them take 105, their blocks waiting for their first tiles most of the time.
+// forward pass.  Bound by the vector instructions around the three exponentials of each score, with the products beside them only in part.
+// 64 clips of 193 rows, 12 heads of 64, float16: 87 us (in four waves with two groups of rows each, two blocks a CU and q and g brought after
+// k and v, 92; by the two passes above and the launch before them, whose blocks wait for their first tiles most of the time, 105), and the
+// forward pass 29 in place of 34 us.
 constexpr int kWholeRows = 256;
+template <int DP, int WAVES>
+constexpr int kWholeLoad = WAVES * 512 / DP;           // rows that one DMA of each wave brings
 
-template <bool BF, int DP, bool CAP>
-__global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a, int padded_rows) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];       // [k or q][v or g] of padded_rows rows, statistics of the rows, kWaves floats
+template <bool BF, int DP, bool CAP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) whole_kernel(const BackwardArgs a, int padded_rows) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];       // k, v, q, g of padded_rows rows each, statistics of the rows, WAVES floats
     const Problem& p = a.p;
     constexpr int kTileBytes = 32 * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -546,83 +550,81 @@ __global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a
     Doc d;
     (void)find_doc<true>(p, blockIdx.x / p.heads, kWholeRows, d);     // one tile per document
     const int nq = d.nq, nk = d.nk, off = nk - nq;
-    const int tq = (nq + 31) / 32, tk = (nk + 31) / 32;
+    const int tq = (nq + 31) / 32;
     const bool any = nq > 0 && nk > 0;
-    char* second = smem + padded_rows * DP * 2;
-    u32x4* stats = reinterpret_cast<u32x4*>(second + padded_rows * DP * 2);
+    const int part = padded_rows * DP * 2;
+    const char *lk = smem, *lv = lk + part, *lq = lv + part, *lg = lq + part;
+    u32x4* stats = reinterpret_cast<u32x4*>(smem + 4 * part);
     float* scratch = reinterpret_cast<float*>(stats + padded_rows);
-    const unsigned lds0 = lds_address(smem), lds1 = lds0 + padded_rows * DP * 2;
+    const unsigned lds0 = lds_address(smem);
     auto limit = [&](int r) { return p.causal ? min(nk, max(d.prefix, min(r, nq - 1) + off + 1)) : nk; };
     auto first_row = [&](int j) { return p.causal && j >= d.prefix ? max(0, j - off) : 0; };
-    typedef Loader<DP, 32, kWaves> Load;
-    auto load_all = [&](const Rows& x, const Rows& y, int tiles, int rows) {
+    constexpr int kLoad = kWholeLoad<DP, WAVES>;
+    typedef Loader<DP, kLoad, WAVES> Load;
+    auto load = [&](const Rows& x, const Rows& y, int rows, unsigned lds) {
         Load lx, ly;
         lx.init(p.dim, x.n, wave);
         ly.init(p.dim, y.n, wave);
-        for (int t = 0; t < tiles; ++t) {
-            lx.load(row_base(x, d, t * 32, head), rows - t * 32, p.dim, x.n, uniform(lds0 + t * kTileBytes), wave);
-            ly.load(row_base(y, d, t * 32, head), rows - t * 32, p.dim, y.n, uniform(lds1 + t * kTileBytes), wave);
+        for (int r = 0; r < rows; r += kLoad) {
+            lx.load(row_base(x, d, r, head), rows - r, p.dim, x.n, uniform(lds + r * DP * 2), wave);
+            ly.load(row_base(y, d, r, head), rows - r, p.dim, y.n, uniform(lds + part + r * DP * 2), wave);
         }
     };
+    if (any) {
+        load(p.k, p.v, nk, lds0);
+        load(p.q, a.g, nq, lds0 + 2 * part);
+    }
     Shape<CAP> sh;
     sh.set(p, head);
     const float back = __builtin_amdgcn_exp2f(-kShift<BF>);
-
-    // dq: a wave has rows 32 wave .. and 128 + 32 wave ..
-    if (any) load_all(p.k, p.v, tk, nk);
-    u32x4 qf[2][DP / 16], gf[2][DP / 16];
-    float lse[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = max(0, min(32 * (wave + 4 * i) + col, nq - 1));
-        load_rows<DP>(qf[i], row_base(p.q, d, r, head), p.dim, any);
-        load_rows<DP>(gf[i], row_base(a.g, d, r, head), p.dim, any);
-        lse[i] = any ? a.lse[d.batch * a.lse_b + head * a.lse_h + r] : 0.f;
-    }
+    const int w0 = 32 * wave, mine = w0 + col;                        // a wave's rows, and then its keys
+    float lse = any ? a.lse[d.batch * a.lse_b + head * a.lse_h + min(mine, nq - 1)] : 0.f;
     wait_all();
     block_sync();
+    asm volatile("" : "+v"(lse));
+
+    // dq
+    u32x4 qf[DP / 16], gf[DP / 16];
+    const int own = any ? min(wave, tq - 1) * kTileBytes : 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        arrived(qf[i]);
-        arrived(gf[i]);
-        asm volatile("" : "+v"(lse[i]));
+    for (int s = 0; s < DP / 16; ++s) {
+        qf[s] = read_rows<DP>(lq + own, 0, s);
+        gf[s] = read_rows<DP>(lg + own, 0, s);
     }
     float phi = 1.f;
     if constexpr (!BF) {
         float g = 0.f, v = 0.f;
-        if (any)
+        if (any) {
+            const int t = min(wave, (nk - 1) / 32);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float sg = 0.f, sv = 0.f;
-                const int t = min(wave + 4 * i, tk - 1);
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
-                    const u32x4 vf = read_rows<DP>(second + t * kTileBytes, 0, s);       // rows past the last repeat it; pieces past the head
-                    const bool in = 16 * s + 8 * half < p.dim;                           // size repeat the first, and are left out
+            for (int s = 0; s < DP / 16; ++s) {
+                const u32x4 vf = read_rows<DP>(lv + t * kTileBytes, 0, s);               // rows past the last repeat it; pieces past the head
+                if (16 * s + 8 * half < p.dim)                                           // size repeat the first, and are left out
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float x = widen<BF>(gf[i][s][e >> 1], e & 1), y = in ? widen<BF>(vf[e >> 1], e & 1) : 0.f;
-                        sg = fmaf(x, x, sg);
-                        sv = fmaf(y, y, sv);
+                        const float x = widen<BF>(gf[s][e >> 1], e & 1), y = widen<BF>(vf[e >> 1], e & 1);
+                        g = fmaf(x, x, g);
+                        v = fmaf(y, y, v);
                     }
-                }
-                g = max2(g, both_sum(sg));
-                v = max2(v, both_sum(sv));
             }
+            g = both_sum(g);
+            v = both_sum(v);
+        }
         phi = phi_of(sqrtf(block_max(g, scratch)) * sqrtf(block_max(v, scratch)));
     }
-    auto products = [&](const u32x4 (&f)[DP / 16], const u32x4 (&h)[DP / 16], int t, f32x16& sx, f32x16& sd) {
+    // pieces past the head size: zero on one side of each product (k and v there repeat others)
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) sx = mfma<BF>(read_rows<DP>(smem + t * kTileBytes, 0, s), f[s], sx);
+    for (int s = 0; s < DP / 16; ++s)
+        if (16 * s + 8 * half >= p.dim) qf[s] = gf[s] = u32x4{0u, 0u, 0u, 0u};
+    auto products = [&](const char* a, const char* b, const u32x4 (&f)[DP / 16], const u32x4 (&h)[DP / 16], f32x16& sx, f32x16& sd) {
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) sd = mfma<BF>(read_rows<DP>(second + t * kTileBytes, 0, s), h[s], sd);
+        for (int s = 0; s < DP / 16; ++s) sx = mfma<BF>(read_rows<DP>(a, 0, s), f[s], sx);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) sd = mfma<BF>(read_rows<DP>(b, 0, s), h[s], sd);
     };
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        const int w0 = 32 * (wave + 4 * i), row = w0 + col;
-        if (w0 >= p.q_rows) break;
-        const int lim = any && row < nq ? limit(row) : 0, wave_lim = any && w0 < nq ? limit(w0 + 31) : 0, full_lim = any && w0 < nq ? limit(w0) : 0;
-        const float l2 = lse[i] == -INFINITY ? INFINITY : lse[i] * kLog2e - kShift<BF>;
+    if (w0 < p.q_rows) {
+        const int lim = any && mine < nq ? limit(mine) : 0, wave_lim = any && w0 < nq ? limit(w0 + 31) : 0, full_lim = any && w0 < nq ? limit(w0) : 0;
+        const float l2 = lse == -INFINITY ? INFINITY : lse * kLog2e - kShift<BF>;
         const float add = (CAP ? p.cap * kLog2e : 0.f) - l2;
         f32x16 dq[DP / 32];
 #pragma unroll
@@ -630,9 +632,8 @@ __global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a
         auto probabilities = [&](int t, f32x16& x, f32x16& dp, f32x16& w) {
             const int j0 = 32 * t;
             x = dp = f32x16{};
-            if (i == 0) products(qf[0], gf[0], t, x, dp);
-            else products(qf[1], gf[1], t, x, dp);
-            sh.template apply<false>(x, w, [&](int) { return add; }, (float)(row + off - j0 - 4 * half), -1.f);
+            products(lk + t * kTileBytes, lv + t * kTileBytes, qf, gf, x, dp);
+            sh.template apply<false>(x, w, [&](int) { return add; }, (float)(mine + off - j0 - 4 * half), -1.f);
             if (j0 + 32 > full_lim) {
                 const int left = lim - j0 - 4 * half;
 #pragma unroll
@@ -658,36 +659,30 @@ __global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a
                 if constexpr (!BF) dp[e] *= phi;
                 if constexpr (CAP) dp[e] *= w[e];
             }
-            accumulate<BF, DP>(dq, smem + t * kTileBytes, 0, dp, nk <= kShortKeys);
+            accumulate<BF, DP>(dq, lk + t * kTileBytes, 0, dp, nk <= kShortKeys);
         }
-        if (row < p.q_rows)
-            store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, row, head)), dq, p.dim, p.scale * back / phi * sh.factor(), lim > 1);      // a softmax over one key is constant
-        if (half == 0 && row < nq) {
+        if (mine < p.q_rows)
+            store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, mine, head)), dq, p.dim, p.scale * back / phi * sh.factor(), lim > 1);     // a softmax over one key is constant
+        if (half == 0 && mine < nq) {
             const u32x2 u = thirds(row_add(p, l2)), v = thirds(-delta);
-            stats[row] = u32x4{u.x, u.y, v.x, v.y};
+            stats[mine] = u32x4{u.x, u.y, v.x, v.y};
         }
     }
-    wait_all();
-    block_sync();                                                     // k and v have been read, the statistics are there
-
-    // dk and dv: a wave has keys 32 wave .. and 128 + 32 wave ..
-    if (any) load_all(p.q, a.g, tq, nq);
-    u32x4 kf[DP / 16], vf[DP / 16];
-    auto load_keys = [&](int i) {
-        const int r = max(0, min(32 * (wave + 4 * i) + col, nk - 1));
-        load_rows<DP>(kf, row_base(p.k, d, r, head), p.dim, any);
-        load_rows<DP>(vf, row_base(p.v, d, r, head), p.dim, any);
-    };
-    load_keys(0);
-    wait_all();
+    wait_but<63>();                                                   // the statistics are written; stores may go on
     block_sync();
-    const u32x4 ones = half == 0 ? u32x4{0x3f803f80u, 0x00003f80u, 0u, 0u} : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        const int w0 = 32 * (wave + 4 * i), key = w0 + col;
-        if (w0 >= p.k_rows) break;
-        if (i == 1) load_keys(1);
-        const int wave_first = any && w0 < nk ? first_row(w0) : nq, wave_full = first_row(min(w0 + 31, nk - 1)), my_first = first_row(key);
+
+    // dk and dv
+    if (w0 < p.k_rows) {
+        u32x4 kf[DP / 16], vf[DP / 16];
+        const int at = any ? min(wave, (nk - 1) / 32) * kTileBytes : 0;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const bool in = 16 * s + 8 * half < p.dim;
+            kf[s] = in ? read_rows<DP>(lk + at, 0, s) : u32x4{0u, 0u, 0u, 0u};
+            vf[s] = in ? read_rows<DP>(lv + at, 0, s) : u32x4{0u, 0u, 0u, 0u};
+        }
+        const u32x4 ones = half == 0 ? u32x4{0x3f803f80u, 0x00003f80u, 0u, 0u} : u32x4{0u, 0u, 0u, 0u};
+        const int wave_first = any && w0 < nk ? first_row(w0) : nq, wave_full = first_row(min(w0 + 31, nk - 1)), my_first = first_row(mine);
         f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) dk[e] = dv[e] = f32x16{};
@@ -699,8 +694,8 @@ __global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a
             if constexpr (CAP) add = lo;
             else x = lo;
             dp = mfma<true>(u32x4{st.z, st.w, 0u, 0u}, ones, f32x16{});
-            products(kf, vf, t, x, dp);
-            sh.template apply<true>(x, w, [&](int e) { return add[e]; }, (float)(i0 + 4 * half + off - key), 1.f);
+            products(lq + t * kTileBytes, lg + t * kTileBytes, kf, vf, x, dp);
+            sh.template apply<true>(x, w, [&](int e) { return add[e]; }, (float)(i0 + 4 * half + off - mine), 1.f);
             if (i0 < wave_full || i0 + 32 > nq) {
                 const int from = my_first - i0 - 4 * half, to = nq - i0 - 4 * half;
 #pragma unroll
@@ -713,15 +708,29 @@ __global__ void __launch_bounds__(kThreads, 2) whole_kernel(const BackwardArgs a
                 if constexpr (!BF) dp[e] *= phi;
                 if constexpr (CAP) dp[e] *= w[e];
             }
-            accumulate<BF, DP>(dv, second + t * kTileBytes, 0, x, nk <= kShortKeys);
-            accumulate<BF, DP>(dk, smem + t * kTileBytes, 0, dp, nk <= kShortKeys);
+            accumulate<BF, DP>(dv, lg + t * kTileBytes, 0, x, nk <= kShortKeys);
+            accumulate<BF, DP>(dk, lq + t * kTileBytes, 0, dp, nk <= kShortKeys);
         }
-        if (key < p.k_rows) {
-            const bool some = key < nk && wave_first < nq;
-            store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, key, head)), dk, p.dim, p.scale * back / phi * sh.factor(), some && nk > 1);
-            store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, key, head)), dv, p.dim, back, some);
+        if (mine < p.k_rows) {
+            const bool some = mine < nk && wave_first < nq;
+            store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, mine, head)), dk, p.dim, p.scale * back / phi * sh.factor(), some && nk > 1);
+            store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, mine, head)), dv, p.dim, back, some);
         }
     }
+}
+
+template <bool BF, int DP, bool CAP, int WAVES>
+int launch_whole(BackwardArgs& b, hipStream_t stream) {
+    Problem& p = b.p;
+    constexpr int kLoad = kWholeLoad<DP, WAVES>;
+    const int rows = (int)((p.q_rows > p.k_rows ? p.q_rows : p.k_rows) + kLoad - 1) / kLoad * kLoad;
+    const auto fn = &whole_kernel<BF, DP, CAP, WAVES>;
+    const size_t lds = (size_t)rows * (4 * DP * 2 + 16) + WAVES * 4;
+    int rc, blocks = 1, cus = 256;
+    if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), 64 * WAVES, lds, &blocks, &cus)) != MMFE_OK) return rc;
+    p.tiles = 1;
+    hipLaunchKernelGGL(fn, dim3((uint32_t)(p.n_docs * p.heads)), dim3(64 * WAVES), lds, stream, b, rows);
+    return launched("attention backward");
 }
 
 template <bool BF, int DP, bool CAP>
@@ -729,15 +738,7 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     Problem& p = b.p;
     int rc = MMFE_OK, blocks = 1, cus = 256;
     if constexpr (DP <= 64)
-        if (b.whole) {
-            const int rows = (int)((p.q_rows > p.k_rows ? p.q_rows : p.k_rows) + 31) / 32 * 32;
-            const auto fn = &whole_kernel<BF, DP, CAP>;
-            const size_t lds = (size_t)rows * (2 * DP * 2 + 16) + kWaves * 4;
-            if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
-            p.tiles = 1;
-            hipLaunchKernelGGL(fn, dim3((uint32_t)(p.n_docs * p.heads)), dim3(kThreads), lds, stream, b, rows);
-            return launched("attention backward");
-        }
+        if (b.whole) return p.q_rows <= kWholeRows / 2 && p.k_rows <= kWholeRows / 2 ? launch_whole<BF, DP, CAP, 4>(b, stream) : launch_whole<BF, DP, CAP, 8>(b, stream);
     const int64_t tk = count_tiles(p, p.k_rows, kRows);
     b.k_tiles = p.tiles;
     const int64_t tq = count_tiles(p, p.q_rows, kRows);
