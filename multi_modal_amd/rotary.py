@@ -88,8 +88,8 @@ class Rotary:
                 raise RuntimeError("inplace=True has no gradient: use it under torch.no_grad()")
             if not q.is_cuda:
                 raise ValueError("inplace=True takes tensors on the GPU")
-            if any(s == 0 and m > 1 for t in given for s, m in zip(t.stride(), t.shape)):
-                raise ValueError("inplace=True cannot write an expanded tensor")
+            if any(map(_folded, given)):
+                raise ValueError("inplace=True cannot write a tensor whose elements share memory")
             if k is not None and _share(q, k):
                 raise ValueError("inplace=True: q and k share elements")
             if any(t.stride(3) != 1 and D > 1 for t in given):
@@ -134,6 +134,18 @@ class Rotary:
 
     def close(self) -> None:
         self._h.close()
+
+
+def _folded(t: torch.Tensor) -> bool:
+    """Whether two of t's elements may be one in memory (expanded and overlapping views)."""
+    if t.is_contiguous() or t.numel() == 0:
+        return False
+    reach = 1
+    for s, m in sorted((s, m) for s, m in zip(t.stride(), t.shape) if m > 1):
+        if s < reach:
+            return True
+        reach += s * (m - 1)
+    return False
 
 
 def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
