@@ -51,17 +51,19 @@ def _counts(x, name: str, n: int, device, limit: Optional[int] = None, rising: b
         return None
     if type(x) is torch.Tensor and x.dtype == torch.int32 and x.is_cuda and x.device == device and x.shape == (n,) and x.is_contiguous():
         return x
-    t = torch.as_tensor(x)
+    t = x if isinstance(x, torch.Tensor) else torch.tensor(x, dtype=None if len(x) else torch.int32)
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise TypeError(f"{name} must be integers")
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must hold {n} entries, got {tuple(t.shape)}")
     if not t.is_cuda and n > 0:
         if int(t.min()) < 0 or (limit is not None and int(t.max()) > limit):
-            raise ValueError(f"{name} must lie in [0, {limit}]")
+            raise ValueError(f"{name} must lie in [0, {limit}]" if limit is not None else f"{name} must not be negative")
         if rising and bool((t[1:] < t[:-1]).any()):
             raise ValueError(f"{name} must not fall")
     if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        if t.dtype == torch.int64:                         # entries past 32 bits are out of range, and stay so
+            t = t.clamp(-1, 2**31 - 1)
         t = t.to(device=device, dtype=torch.int32).contiguous()
     return t
 
@@ -197,7 +199,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
         call.k_off = call.q_off if kv_offsets is None else _counts(kv_offsets, "kv_offsets", m + 1, device, s, rising=True)
     else:
         call.q_len = _counts(lengths, "lengths", m, device, n)
-        call.k_len = call.q_len if kv_lengths is lengths else _counts(kv_lengths, "kv_lengths", m, device, s)
+        call.k_len = call.q_len if kv_lengths is lengths and s == n else _counts(kv_lengths, "kv_lengths", m, device, s)
     call.prefix = _counts(prefix, "prefix", m, device)
     call.slopes = None
     if slopes is not None:

@@ -456,3 +456,60 @@ def test_many_documents(mm):
     d = int((lens == 3).nonzero()[-1])
     s = slice(int(off[d]), int(off[d]) + 3)
     assert torch.equal(o[s], fn(q[None, s], k[None, s], v[None, s], causal=True)[0])
+
+
+SHORT = [
+    # lens, N, kv, S, H, D, dtype, causal, prefix, bias, cap: a key head per query head, up to 256 rows and keys
+    ([256, 255, 129, 0], 256, None, 256, 2, 64, HF, True, False, False, 0.0),
+    ([1, 20], 20, [256, 225], 256, 3, 64, BF, False, False, True, 0.0),
+    ([250, 256], 256, [3, 32], 32, 2, 32, HF, True, True, False, 0.0),
+    ([128, 97], 128, None, 128, 2, 64, HF, True, False, True, 12.0),
+    ([33, 32, 31], 33, [64, 65, 128], 128, 1, 40, BF, True, True, False, 6.0),
+    ([130, 7], 130, [129, 256], 256, 2, 8, BF, True, False, False, 0.0),
+    ([160, 193], 193, None, 193, 2, 48, HF, False, False, True, 5.0),
+    ([1, 0, 1], 1, [1, 1, 0], 1, 2, 64, HF, True, False, False, 0.0),
+]
+
+
+@pytest.mark.parametrize("case", SHORT, ids=lambda c: f"{c[0]}x{c[3]}x{c[5]}")
+@pytest.mark.parametrize("size", [1e-4, 1.0, 1e2])
+def test_short_documents(mm, O, case, size):
+    """Around the sizes where one block does a head's gradients, with incoming gradients of every size."""
+    lens, N, kv, S, H, D, dtype, causal, prefix, bias, cap = case
+    B = len(lens)
+    gen = torch.Generator().manual_seed(N * 5 + S + D)
+    q = torch.randn(B, N, H, D, generator=gen).to(dtype).cuda()
+    k, v = (torch.randn(B, S, H, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    g = (torch.randn(B, N, H, D, generator=gen) * size).to(dtype).cuda()
+    m = kv or lens
+    host, opts = {}, dict(causal=causal, cap=cap, lengths=lens, kv_lengths=m)
+    if prefix:
+        host["prefix"] = opts["prefix"] = [x // 2 for x in m]
+    if bias:
+        host["slopes"] = opts["slopes"] = slopes_of(H)
+    for b in range(B):
+        for t, n in ((q, lens[b]), (g, lens[b]), (k, m[b]), (v, m[b])):
+            t[b, n:] = math.nan
+    check(mm, O, q, k, v, docs_padded(lens, m, N, S), opts, g=g, flat=flat4, lse_flat=lse4, host=host)
+    # one row or key more of room, which nothing uses: another launch, the same results within the bounds
+    wide = (torch.cat([t, torch.full_like(t[:, :1], math.nan)], 1) for t in (q, k, v))
+    ref, tol = O.attention(flat4(q), flat4(k), flat4(v), docs_padded(lens, m, N, S), cap=cap, slopes=host.get("slopes"), causal=causal, prefix=host.get("prefix"),
+                           g=flat4(g), **limits(dtype))
+    x = [t.requires_grad_() for t in wide]
+    got = torch.autograd.grad(mm.attention.attention(*x, **opts), x, torch.cat([g, torch.full_like(g[:, :1], math.nan)], 1))
+    for name, t, n in zip(("dq", "dk", "dv"), got, (N, S, S)):
+        assert (t[:, n] == 0).all()
+        within(name, flat4(t[:, :n]), ref[name], tol[name])
+
+
+def test_counts_past_32_bits(mm):
+    """64-bit counts on the device are clamped, not cut off; one list of lengths serves rows and fewer keys."""
+    fn = mm.attention.attention
+    q, k, v = (torch.randn(2, 40, 2, 64, device="cuda").to(BF) for _ in "qkv")
+    assert torch.equal(fn(q, k, v, lengths=torch.tensor([2 ** 32 + 5, 2 ** 40], device="cuda")), fn(q, k, v))
+    assert (fn(q, k, v, lengths=torch.tensor([-2 ** 40, -2 ** 32 + 9], device="cuda")) == 0).all()
+    assert torch.equal(fn(q, k, v, causal=True, prefix=[2 ** 32, 2 ** 33]), fn(q, k, v))
+    lens = [40, 3]
+    with pytest.raises(ValueError):
+        fn(q, k[:, :30], v[:, :30], lengths=lens, kv_lengths=lens)
+    assert fn(q[:0], k[:0], v[:0], lengths=[]).shape == q[:0].shape

@@ -219,3 +219,25 @@ def test_attention_entries_refuse(N):
     assert lib.mmfe_attention_backward_workspace(ctypes.byref(args())) > 0 and lib.mmfe_attention_backward_workspace(ctypes.byref(args(dim=9))) == -1
     assert lib.mmfe_attention_forward(None, None, 0, None) == -1 and lib.mmfe_attention_backward(None, None, None, 0, None) == -1
     assert forward(n_docs=0, q=None, k=None, v=None, out=None) == 0 and forward(q_rows=0, q=None, out=None) == 0
+
+
+def test_attention_counts():
+    """Entries past 32 bits stay out of range (they must not wrap round into it); an empty list fits an empty batch."""
+    from multi_modal_amd.attention import _counts
+    cpu = torch.device("cpu")
+    assert _counts([2 ** 32 + 5], "prefix", 1, cpu).tolist() == [2 ** 31 - 1]
+    assert _counts(torch.tensor([7, 0], dtype=torch.uint8), "lengths", 2, cpu, 7).tolist() == [7, 0]
+    assert _counts([], "lengths", 0, cpu, 5).shape == (0,)
+    for bad, limit, error in (([2 ** 32], 9, ValueError), ([-1], None, ValueError), ([True], 9, TypeError), ([1.0], 9, TypeError), ([1, 2], 9, ValueError)):
+        with pytest.raises(error):
+            _counts(bad, "lengths", 1, cpu, limit)
+    with pytest.raises(ValueError, match="must not fall"):
+        _counts([0, 3, 2], "offsets", 3, cpu, 9, rising=True)
+
+
+def test_folded_views():
+    """What inplace=True refuses to write: views whose elements share memory."""
+    from multi_modal_amd.rotary import _folded
+    x = torch.zeros(2, 5, 12, 8)
+    assert not any(map(_folded, (x, x[:, :, 2:5], x[:, ::2], x.transpose(1, 2), x[:0], x[:, :1], x[..., :3])))
+    assert _folded(x[:, :1].expand(2, 5, 12, 8)) and _folded(x.view(-1).as_strided((1, 9, 2, 8), (0, 8, 8, 1)))
