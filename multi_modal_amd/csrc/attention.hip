@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
 // ---- few rows over many keys ----
 //
 // The rows of one key head are its query heads' rows, row r = (token r / group, query head r % group), so that a group reads its keys
-// once; a block takes 32 of them and one chunk of the keys.  Its 4 waves work on tiles of 32 keys of their own (every fourth one), each
+// once; a block takes 32 of them and one chunk of the keys.  Its 2 waves work on tiles of 32 keys of their own (every other one), each
 // with its own double-buffered LDS tiles and no barrier, and meet once at the end.  Bound by reading k and v: the products run at
 // 32 rows whatever the number of valid ones, and p enters with both halves (hi + rest), which costs nothing here.
 
@@ -569,6 +569,20 @@ split_fn pick_split(int dim) {
 }
 
 // Keys of a chunk and chunks of a unit, or no chunks: the row kernel serves the call.
+//
+// A unit's block takes about 8 us to start and end and 16 (head size 64: 15) per 1000 keys, a block of the row kernel the same for the 4 rows' tiles it
+// shares its keys among, so that cutting pays where blocks are few or, with key heads shared by query heads, few rows would read their keys once
+// per query head.  Measured over 1 to 64 rows, 1 to 128 documents of 200 to 32000 keys, 12 heads and 16 on 4, of 64 and 128, all documents as long as
+// their room and of lengths from 1 to 30 in 32:
+//   - up to 512 keys, and up to 2048 where 256 units fill the CUs: no cut; the row kernel, unless units share keys and its blocks do not all run at
+//     once (128 streams of 500 keys, one row, 16 heads on 4: 26.6 us, row kernel 61.4; 32 of them 17.3 and 18.3; 64 rows of 32 documents
+//     of 1000 keys, 12 heads of 64: 27, cut in 512 keys 75)
+//   - more rows than a unit takes, in 192 blocks of the row kernel or more: the row kernel (64 rows, 32 documents of 8000 keys, 12 heads of 128:
+//     317 us, cut 481; 8 documents, 96 blocks: 166 and 139; 512 rows over 32000 keys, 12 heads of 64: 574 and 159)
+//   - else chunks that make 512 blocks, two on each CU, of 256 keys at least, and of 1024 at most (documents shorter than their room leave chunks
+//     empty) unless that makes more than 2048: 16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 109 / 93 / 100 / 113 us with 512 /
+//     1024 / 2048 / 4096 keys; 32 streams of 2000 keys, one row, 4 key heads of 128: 39 / 34 / 33 with 256 / 512 / 1024.
+// Over all of it a call takes 3 % longer on average than with the best of these choices for it (with even lengths 2.5, uneven 4).
 struct Cut {
     int row_tiles = 0, chunk = 0, n_splits = 0;
     int64_t units = 0;
@@ -576,22 +590,20 @@ struct Cut {
 Cut cut_keys(const mmfe_attention_args* a) {
     Cut c;
     if (a->packed || a->q_rows < 1 || a->n_docs < 1) return c;
-    const int64_t rows = a->q_rows * (a->heads / a->kv_heads);
-    if (a->q_rows > 64 || rows > 1024 || a->k_rows <= kShortKeys) return c;
-    c.row_tiles = (int)((rows + 31) / 32);
-    c.units = (int64_t)a->n_docs * c.row_tiles * a->kv_heads;
-    // About 2048 blocks if every document fills its room (two or more on each CU, so that one's start and end run beside another's reads; and
-    // documents shorter than their room leave chunks empty), but 512 keys where 1024 blocks have them and 256 otherwise: every chunk
-    // costs its block's start and a part to join.  16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 111 / 97 / 104 us with 512 / 1024 /
-    // 2048 keys; 64 streams of 2048: 70 / 61 us with 256 / 512.  Up to 512 keys stay in one block: 8 tiles a wave take less than a second launch.
-    const int64_t all = a->k_rows * c.units;
-    int64_t chunk = ((all + 2047) / 2048 + 127) / 128 * 128;
-    const int64_t least = all >= 512 * 1024 ? 512 : 256;
-    if (chunk < least) chunk = least;
-    if (a->k_rows <= 512) chunk = 512;
+    const int64_t keys = a->k_rows, row_tiles = (a->q_rows * (a->heads / a->kv_heads) + 31) / 32, units = a->n_docs * row_tiles * a->kv_heads;
+    const int64_t blocks = a->n_docs * ((a->q_rows + kRows - 1) / kRows) * a->heads;       // of the row kernel
+    if (keys <= kShortKeys) return c;
+    const bool whole = keys <= 512 || (keys <= 2048 && units >= 256);
+    if (whole ? units >= blocks || blocks <= 512 : units > blocks && blocks >= 192) return c;
+    const int64_t all = keys * units;
+    int64_t chunk = (all + 511) / 512, most = (all + 2047) / 2048;
+    if (most < 1024) most = 1024;
+    chunk = chunk < 256 ? 256 : chunk > most ? most : chunk;
+    chunk = whole ? keys : (chunk + 127) / 128 * 128;
+    c.row_tiles = (int)row_tiles;
+    c.units = units;
     c.chunk = (int)chunk;
-    c.n_splits = (int)((a->k_rows + chunk - 1) / chunk);
-    if (c.n_splits < 1) c.n_splits = 1;
+    c.n_splits = (int)((keys + chunk - 1) / chunk);
     return c;
 }
 

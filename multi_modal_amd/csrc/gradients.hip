@@ -9,7 +9,7 @@
 // Sums are float64 from the first square on: bfloat16 and float32 gradients reach 1e38, whose square float32 cannot hold, and a
 // sum over 1e9 values would lose 2^-24 per step.  (A double-precision fma runs at half the float32 rate here, far above what
 // the memory delivers.)  Every block writes one partial, and the partials are summed in a fixed order: the same list gives the same bits.
-// The blocks of the clipping pass each sum the (at most 2048 per launch) partials again, from L2, instead of waiting for a
+// The blocks of the clipping pass each sum the (at most 1024 per launch) partials again, from L2, instead of waiting for a
 // launch that does it.  When c = 1 and the result goes back in place there is nothing to write and the pass ends there: g * 1 is g.
 #include "mmfe_internal.h"
 
@@ -21,8 +21,11 @@ namespace mmfe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 16384;            // elements of a chunk: 64 (16-bit: 32) KB
-constexpr int kMaxBlocks = 2048;         // blocks, and partials, of one launch
+// Elements of a chunk, and blocks (and partials) of one launch: 4 blocks a CU.  200 bfloat16 tensors of 6.5 million: norm 434 us (6.0 TB/s) and
+// clipping 1467 us (5.4), with 2048 blocks 464 and 1527; 96 tensors of up to 590 thousand float32: clipping 20.9 us, with chunks of 4096 25.4,
+// of 65536 19.7; two small tensors: 5.9 us, 5.4 and 7.5.
+constexpr int kChunk = 16384;
+constexpr int kMaxBlocks = 1024;
 constexpr int kMaxNorm = 160;            // tensors of one launch: 24 bytes each in the argument block
 constexpr int kMaxScale = 112;           // 32 bytes each
 

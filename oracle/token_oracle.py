@@ -47,8 +47,12 @@ def attention_tolerances(r, q, k, v, g, scale, eps, tiny):
     """Bounds on |kernel - exact| of o (and dq, dk, dv).  u = eps / 2 is half a step of the 16-bit type, `tiny` half its smallest
     subnormal.  p is rounded to 16 bits (u relative, or tiny against a largest value of at least 1; with the kernels' scaling of
     float16 gradients the subnormals are 2^-8 of that and left in); p itself carries its score's float32 error es; results are
-    rounded once.  delta is formed from the rounded o."""
-    u, u32 = eps / 2, 2.0 ** -24
+    rounded once.  delta is formed from the rounded o.
+    bfloat16 has float32's exponents, so its subnormals are those of the arithmetic itself, which the exponential and the matrix
+    instructions take as zeros: p, ds and results below 2^-126 may be lost whole.  A lost p is an error of at most 2^-126 in o's and dv's
+    terms and of 2^-126 |dp - delta| <= 2^-126 (|g||v| + |delta|) in ds, a lost ds one of 2^-126."""
+    u, u32, lost = eps / 2, 2.0 ** -24, 2.0 ** -126
+    tiny = max(tiny, lost)
     ep = 1.02 * u + 64 * u32                                        # relative error of a rounded p, without its score's
     tol = {"o": u * r["o"].abs() * 1.01 + ep * r["A"] + 1.1 * r["Ae"] + tiny * (r["sv"] + 1)}
     if g is None:
@@ -61,6 +65,7 @@ def attention_tolerances(r, q, k, v, g, scale, eps, tiny):
     eds = r["ds"].abs() * (ep + 1.1 * es) + p * r["f"] * (edelta + edp) + p * (r["gv"] + r["delta"].abs()) * 16 * u32
     # subnormal ds of float16: relative to the largest possible |g||v| of the document, 2^-29 of it is still a normal number
     eds = eds + r["see"].double() * (tiny * 2.0 ** -3 * float(g.norm(dim=1).max() if g.numel() else 0) * float(v.norm(dim=1).max() if v.numel() else 0))
+    eds = eds + r["see"].double() * lost * (1 + r["gv"] + r["delta"].abs())
     tol["dq"] = 1.01 * u * r["dq"].abs() + scale * (eds @ k.abs()) + tiny
     tol["dk"] = 1.01 * u * r["dk"].abs() + scale * (eds.T @ q.abs()) + tiny
     return tol

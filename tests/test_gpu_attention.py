@@ -513,3 +513,18 @@ def test_counts_past_32_bits(mm):
     with pytest.raises(ValueError):
         fn(q, k[:, :30], v[:, :30], lengths=lens, kv_lengths=lens)
     assert fn(q[:0], k[:0], v[:0], lengths=[]).shape == q[:0].shape
+
+
+MANY = [
+    # as TOKENS: keys in one chunk (shared heads, many streams), and rows of several tiles over many keys
+    (1, [1, 0, 200, 129, 33, 150, 64] * 20, 200, 8, 2, 64, BF, True, False, False, 0.0),
+    (3, [512, 500, 31] * 35, 512, 6, 1, 32, HF, True, False, True, 15.0),
+    (300, [5000, 299, 1024], 5000, 2, 2, 64, HF, True, False, False, 0.0),
+    (129, [2500], 2500, 6, 2, 128, BF, True, True, True, 0.0),
+    (700, [3000, 20], 3000, 3, 1, 40, BF, False, False, False, 9.0),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{c[0]}x{c[2]}x{c[3]}x{c[5]}")
+def test_rows_over_kept_keys(mm, O, case):
+    test_few_rows_over_many_keys(mm, O, case)
