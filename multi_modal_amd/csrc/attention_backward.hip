@@ -7,7 +7,7 @@
 // That is 7 matrix products where one pass with atomic additions into dq would need 5, but every sum has one owner and a fixed
 // order: the same call gives the same bits.  As in the forward pass, products are arranged so that a result is the next operand: the key pass
 // forms scores as rows x keys (a lane has one key), the row pass as keys x rows (a lane has one row); sums over the lane's own index stay in
-// registers for the whole walk.
+// registers for the whole walk.  Where there are few blocks with long walks, the walks are cut into parts that another launch adds up in order.
 //
 // What is rounded: p and ds to the 16-bit type, for the second products; dp and all sums are float32, and delta is formed from o and
 // the rest that its rounding lost.  Short documents add second products with what the rounding of p and ds lost, as the forward pass does.  float16 has 5
@@ -39,9 +39,10 @@ struct BackwardArgs {
     const float* lse;
     float *lse2, *delta;              // like lse: lse in log2 units (less the shift of p; +inf for rows without keys), g . o
     u32x4* aux;                       // like lse, 16 bytes: both again in the form keys_kernel takes (see there)
-    float *part_k, *part_v;           // keys_kernel, one block per query head: (heads, keys, dim) gradients to be summed over the heads that share
+    float *part, *part_v;             // walks cut into parts: their gradients in float32, keys_kernel's (key heads, cuts, keys, dim) of k and then of v,
+                                      // rows_kernel's (cuts, heads, rows, dim)
     bool whole;                       // whole_kernel serves the call
-    int sub;                          // ... and how many blocks a key head's query heads are spread over (1 or group)
+    int k_cuts, q_cuts;               // parts of keys_kernel's walk over the rows, and of rows_kernel's over the keys
     int64_t lse_b, lse_h;
     float *norm_g, *norm_v;           // float16: largest squared row norm of each 128-row tile, (heads, q_slots) and (kv_heads, k_slots)
     int q_slots, k_slots, q_tiles, k_tiles, q_blocks;
@@ -233,6 +234,20 @@ __device__ __forceinline__ void store_rows(char* to, const f32x16 (&o)[DP / 32],
         }
 }
 
+// the same in float32
+template <int DP>
+__device__ __forceinline__ void store_part(float* to, const f32x16 (&o)[DP / 32], int dim, float by, bool some) {
+    const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int e = 32 * i + 8 * g;
+            if (e >= dim) continue;
+            *reinterpret_cast<float4*>(to + e + 4 * half) = some ? make_float4(o[i][4 * g] * by, o[i][4 * g + 1] * by, o[i][4 * g + 2] * by, o[i][4 * g + 3] * by) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+}
+
 template <int DP>
 __device__ __forceinline__ void load_rows(u32x4 (&f)[DP / 16], const char* row, int dim, bool some) {
     const int half = (threadIdx.x >> 5) & 1;
@@ -279,10 +294,10 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
     constexpr int kTileBytes = kTile * DP * 2;
     constexpr int kBuf = 2 * kTileBytes + kTile * 16;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int lot = blockIdx.x % (p.kv_heads * a.sub), kvh = lot % p.kv_heads;
+    const int lot = blockIdx.x % (p.kv_heads * a.k_cuts), kvh = lot % p.kv_heads, cut = lot / p.kv_heads;
     Doc d;
-    if (!find_doc<false>(p, blockIdx.x / (p.kv_heads * a.sub), kRows, d)) return;
-    const int heads = p.group / a.sub, head0 = kvh * p.group + lot / p.kv_heads * heads;         // query heads of this block
+    if (!find_doc<false>(p, blockIdx.x / (p.kv_heads * a.k_cuts), kRows, d)) return;
+    const int head0 = kvh * p.group;
     const int key0 = d.tile * kRows, w0 = key0 + 32 * wave, key = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
     // rows [first, nq) see key j: all of them, or those from j - off on
@@ -292,14 +307,18 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
     const int wave_full = first_row(min(w0 + 31, nk - 1));            // from here on every row sees all keys of the wave
     const int my_first = first_row(key);
     const int t_first = block_first / kTile, t_end = block_first < nq ? (nq + kTile - 1) / kTile : t_first;
-    const int steps = (t_end - t_first) * heads;
+    // the tiles of all query heads, one head after the other, and this block's part of them
+    const int all_steps = (t_end - t_first) * p.group, part_steps = (all_steps + a.k_cuts - 1) / a.k_cuts;
+    const int first_step = min(cut * part_steps, all_steps), steps = min(part_steps, all_steps - first_step);
+    const int first_g = steps > 0 ? first_step / (t_end - t_first) : 0;
 
     typedef Loader<DP, kTile, kWaves> Load;
     Load lq, lg;
     lq.init(p.dim, p.q.n, wave);
     lg.init(p.dim, a.g.n, wave);
     const unsigned lds0 = lds_address(smem);
-    int ask_g = 0, ask_t = t_first, ask = 0;                          // the next tile to ask for
+    int g = first_g, t = t_first + (steps > 0 ? first_step - first_g * (t_end - t_first) : 0);
+    int ask_g = g, ask_t = t, ask = 0;                                // the next tile to ask for
     auto stage = [&]() {
         const int head = head0 + ask_g, r0 = ask_t * kTile;
         const unsigned dst = uniform(lds0 + (ask % kRing) * kBuf);
@@ -340,8 +359,7 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
     arrived(vf);
     if (steps > 0) products(smem, 0, x, dp);
     Shape<CAP> sh;
-    sh.set(p, head0);
-    int g = 0, t = t_first;
+    sh.set(p, head0 + g);
     for (int step = 0; step < steps; ++step) {
         if (step + kRing - 2 < steps) wait_but<2 * Load::kCount>();   // tile step + 1 is there; what step - 1 asked for may be on its way
         else wait_all();
@@ -386,50 +404,48 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
         }
         if (++t == t_end) {
             t = t_first;
-            if (++g < heads) sh.set(p, head0 + g);
+            if (++g < p.group) sh.set(p, head0 + g);
         }
     }
     if (key >= d.rows) return;
     const float back = __builtin_amdgcn_exp2f(-kShift<BF>), fk = p.scale * back / phi * sh.factor();
     const bool any = key < nk && steps > 0, any_k = any && nk > 1;    // a softmax over one key is constant
-    if (a.sub == 1) {
+    if (a.k_cuts == 1) {
         store_rows<BF, DP>(const_cast<char*>(row_base(a.dk, d, d.k0 + key, kvh)), dk, p.dim, fk, any_k);
         store_rows<BF, DP>(const_cast<char*>(row_base(a.dv, d, d.k0 + key, kvh)), dv, p.dim, back, any);
         return;
     }
     const int64_t rows = p.packed ? p.k_rows : p.k_rows * p.n_docs;
-    const int64_t at = (head0 * rows + (p.packed ? d.k0 : d.batch * p.k_rows) + key) * p.dim;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int e = 32 * i + 2 * r;
-            if (e >= p.dim) continue;
-            *reinterpret_cast<float4*>(a.part_k + at + e + 4 * half) = any_k ? make_float4(dk[i][r] * fk, dk[i][r + 1] * fk, dk[i][r + 2] * fk, dk[i][r + 3] * fk) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(a.part_v + at + e + 4 * half) = any ? make_float4(dv[i][r] * back, dv[i][r + 1] * back, dv[i][r + 2] * back, dv[i][r + 3] * back) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+    const int64_t at = (((int64_t)kvh * a.k_cuts + cut) * rows + (p.packed ? d.k0 : d.batch * p.k_rows) + key) * p.dim;
+    store_part<DP>(a.part + at, dk, p.dim, fk, any_k);
+    store_part<DP>(a.part_v + at, dv, p.dim, back, any);
 }
 
-// Sums of the query heads' parts, 4 elements a thread.
+// Sums of the parts of one or two gradients, 4 elements a thread.
+struct Sum {
+    const float* part[2];
+    Rows to[2];
+    int64_t rows, batch_rows;         // of a head, and of a batch entry (all of them where documents are packed)
+    int64_t head_step, part_step;     // from one head's first part, and one part, to the next
+    int heads, parts, pieces, tensors;
+};
 template <bool BF>
-__global__ void __launch_bounds__(kThreads) sum_kernel(const BackwardArgs a, int64_t n) {
-    const Problem& p = a.p;
-    const int64_t rows = p.packed ? p.k_rows : p.k_rows * p.n_docs;
-    const int pieces = p.dim / 4;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t which = i >= n / 2, j = i - which * (n / 2);
-        const int64_t hr = j / pieces;
-        const int e = 4 * (int)(j - hr * pieces), kvh = (int)(hr / rows);
-        const int64_t row = hr - kvh * rows;
-        const float* part = (which ? a.part_v : a.part_k) + ((int64_t)kvh * p.group * rows + row) * p.dim + e;
+__global__ void __launch_bounds__(kThreads) sum_kernel(const Sum a) {
+    const int64_t n = a.rows * a.heads * a.pieces;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n * a.tensors; i += (int64_t)gridDim.x * kThreads) {
+        const int which = i >= n;
+        const int64_t j = i - which * n, hr = j / a.pieces;
+        const int e = 4 * (int)(j - hr * a.pieces), head = (int)(hr / a.rows);
+        const int64_t row = hr - head * a.rows;
+        const float* part = a.part[which] + head * a.head_step + row * (4 * a.pieces) + e;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int h = 0; h < p.group; ++h) {
-            const float4 v = *reinterpret_cast<const float4*>(part + h * rows * p.dim);
+        for (int c = 0; c < a.parts; ++c) {
+            const float4 v = *reinterpret_cast<const float4*>(part + c * a.part_step);
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
-        const Rows& to = which ? a.dv : a.dk;
-        const int64_t b = p.packed ? 0 : row / p.k_rows;
-        store4<BF>(static_cast<char*>(const_cast<void*>(to.p)) + 2 * (b * to.b + (row - b * p.k_rows) * to.n + kvh * to.h + e), nullptr, s.x, s.y, s.z, s.w);
+        const Rows& to = a.to[which];
+        const int64_t b = row / a.batch_rows;
+        store4<BF>(static_cast<char*>(const_cast<void*>(to.p)) + 2 * (b * to.b + (row - b * a.batch_rows) * to.n + head * to.h + e), nullptr, s.x, s.y, s.z, s.w);
     }
 }
 
@@ -443,8 +459,9 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     constexpr int kTileBytes = kKeys * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     Doc d;
-    if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
-    const int head = head_of(p, blockIdx.x % p.heads), kvh = head / p.group;
+    const int lot = blockIdx.x % (p.heads * a.q_cuts), cut = lot / p.heads;
+    if (!find_doc<true>(p, blockIdx.x / (p.heads * a.q_cuts), kRows, d)) return;
+    const int head = head_of(p, lot % p.heads), kvh = head / p.group;
     const int row0 = d.tile * kRows, w0 = row0 + 32 * wave, row = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
     auto limit = [&](int r) {
@@ -455,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     const int wave_lim = w0 < nq ? limit(w0 + 31) : 0;
     const int full_lim = w0 < nq ? limit(w0) : 0;
     const int lim = row < nq ? limit(row) : 0;
-    const int n = block_lim > 0 ? (block_lim + kKeys - 1) / kKeys : 0;
+    const int all = block_lim > 0 ? (block_lim + kKeys - 1) / kKeys : 0, part = (all + a.q_cuts - 1) / a.q_cuts;
+    const int t0 = min(cut * part, all), n = min(t0 + part, all);     // this block's tiles
 
     typedef Loader<DP, kKeys, kWaves> Load;
     Load lk, lv;
@@ -477,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     float delta = nq > 0 ? -a.delta[at] * phi : 0.f;
     Shape<CAP> sh;
     sh.set(p, head);
-    for (int i = 0; i < kRing - 1 && i < n; ++i) stage(i);
+    for (int i = t0; i < t0 + kRing - 1 && i < n; ++i) stage(i);
     f32x16 dq[DP / 32], x{}, dp{};
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) dq[i] = f32x16{};
@@ -494,8 +512,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     arrived(qf);
     arrived(gf);
     asm volatile("" : "+v"(add), "+v"(delta));
-    if (wave_lim > 0) products(smem, x, dp);
-    for (int t = 0; t < n; ++t) {
+    if (t0 < n && t0 * kKeys < wave_lim) products(smem + (t0 % kRing) * 2 * kTileBytes, x, dp);
+    for (int t = t0; t < n; ++t) {
         if (t + kRing - 2 < n) wait_but<2 * Load::kCount>();
         else wait_all();
         block_sync();
@@ -523,7 +541,14 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     }
     wait_all();
     if (row >= d.rows) return;
-    store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi * sh.factor(), lim > 1);       // a softmax over one key is constant
+    const float by = p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi * sh.factor();
+    const bool some = lim > 1;                                        // a softmax over one key is constant
+    if (a.q_cuts == 1) {
+        store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, by, some);
+        return;
+    }
+    const int64_t rows = p.packed ? p.q_rows : p.q_rows * p.n_docs;
+    store_part<DP>(a.part + (((int64_t)cut * p.heads + head) * rows + (p.packed ? d.q0 : d.batch * p.q_rows) + row) * p.dim, dq, p.dim, by, some);
 }
 
 // ---- short documents ----
@@ -719,6 +744,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) whole_kernel(const BackwardArgs
     }
 }
 
+template <bool BF>
+void launch_sum(const Sum& s, hipStream_t stream) {
+    const int64_t need = (s.rows * s.heads * s.pieces * s.tensors + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL(sum_kernel<BF>, dim3((uint32_t)(need < 8192 ? need : 8192)), dim3(kThreads), 0, stream, s);
+}
+
 template <bool BF, int DP, bool CAP, int WAVES>
 int launch_whole(BackwardArgs& b, hipStream_t stream) {
     Problem& p = b.p;
@@ -751,10 +782,10 @@ int launch(BackwardArgs& b, hipStream_t stream) {
         const auto fn = &keys_kernel<BF, DP, CAP>;
         const size_t lds = kRing * (2 * (size_t)kTile * DP * 2 + kTile * 16);
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
-        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.sub)), dim3(kThreads), lds, stream, b);
-        if (b.sub > 1) {
-            const int64_t n = 2 * (p.packed ? p.k_rows : p.k_rows * p.n_docs) * p.kv_heads * (p.dim / 4), need = (n + kThreads - 1) / kThreads;
-            hipLaunchKernelGGL(sum_kernel<BF>, dim3((uint32_t)(need < 8192 ? need : 8192)), dim3(kThreads), 0, stream, b, n);
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.k_cuts)), dim3(kThreads), lds, stream, b);
+        if (b.k_cuts > 1) {
+            const int64_t rows = p.packed ? p.k_rows : p.k_rows * p.n_docs;
+            launch_sum<BF>(Sum{{b.part, b.part_v}, {b.dk, b.dv}, rows, p.k_rows, b.k_cuts * rows * p.dim, rows * p.dim, p.kv_heads, b.k_cuts, p.dim / 4, 2}, stream);
         }
     }
     if (tq > 0) {
@@ -762,7 +793,11 @@ int launch(BackwardArgs& b, hipStream_t stream) {
         const auto fn = &rows_kernel<BF, DP, CAP>;
         const size_t lds = kRing * 2 * (size_t)32 * DP * 2;
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
-        hipLaunchKernelGGL(fn, dim3((uint32_t)(tq * p.heads)), dim3(kThreads), lds, stream, b);
+        hipLaunchKernelGGL(fn, dim3((uint32_t)(tq * p.heads * b.q_cuts)), dim3(kThreads), lds, stream, b);
+        if (b.q_cuts > 1) {
+            const int64_t rows = p.packed ? p.q_rows : p.q_rows * p.n_docs;
+            launch_sum<BF>(Sum{{b.part, nullptr}, {b.dq, Rows{}}, rows, p.q_rows, rows * p.dim, rows * p.heads * p.dim, p.heads, b.q_cuts, p.dim / 4, 1}, stream);
+        }
     }
     return launched("attention backward");
 }
@@ -782,14 +817,34 @@ bool is_whole(const mmfe_attention_args* a) {
     return !a->packed && a->n_docs > 0 && a->heads == a->kv_heads && a->dim <= 64 && a->q_rows <= kWholeRows && a->k_rows <= kWholeRows && a->q_rows + a->k_rows > 0;
 }
 
-// Blocks that a key head's query heads are spread over: one, or one per query head (whose parts a second launch sums in float32)
-// where one would leave fewer than 1024 blocks, 4 a CU, and walk over 2048 rows at least.  4096 rows, 16 heads on 4 of 128: 766 us in 128
-// blocks, 405 in 512 and the sums; at 1024 blocks and more both take the same and the parts' traffic is saved.
-int spread(const mmfe_attention_args* a) {
-    const int64_t rows = a->packed ? a->k_rows : a->k_rows * a->n_docs;
-    return a->heads > a->kv_heads && (rows + kRows - 1) / kRows * a->kv_heads < 1024 && a->q_rows * (a->heads / a->kv_heads) >= 2048 ? a->heads / a->kv_heads : 1;
+// Parts that the walks of `rows` (the keys, or the rows) over `partners` are cut into, whose float32 sums another launch adds: as many as fill
+// the machine, about 768 blocks in all (512 in keys_kernel at head size 128, where a CU holds one), each of 256 partners or more.  Walks of
+// less than 1000 are not worth that launch, nor of 2000 where half of the blocks are there.  Of packed documents only the mean is known here; the
+// long ones are taken to have three times as many partners.  A causal mask leaves a key min(rows, keys) of them.  Forward and backward, causal,
+// head size 64: 4000 rows, 4 query heads on one key head: 548 us uncut, 275 with a block per query head, 158 so; 64 rows over 8000 keys, 6 heads: 234 and
+// 62; 32 documents of 400, 12 heads on 4, which 512 blocks serve: 132, and 151 if cut.  Over 90 shapes of 1 to 32 documents of 64 to 8000 rows
+// a call takes 3 % longer on average than with the best choice for it, uncut 82 %; the worst is 8 packed recordings of 1000 rows, 6 heads, taken for
+// longer ones: 122 us, uncut 107.
+int64_t in_all(const mmfe_attention_args* a, int64_t rows) { return a->packed ? rows : rows * a->n_docs; }
+int cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t partners, int64_t want) {
+    if (a->n_docs < 1 || rows < 1) return 1;
+    const int64_t tiles = (rows + kRows - 1) / kRows, blocks = (a->packed ? tiles : tiles * a->n_docs) * heads;
+    if (a->packed && a->n_docs > 3) partners = partners * 3 / a->n_docs;
+    if (partners < (2 * blocks < want ? 1000 : 2000)) return 1;
+    int64_t n = (want + blocks / 2) / blocks;
+    if (n > partners / 256) n = partners / 256;
+    return n < 1 ? 1 : (int)n;
 }
-int64_t part_size(const mmfe_attention_args* a) { return spread(a) > 1 ? (a->packed ? a->k_rows : a->k_rows * a->n_docs) * a->heads * a->dim : 0; }
+int key_cuts(const mmfe_attention_args* a) {
+    const int64_t seen = a->causal && a->prefix == nullptr && a->k_rows < a->q_rows ? a->k_rows : a->q_rows;
+    return cuts(a, a->k_rows, a->kv_heads, seen * (a->heads / a->kv_heads), a->dim > 64 ? 512 : 768);
+}
+int row_cuts(const mmfe_attention_args* a) { return cuts(a, a->q_rows, a->heads, a->k_rows, 768); }
+int64_t key_parts(const mmfe_attention_args* a) { return key_cuts(a) > 1 ? key_cuts(a) * in_all(a, a->k_rows) * a->kv_heads * a->dim : 0; }
+int64_t parts(const mmfe_attention_args* a) {          // the two passes use them one after the other
+    const int64_t q = row_cuts(a) > 1 ? row_cuts(a) * in_all(a, a->q_rows) * a->heads * a->dim : 0;
+    return 2 * key_parts(a) > q ? 2 * key_parts(a) : q;
+}
 int64_t lse_size(const mmfe_attention_args* a) { return (a->packed ? 1 : (int64_t)a->n_docs) * a->heads * a->q_rows; }
 
 }  // namespace
@@ -804,7 +859,7 @@ int64_t mmfe_attention_backward_workspace(const mmfe_attention_args* a) {
     if (make_problem(a, p)) return -1;
     if (is_whole(a)) return 0;
     const int64_t norms = a->dtype == MMFE_OUT_F16 ? a->heads * slots(a, a->q_rows) + a->kv_heads * slots(a, a->k_rows) : 0;
-    return (6 * lse_size(a) + 2 * part_size(a) + norms + 4) * (int64_t)sizeof(float);
+    return (6 * lse_size(a) + parts(a) + norms + 4) * (int64_t)sizeof(float);
 }
 
 int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_grads* g, void* workspace, int device, void* hip_stream) {
@@ -828,10 +883,10 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     b.dq = rows(g->grad_q, g->grad_q_stride); b.dk = rows(g->grad_k, g->grad_k_stride); b.dv = rows(g->grad_v, g->grad_v_stride);
     b.lse = a->lse; b.lse_b = a->lse_stride[0]; b.lse_h = a->lse_stride[1];
     b.whole = whole;
-    b.sub = spread(a);
+    b.k_cuts = key_cuts(a); b.q_cuts = row_cuts(a);
     b.aux = static_cast<u32x4*>(workspace);
-    b.part_k = reinterpret_cast<float*>(b.aux + lse_size(a)); b.part_v = b.part_k + part_size(a);
-    b.lse2 = b.part_v + part_size(a); b.delta = b.lse2 + lse_size(a);
+    b.part = reinterpret_cast<float*>(b.aux + lse_size(a)); b.part_v = b.part + key_parts(a);
+    b.lse2 = b.part + parts(a); b.delta = b.lse2 + lse_size(a);
     b.q_slots = (int)slots(a, a->q_rows); b.k_slots = (int)slots(a, a->k_rows);
     b.norm_g = b.delta + lse_size(a); b.norm_v = b.norm_g + (int64_t)a->heads * b.q_slots;
     OnDevice on(device);

@@ -528,3 +528,18 @@ MANY = [
 @pytest.mark.parametrize("case", MANY, ids=lambda c: f"{c[0]}x{c[2]}x{c[3]}x{c[5]}")
 def test_rows_over_kept_keys(mm, O, case):
     test_few_rows_over_many_keys(mm, O, case)
+
+
+LONG = [
+    # few blocks and long walks: both passes of the gradients in parts
+    ("padded", ([1500, 3], 1500, None, 1500, 2, 1, 128, HF, True, False, False, 0.0)),
+    ("padded", ([1100], 1100, None, 1100, 1, 1, 40, BF, False, False, True, 7.0)),
+    ("padded", ([90, 2000], 2000, [2100, 0], 2100, 4, 2, 64, HF, True, True, False, 0.0)),
+    ("packed", ([1300, 20, 0], 5, 140, 3, 1, 64, BF, True, True, False, 0.0)),
+    ("packed", ([2050], 0, 0, 2, 2, 72, HF, False, False, False, 12.0)),
+]
+
+
+@pytest.mark.parametrize("form, case", LONG, ids=lambda c: c if isinstance(c, str) else f"{c[0]}x{c[-8]}x{c[-6]}")
+def test_gradients_in_parts(mm, O, form, case):
+    (test_padded if form == "padded" else test_packed)(mm, O, case)
