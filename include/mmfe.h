@@ -332,7 +332,7 @@ typedef struct mmfe_attention_args {
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   /* batch, row, head */
     int64_t lse_stride[2];    /* batch, head; rows are contiguous */
 } mmfe_attention_args;
-/* Bytes of device memory mmfe_attention_forward needs for these arguments (few rows over many keys are cut into chunks of keys
+/* Bytes of device memory mmfe_attention_forward needs for these arguments (the keys are cut where there are few blocks of rows, into parts
  * whose results are joined): 16-byte aligned, the call's own until it has run.  0: none.  -1: the arguments are refused. */
 int64_t mmfe_attention_workspace(const mmfe_attention_args* args);
 int mmfe_attention_forward(const mmfe_attention_args* args, void* workspace, int device, void* hip_stream);

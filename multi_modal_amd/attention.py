@@ -97,7 +97,7 @@ class _Call:
             if self.backward_bytes:            # 0: the backward pass reads neither out nor its rest
                 rest = torch.empty(q.shape, dtype=q.dtype, device=device)
                 args = self.args(q, k, v, out, rest, lse)
-        need = N.attention_workspace(args) if k.shape[-3] > 512 and not self.packed else 0
+        need = N.attention_workspace(args) if k.shape[-3] > 512 else 0
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         N.attention_forward(args, _ptr(work), self.device, raw_stream(self.device))
         return out, rest, lse

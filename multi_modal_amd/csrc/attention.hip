@@ -23,10 +23,17 @@
 // types hold, and most tiles skip the rescaling of o.
 #include "attention_tiles.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace mmfe {
 using namespace attn;
+
+namespace attn {
+int64_t in_all(const mmfe_attention_args* a, int64_t rows);
+int walk_cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t partners, int64_t want);
+}  // namespace attn
+
 namespace {
 
 constexpr int kSplitTile = 32;         // keys of a wave's tile in split_kernel
@@ -38,6 +45,9 @@ struct ForwardArgs {
     char* rest;                       // like out: what its rounding lost; NULL: not wanted
     float* lse;                       // (batch, heads, rows) or (heads, rows); NULL: not wanted
     int64_t lse_b, lse_h;
+    int cuts;                         // parts of forward_kernel's walk over the keys; more than one: (cuts, heads, rows) results over their own
+    float* part;                      // maximum, in float32, and that maximum and sum
+    float2* part_ml;
 };
 
 // How scores leave the linear form (bits); anything but kPlain takes them to log2 units before the maximum.
@@ -127,6 +137,7 @@ __device__ __forceinline__ void hide(f32x16& x, int left) {
 // Keys of a step, and tiles of keys (and of values) in LDS.
 constexpr int kStepKeys = 32;
 constexpr int kRing = 4;
+constexpr float kLowest = -3e38f;      // maximum of keys that are seen and have scores of -infinity, which no keys at all have
 static_assert(kStepKeys * kRing >= kShortKeys, "a short document's keys are in LDS at once");
 
 template <bool BF, int DP, int SHAPE>
@@ -135,10 +146,10 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     const Problem& p = a.p;
     constexpr int kTileBytes = kStepKeys * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int j = blockIdx.x % p.heads;
+    const int lot = blockIdx.x % (p.heads * a.cuts), cut = lot / p.heads;
     Doc d;
-    if (!find_doc<true>(p, blockIdx.x / p.heads, kRows, d)) return;
-    const int head = head_of(p, j), kvh = head / p.group;
+    if (!find_doc<true>(p, blockIdx.x / (p.heads * a.cuts), kRows, d)) return;
+    const int head = head_of(p, lot % p.heads), kvh = head / p.group;
     const int row0 = d.tile * kRows, w0 = row0 + 32 * wave, row = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
     // keys [0, limit of the block / the wave / the row) are visible
@@ -150,7 +161,9 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     const int wave_lim = w0 < nq ? limit(w0 + 31) : 0;
     const int full_lim = w0 < nq ? limit(w0) : 0;                             // keys that all rows of the wave see
     const int lim = row < nq ? limit(row) : 0;
-    const int n = block_lim > 0 ? (block_lim + kStepKeys - 1) / kStepKeys : 0;            // steps
+    const bool at_once = nk <= kShortKeys;                                    // at most kRing tiles: all of them are asked for at the start
+    const int all = block_lim > 0 ? (block_lim + kStepKeys - 1) / kStepKeys : 0, share = at_once ? all : (all + a.cuts - 1) / a.cuts;
+    const int t0 = min(cut * share, all), n = min(t0 + share, all);           // this block's steps
 
     typedef Loader<DP, kStepKeys, kWaves> Load;
     Load lk, lv;
@@ -164,12 +177,12 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
         lv.load(row_base(p.v, d, d.k0 + (int64_t)t * kStepKeys, kvh), nk - t * kStepKeys, p.dim, p.v.n, uniform(lds0 + (kRing + t % kRing) * kTileBytes), wave);
     };
     // in the order in which the steps need them
-    if (n > 0) load_k(0);
-    if (n > 1) load_k(1);
+    if (t0 < n) load_k(t0);
+    if (t0 + 1 < n) load_k(t0 + 1);
 #pragma unroll
-    for (int t = 0; t < kRing - 2; ++t) {
-        if (t < n) load_v(t);
-        if (t + 2 < n) load_k(t + 2);
+    for (int i = 0; i < kRing - 2; ++i) {
+        if (t0 + i < n) load_v(t0 + i);
+        if (t0 + i + 2 < n) load_k(t0 + i + 2);
     }
 
     u32x4 qf[DP / 16];
@@ -216,16 +229,15 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
         }
     };
 
-    const bool at_once = nk <= kShortKeys;                                    // at most kRing tiles: all of them are asked for here
     if (at_once)
 #pragma unroll
         for (int t = kRing - 2; t < kRing; ++t)
-            if (t < n) load_v(t);
+            if (t0 == 0 && t < n) load_v(t);
     wait_all();
     block_sync();
     arrived(qf);
     if (at_once) {
-        for (int t = 0; t < n && t * kStepKeys < wave_lim; ++t) {
+        for (int t = t0; t < n && t * kStepKeys < wave_lim; ++t) {
             x = scores(t);
             const float lack = shape_and_hide(t);
             rescale(State::largest(x, lack));
@@ -237,14 +249,14 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
                 values(t, s, operand_rest<BF>(x, s, pf));
             }
         }
-    } else if (n > 0) {
+    } else if (t0 < n) {
         // Products of one step run beside the softmax of another: step t turns the scores of its 32 keys, computed a step earlier, into p,
         // while the matrix pipe adds step t - 1 to o (beside the maximum) and forms the scores of step t + 1 (beside the exponentials).
         // So step t needs k of t + 1 and v of t - 1; their buffers' former tiles were used up in step t - 1 at the latest, and it asks for
         // k of t + kRing and v of t + kRing - 2: kRing - 1 steps ahead of their use.
         constexpr int kAhead = (kRing - 2) * 2 * Load::kCount;
         u32x4 pf[2];
-        if (wave_lim > 0) x = scores(0);
+        if (t0 * kStepKeys < wave_lim) x = scores(t0);
         auto step = [&](int t) {           // every wave's parts have arrived, and its reads of the buffers that are asked for now are done
             if (t - 1 + kRing < n) wait_but<kAhead>();     // the last kRing - 2 steps asked for a whole tile of each
             else wait_all();
@@ -252,12 +264,13 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
             if (t + kRing < n) load_k(t + kRing);
             if (t + kRing - 2 < n) load_v(t + kRing - 2);
         };
-        const int mine = (wave_lim + kStepKeys - 1) / kStepKeys;       // steps of this wave; it only keeps step with the others behind them
-        for (int t = 0; t < mine; ++t) {
+        // this wave's steps end before `mine`; it only keeps step with the others behind them
+        const int mine = max(t0, min(n, (wave_lim + kStepKeys - 1) / kStepKeys));
+        for (int t = t0; t < mine; ++t) {
             step(t);
             const float lack = shape_and_hide(t);
             const float mx = State::largest(x, lack);
-            if (t > 0) {
+            if (t > t0) {
                 values(t - 1, 0, pf[0]);
                 values(t - 1, 1, pf[1]);
             }
@@ -273,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
             wait_all();
             block_sync();
         }
-        if (mine > 0) {
+        if (mine > t0) {
             values(mine - 1, 0, pf[0]);
             values(mine - 1, 1, pf[1]);
         }
@@ -285,6 +298,19 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     }
     const float l = both_sum(st.l);
     if (row >= d.rows) return;
+    if (a.cuts > 1) {
+        const int64_t place = ((int64_t)cut * p.heads + head) * (p.packed ? p.q_rows : p.q_rows * p.n_docs) + (p.packed ? d.q0 : d.batch * p.q_rows) + row;
+        const bool sees = lim > t0 * kStepKeys && t0 < n;
+        if (half == 0) a.part_ml[place] = sees ? make_float2(st.m == -INFINITY ? kLowest : st.m * unit, l) : make_float2(-INFINITY, 0.f);
+        if (!sees) return;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (32 * i + 8 * g < p.dim)
+                    *reinterpret_cast<float4*>(a.part + place * p.dim + 32 * i + 8 * g + 4 * half) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+        return;
+    }
     const bool some = lim > 0;
     const float inv = some ? 1.f / l : 0.f;
     const int64_t at = 2 * (d.batch * a.out.b + (d.q0 + row) * a.out.n + head * a.out.h);
@@ -302,6 +328,39 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
         }
     if (a.lse != nullptr && half == 0)
         a.lse[d.batch * a.lse_b + head * a.lse_h + d.q0 + row] = some ? (st.m * unit + __builtin_amdgcn_logf(l)) * (1.f / kLog2e) : -INFINITY;
+}
+
+// The parts of cut walks, 4 elements of a row a thread.
+template <bool BF>
+__global__ void __launch_bounds__(kThreads) gather_kernel(const ForwardArgs a) {
+    const Problem& p = a.p;
+    const int pieces = p.dim / 4;
+    const int64_t rows = p.packed ? p.q_rows : p.q_rows * p.n_docs, step = rows * p.heads, n = step * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t hr = i / pieces;
+        const int e = 4 * (int)(i - hr * pieces), head = (int)(hr / rows);
+        const int64_t row = hr - head * rows;
+        float top = -INFINITY;
+        for (int c = 0; c < a.cuts; ++c) top = max2(top, a.part_ml[c * step + hr].x);
+        const bool some = top != -INFINITY;
+        float total = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < a.cuts; ++c) {
+            const float2 ml = a.part_ml[c * step + hr];
+            if (ml.x == -INFINITY) continue;                          // sees none of these keys
+            const float k = exp2_fast(ml.x - top);
+            const float4 u = *reinterpret_cast<const float4*>(a.part + (c * step + hr) * p.dim + e);
+            total += k * ml.y;
+            v.x += k * u.x; v.y += k * u.y; v.z += k * u.z; v.w += k * u.w;
+        }
+        const int64_t b = p.packed ? 0 : row / p.q_rows, r = row - b * p.q_rows;
+        const int64_t at = 2 * (b * a.out.b + r * a.out.n + head * a.out.h + e);
+        const float inv = some ? 1.f / total : 0.f;
+        char* out = static_cast<char*>(const_cast<void*>(a.out.p)) + at;
+        if (some) store4<BF>(out, a.rest ? a.rest + at : nullptr, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        else store4<BF>(out, a.rest ? a.rest + at : nullptr, 0.f, 0.f, 0.f, 0.f);
+        if (e == 0 && a.lse != nullptr) a.lse[b * a.lse_b + head * a.lse_h + r] = some ? (top + __builtin_amdgcn_logf(total)) * (1.f / kLog2e) : -INFINITY;
+    }
 }
 
 // ---- few rows over many keys ----
@@ -568,38 +627,40 @@ split_fn pick_split(int dim) {
     return dim <= 32 ? &split_kernel<BF, 32> : dim <= 64 ? &split_kernel<BF, 64> : &split_kernel<BF, 128>;
 }
 
-// Keys of a chunk and chunks of a unit, or no chunks: the row kernel serves the call.
+// How a call's keys are cut: chunks of split_kernel (n_splits > 0), or parts of forward_kernel's walks.
 //
-// A unit's block takes about 8 us to start and end and 16 (head size 64: 15) per 1000 keys, a block of the row kernel the same for the 4 rows' tiles it
-// shares its keys among, so that cutting pays where blocks are few or, with key heads shared by query heads, few rows would read their keys once
-// per query head.  Measured over 1 to 64 rows, 1 to 128 documents of 200 to 32000 keys, 12 heads and 16 on 4, of 64 and 128, all documents as long as
-// their room and of lengths from 1 to 30 in 32:
-//   - up to 512 keys, and up to 2048 where 256 units fill the CUs: no cut; the row kernel, unless units share keys and its blocks do not all run at
-//     once (128 streams of 500 keys, one row, 16 heads on 4: 26.6 us, row kernel 61.4; 32 of them 17.3 and 18.3; 64 rows of 32 documents
-//     of 1000 keys, 12 heads of 64: 27, cut in 512 keys 75)
-//   - more rows than a unit takes, in 192 blocks of the row kernel or more: the row kernel (64 rows, 32 documents of 8000 keys, 12 heads of 128:
-//     317 us, cut 481; 8 documents, 96 blocks: 166 and 139; 512 rows over 32000 keys, 12 heads of 64: 574 and 159)
+// A unit's block takes about 8 us to start and end and 16 (head size 64: 15) per 1000 keys, a block of the row kernel 19 for the four times as many
+// rows it shares its keys among.  So split_kernel pays for units of few rows, above all where query heads share their keys, which the row
+// kernel reads once per query head.  Measured over 1 to 8000 rows, 1 to 128 documents of 200 to 32000 keys, 12 heads, 16 on 4 and smaller sets, of 64 and 128,
+// documents as long as their room and of lengths from 1 to 30 in 32:
+//   - up to 512 keys, and up to 2048 where 256 units fill the CUs: no chunks; the row kernel, unless units share keys and its blocks do not all run
+//     at once (128 streams of 500 keys, one row, 16 heads on 4: 26.6 us, row kernel 61.4; 32 of them 17.3 and 18.3; 64 rows of 32 documents
+//     of 1000 keys, 12 heads of 64: 27, in chunks of 512 keys 75)
+//   - more rows than a unit takes, in more than 64 units: the row kernel, its walks cut (8000 keys, 16 heads on 4 of 128, 512 rows: 61 us, uncut 172, in
+//     chunks 120; 128 rows, 64 units: 39 in chunks, 173 uncut; 4 documents of 128 rows, 2000 keys, 12 heads on 4 of 64, 192 units: 24 cut, 33 in chunks)
 //   - else chunks that make 512 blocks, two on each CU, of 256 keys at least, and of 1024 at most (documents shorter than their room leave chunks
 //     empty) unless that makes more than 2048: 16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 109 / 93 / 100 / 113 us with 512 /
 //     1024 / 2048 / 4096 keys; 32 streams of 2000 keys, one row, 4 key heads of 128: 39 / 34 / 33 with 256 / 512 / 1024.
-// Over all of it a call takes 3 % longer on average than with the best of these choices for it (with even lengths 2.5, uneven 4).
+// Over all of it a call takes 3 % longer on average than with the best of these choices for it.
 struct Cut {
-    int row_tiles = 0, chunk = 0, n_splits = 0;
+    int row_tiles = 0, chunk = 0, n_splits = 0, cuts = 1;
     int64_t units = 0;
 };
 Cut cut_keys(const mmfe_attention_args* a) {
     Cut c;
+    c.cuts = std::min(12, walk_cuts(a, a->q_rows, a->heads, a->k_rows, a->dim > 64 ? 512 : 768));
     if (a->packed || a->q_rows < 1 || a->n_docs < 1) return c;
     const int64_t keys = a->k_rows, row_tiles = (a->q_rows * (a->heads / a->kv_heads) + 31) / 32, units = a->n_docs * row_tiles * a->kv_heads;
     const int64_t blocks = a->n_docs * ((a->q_rows + kRows - 1) / kRows) * a->heads;       // of the row kernel
     if (keys <= kShortKeys) return c;
     const bool whole = keys <= 512 || (keys <= 2048 && units >= 256);
-    if (whole ? units >= blocks || blocks <= 512 : units > blocks && blocks >= 192) return c;
+    if (whole ? units >= blocks || blocks <= 512 : units > blocks && units > 64) return c;
     const int64_t all = keys * units;
     int64_t chunk = (all + 511) / 512, most = (all + 2047) / 2048;
     if (most < 1024) most = 1024;
     chunk = chunk < 256 ? 256 : chunk > most ? most : chunk;
     chunk = whole ? keys : (chunk + 127) / 128 * 128;
+    c.cuts = 1;
     c.row_tiles = (int)row_tiles;
     c.units = units;
     c.chunk = (int)chunk;
@@ -610,6 +671,25 @@ Cut cut_keys(const mmfe_attention_args* a) {
 }  // namespace
 
 namespace attn {
+
+int64_t in_all(const mmfe_attention_args* a, int64_t rows) { return a->packed ? rows : rows * a->n_docs; }
+// Parts that the walks of `rows` (the rows, or for the gradients of k and v the keys) over `partners` are cut into, whose float32 sums another
+// launch adds: as many as fill the machine, about `want` blocks in all (768; 512 where a CU holds fewer, at head size 128), each of 256 partners or
+// more.  Walks of less than 1000 are not worth that launch, nor of 2000 where half of the blocks are there.  Of packed documents only the mean
+// is known here; the long ones are taken to have three times as many partners.  Forward and backward, causal, head size 64: 4000 rows, 4 query
+// heads on one key head: 548 us uncut, 126 so; 64 rows over 8000 keys, 6 heads: 234 and 62; 32 documents of 400, 12 heads on 4, which 512 blocks
+// serve: 132, and 151 if cut.  Forward alone: 4000 rows, 2 key heads of 128 and 4 query heads: 104 and 46; one recording of 4000 among 12 of 50, 6 heads: 86
+// and 40.  Over 200 shapes of 1 to 32 documents of 64 to 8000 rows each pass takes 1 to 4 % longer on average than with the best choice
+// for it; the worst is 8 packed recordings of 1000 rows, 6 heads, taken for longer ones: forward and backward 125 us, uncut 107.
+int walk_cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t partners, int64_t want) {
+    if (a->n_docs < 1 || rows < 1) return 1;
+    const int64_t tiles = (rows + kRows - 1) / kRows, blocks = (a->packed ? tiles : tiles * a->n_docs) * heads;
+    if (a->packed && a->n_docs > 3) partners = partners * 3 / a->n_docs;
+    if (partners < (2 * blocks < want ? 1000 : 2000)) return 1;
+    int64_t n = (want + blocks / 2) / blocks;
+    if (n > partners / 256) n = partners / 256;
+    return n < 1 ? 1 : (int)n;
+}
 
 int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
@@ -674,7 +754,8 @@ int64_t mmfe_attention_workspace(const mmfe_attention_args* a) {
     Problem p{};
     if (make_problem(a, p)) return -1;
     const Cut c = cut_keys(a);
-    return c.n_splits > 1 ? c.units * c.n_splits * 32 * (a->dim + 2) * (int64_t)sizeof(float) : 0;
+    const int64_t rows = c.n_splits > 1 ? c.units * c.n_splits * 32 : c.cuts > 1 ? c.cuts * a->heads * in_all(a, a->q_rows) : 0;
+    return rows * (a->dim + 2) * (int64_t)sizeof(float);
 }
 
 int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int device, void* hip_stream) {
@@ -691,7 +772,7 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     f.lse = a->lse; f.lse_b = a->lse_stride[0]; f.lse_h = a->lse_stride[1];
     const Cut c = cut_keys(a);
-    if (c.n_splits > 1 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
+    if ((c.n_splits > 1 || c.cuts > 1) && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
     if (c.units * c.n_splits > 0x7fffffffll || c.units > 0x3ffffff) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
     OnDevice on(device);
     if (on.rc) return on.rc;
@@ -720,7 +801,15 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
     int blocks = 1, cus = 256;
     rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);
     if (rc) return rc;
-    hipLaunchKernelGGL(fn, dim3((uint32_t)(tiles * a->heads)), dim3(kThreads), lds, reinterpret_cast<hipStream_t>(hip_stream), f);
+    f.cuts = c.cuts;
+    const int64_t rows = a->heads * in_all(a, a->q_rows);
+    f.part = static_cast<float*>(workspace);
+    f.part_ml = c.cuts > 1 ? reinterpret_cast<float2*>(f.part + c.cuts * rows * a->dim) : nullptr;
+    hipLaunchKernelGGL(fn, dim3((uint32_t)(tiles * a->heads * c.cuts)), dim3(kThreads), lds, reinterpret_cast<hipStream_t>(hip_stream), f);
+    if (c.cuts > 1) {
+        const int64_t need = (rows * (a->dim / 4) + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(bf ? &gather_kernel<true> : &gather_kernel<false>, dim3((uint32_t)(need < 8192 ? need : 8192)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(hip_stream), f);
+    }
     return launched("attention");
 }
 

@@ -28,6 +28,8 @@ bool bad_rows(const char* name, const void* ptr, const int64_t* s);
 int make_problem(const mmfe_attention_args* a, Problem& p);
 int64_t count_tiles(Problem& p, int64_t rows, int tile_rows);
 int launched(const char* what);
+int64_t in_all(const mmfe_attention_args* a, int64_t rows);
+int walk_cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t partners, int64_t want);
 }  // namespace attn
 
 namespace {
@@ -817,29 +819,12 @@ bool is_whole(const mmfe_attention_args* a) {
     return !a->packed && a->n_docs > 0 && a->heads == a->kv_heads && a->dim <= 64 && a->q_rows <= kWholeRows && a->k_rows <= kWholeRows && a->q_rows + a->k_rows > 0;
 }
 
-// Parts that the walks of `rows` (the keys, or the rows) over `partners` are cut into, whose float32 sums another launch adds: as many as fill
-// the machine, about 768 blocks in all (512 in keys_kernel at head size 128, where a CU holds one), each of 256 partners or more.  Walks of
-// less than 1000 are not worth that launch, nor of 2000 where half of the blocks are there.  Of packed documents only the mean is known here; the
-// long ones are taken to have three times as many partners.  A causal mask leaves a key min(rows, keys) of them.  Forward and backward, causal,
-// head size 64: 4000 rows, 4 query heads on one key head: 548 us uncut, 275 with a block per query head, 158 so; 64 rows over 8000 keys, 6 heads: 234 and
-// 62; 32 documents of 400, 12 heads on 4, which 512 blocks serve: 132, and 151 if cut.  Over 90 shapes of 1 to 32 documents of 64 to 8000 rows
-// a call takes 3 % longer on average than with the best choice for it, uncut 82 %; the worst is 8 packed recordings of 1000 rows, 6 heads, taken for
-// longer ones: 122 us, uncut 107.
-int64_t in_all(const mmfe_attention_args* a, int64_t rows) { return a->packed ? rows : rows * a->n_docs; }
-int cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t partners, int64_t want) {
-    if (a->n_docs < 1 || rows < 1) return 1;
-    const int64_t tiles = (rows + kRows - 1) / kRows, blocks = (a->packed ? tiles : tiles * a->n_docs) * heads;
-    if (a->packed && a->n_docs > 3) partners = partners * 3 / a->n_docs;
-    if (partners < (2 * blocks < want ? 1000 : 2000)) return 1;
-    int64_t n = (want + blocks / 2) / blocks;
-    if (n > partners / 256) n = partners / 256;
-    return n < 1 ? 1 : (int)n;
-}
+// parts of the two walks; a causal mask leaves a key min(rows, keys) rows
 int key_cuts(const mmfe_attention_args* a) {
     const int64_t seen = a->causal && a->prefix == nullptr && a->k_rows < a->q_rows ? a->k_rows : a->q_rows;
-    return cuts(a, a->k_rows, a->kv_heads, seen * (a->heads / a->kv_heads), a->dim > 64 ? 512 : 768);
+    return walk_cuts(a, a->k_rows, a->kv_heads, seen * (a->heads / a->kv_heads), a->dim > 64 ? 512 : 768);
 }
-int row_cuts(const mmfe_attention_args* a) { return cuts(a, a->q_rows, a->heads, a->k_rows, 768); }
+int row_cuts(const mmfe_attention_args* a) { return walk_cuts(a, a->q_rows, a->heads, a->k_rows, 768); }
 int64_t key_parts(const mmfe_attention_args* a) { return key_cuts(a) > 1 ? key_cuts(a) * in_all(a, a->k_rows) * a->kv_heads * a->dim : 0; }
 int64_t parts(const mmfe_attention_args* a) {          // the two passes use them one after the other
     const int64_t q = row_cuts(a) > 1 ? row_cuts(a) * in_all(a, a->q_rows) * a->heads * a->dim : 0;

@@ -543,3 +543,18 @@ LONG = [
 @pytest.mark.parametrize("form, case", LONG, ids=lambda c: c if isinstance(c, str) else f"{c[0]}x{c[-8]}x{c[-6]}")
 def test_gradients_in_parts(mm, O, form, case):
     (test_padded if form == "padded" else test_packed)(mm, O, case)
+
+
+def test_cut_walks_keep_nan_and_empty_rows(mm):
+    """1200 rows over 1200 keys of one head: a NaN in any part of the keys reaches every row that sees it; rows that see no key are zeros."""
+    fn = mm.attention.attention
+    q, k, v = (torch.randn(1, 1200, 1, 64, device="cuda").to(HF) for _ in "qkv")
+    want, lse = fn(q, k, v, lengths=[1000], kv_lengths=[700], causal=True, return_lse=True)        # the first 300 rows see nothing
+    assert (want[0, :300] == 0).all() and (lse[0, 0, :300] == -math.inf).all() and want[0, 300:1000].abs().amin() >= 0
+    assert lse[0, 0, 300:1000].isfinite().all() and (want[0, 1000:] == 0).all() and (lse[0, 0, 1000:] == -math.inf).all()
+    for at in (0, 31, 32, 599, 600, 1199):
+        x = k.clone()
+        x[0, at, 0, 5] = math.nan
+        assert fn(q, x, v).isnan().all()
+        y, l = fn(q, x, v, causal=True, return_lse=True)
+        assert y[0, at:].isnan().all() and l[0, 0, at:].isnan().all() and not y[0, :max(0, at - 63)].isnan().any()
