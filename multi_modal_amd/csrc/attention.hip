@@ -140,15 +140,16 @@ constexpr int kRing = 4;
 constexpr float kLowest = -3e38f;      // maximum of keys that are seen and have scores of -infinity, which no keys at all have
 static_assert(kStepKeys * kRing >= kShortKeys, "a short document's keys are in LDS at once");
 
-template <bool BF, int DP, int SHAPE>
+// CUT: the walk is cut into parts (as an argument that any call could have, 3 % slower where it is not)
+template <bool BF, int DP, int SHAPE, bool CUT>
 __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];               // [kRing k tiles][kRing v tiles]
     const Problem& p = a.p;
     constexpr int kTileBytes = kStepKeys * DP * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int lot = blockIdx.x % (p.heads * a.cuts), cut = lot / p.heads;
+    const int cuts = CUT ? a.cuts : 1, lot = blockIdx.x % (p.heads * cuts), cut = CUT ? lot / p.heads : 0;
     Doc d;
-    if (!find_doc<true>(p, blockIdx.x / (p.heads * a.cuts), kRows, d)) return;
+    if (!find_doc<true>(p, blockIdx.x / (p.heads * cuts), kRows, d)) return;
     const int head = head_of(p, lot % p.heads), kvh = head / p.group;
     const int row0 = d.tile * kRows, w0 = row0 + 32 * wave, row = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
@@ -162,8 +163,8 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     const int full_lim = w0 < nq ? limit(w0) : 0;                             // keys that all rows of the wave see
     const int lim = row < nq ? limit(row) : 0;
     const bool at_once = nk <= kShortKeys;                                    // at most kRing tiles: all of them are asked for at the start
-    const int all = block_lim > 0 ? (block_lim + kStepKeys - 1) / kStepKeys : 0, share = at_once ? all : (all + a.cuts - 1) / a.cuts;
-    const int t0 = min(cut * share, all), n = min(t0 + share, all);           // this block's steps
+    const int all = block_lim > 0 ? (block_lim + kStepKeys - 1) / kStepKeys : 0, share = !CUT || at_once ? all : (all + cuts - 1) / cuts;
+    const int t0 = CUT ? min(cut * share, all) : 0, n = min(t0 + share, all); // this block's steps
 
     typedef Loader<DP, kStepKeys, kWaves> Load;
     Load lk, lv;
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs 
     }
     const float l = both_sum(st.l);
     if (row >= d.rows) return;
-    if (a.cuts > 1) {
+    if constexpr (CUT) {
         const int64_t place = ((int64_t)cut * p.heads + head) * (p.packed ? p.q_rows : p.q_rows * p.n_docs) + (p.packed ? d.q0 : d.batch * p.q_rows) + row;
         const bool sees = lim > t0 * kStepKeys && t0 < n;
         if (half == 0) a.part_ml[place] = sees ? make_float2(st.m == -INFINITY ? kLowest : st.m * unit, l) : make_float2(-INFINITY, 0.f);
@@ -613,14 +614,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const SplitArgs a) {
 
 typedef void (*forward_fn)(const ForwardArgs);
 typedef void (*split_fn)(const SplitArgs);
-template <bool BF, int SHAPE>
+template <bool BF, int SHAPE, bool CUT>
 forward_fn pick_dim(int dim) {
-    return dim <= 32 ? &forward_kernel<BF, 32, SHAPE> : dim <= 64 ? &forward_kernel<BF, 64, SHAPE> : &forward_kernel<BF, 128, SHAPE>;
+    return dim <= 32 ? &forward_kernel<BF, 32, SHAPE, CUT> : dim <= 64 ? &forward_kernel<BF, 64, SHAPE, CUT> : &forward_kernel<BF, 128, SHAPE, CUT>;
 }
-template <bool BF>
+template <bool BF, bool CUT>
 forward_fn pick_forward(int dim, bool bias, bool cap) {
-    if (bias) return cap ? pick_dim<BF, kBias | kCap>(dim) : pick_dim<BF, kBias>(dim);
-    return cap ? pick_dim<BF, kCap>(dim) : pick_dim<BF, kPlain>(dim);
+    if (bias) return cap ? pick_dim<BF, kBias | kCap, CUT>(dim) : pick_dim<BF, kBias, CUT>(dim);
+    return cap ? pick_dim<BF, kCap, CUT>(dim) : pick_dim<BF, kPlain, CUT>(dim);
 }
 template <bool BF>
 split_fn pick_split(int dim) {
@@ -796,7 +797,8 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
         return launched("attention");
     }
     const bool bias = a->slopes != nullptr, cap = a->cap > 0.f;
-    const forward_fn fn = bf ? pick_forward<true>(a->dim, bias, cap) : pick_forward<false>(a->dim, bias, cap);
+    const forward_fn fn = c.cuts > 1 ? (bf ? pick_forward<true, true>(a->dim, bias, cap) : pick_forward<false, true>(a->dim, bias, cap))
+                                     : (bf ? pick_forward<true, false>(a->dim, bias, cap) : pick_forward<false, false>(a->dim, bias, cap));
     const size_t lds = 2 * (size_t)kRing * kStepKeys * padded_dim(a->dim) * 2;
     int blocks = 1, cus = 256;
     rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);
