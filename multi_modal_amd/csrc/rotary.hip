@@ -8,7 +8,8 @@
 // [-1/2, 1/2] and only then rounded to float32, so that positions in the millions keep their phase; float32 products would be
 // off by 2^-24 * position radians.  One angle serves the pair in all query and key heads of its token, so a block computes the
 // angles of its tokens once, keeps their cosines and sines in LDS, and walks the heads of q and k over them in one launch.
-// Rounding: inputs are widened to float32, the result is rounded once to the tensors' type.
+// Rounding: inputs are widened to float32, the result is rounded once to the tensors' type (the fused products are written out, so that
+// every path through the kernel gives the same bits).
 #include "mmfe_internal.h"
 
 #include <cmath>
@@ -51,6 +52,7 @@ struct RotaryArgs {
     int64_t tokens;                      // B * N
     int N, D, R, T;                      // T: tokens of a block
     int chunks;                          // vectors of a head
+    int again;                           // elements may be computed twice (not in place)
     float sign;
     FastDiv dN, dR, dItems, dChunks;     // items of a token = (heads of q + heads of k) * chunks
 };
@@ -89,8 +91,13 @@ __device__ __forceinline__ Vec<E> load_vec(const E* p) {
 template <typename E>
 __device__ __forceinline__ void store_vec(E* p, const Vec<E>& r) { __builtin_memcpy(p, &r, 16); }
 
+// 64 x 192 tokens, 24 heads of 64, float16, out of a packed projection: 15 us (4.9 TB/s); 25088 tokens, 20 heads of 128, bfloat16: 48 us (5.4 TB/s),
+// with sections of 15 + 21 + 27 pairs 67.
+//
 // HALVES: the pair of element i is element i + R; otherwise pairs are (2 i, 2 i + 1).
-// Item = one vector of pairs of one head (HALVES: a vector of first and a vector of second elements).
+// Item = one vector of pairs of one head (HALVES: a vector of first and a vector of second elements).  Where the elements do not fill their last
+// vector, it is moved back over the one before it, and both compute the same values; in place, or with less than a vector, the elements
+// are read one by one, all of them before the first is written (one at a time, each waited for, the sections of 15 + 21 + 27 took 152 us).
 template <typename E, typename P, bool HALVES>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -130,49 +137,69 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs p) {
         const float2* a = cs + t * p.R;
         const int n_rot = HALVES ? (p.R + V - 1) / V : (2 * p.R + V - 1) / V;
         if (c >= n_rot) {                                        // the elements without a pair
-            const int e = 2 * p.R + (c - n_rot) * V;
+            const int e = p.again && p.D - 2 * p.R >= V ? min(2 * p.R + (c - n_rot) * V, p.D - V) : 2 * p.R + (c - n_rot) * V;
             if (e + V <= p.D) store_vec(y + e, load_vec(x + e));
-            else
-                for (int j = e; j < p.D; ++j) y[j] = x[j];
+            else {
+                E u[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) u[j] = x[e + j < p.D ? e + j : e];
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (e + j < p.D) y[e + j] = u[j];
+            }
         } else if constexpr (HALVES) {
-            const int e = c * V;
+            const int e = p.again && p.R >= V ? min(c * V, p.R - V) : c * V;
             if (e + V <= p.R) {
                 Vec<E> u = load_vec(x + e), w = load_vec(x + e + p.R);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float2 k = a[e + j];
                     const float xu = Elem<E>::get(u.v[j]), xw = Elem<E>::get(w.v[j]);
-                    u.v[j] = Elem<E>::put(xu * k.x - xw * k.y);
-                    w.v[j] = Elem<E>::put(xw * k.x + xu * k.y);
+                    u.v[j] = Elem<E>::put(fmaf(xu, k.x, -(xw * k.y)));
+                    w.v[j] = Elem<E>::put(fmaf(xw, k.x, xu * k.y));
                 }
                 store_vec(y + e, u);
                 store_vec(y + e + p.R, w);
             } else {
-                for (int j = e; j < p.R; ++j) {
-                    const float2 k = a[j];
-                    const float xu = Elem<E>::get(x[j]), xw = Elem<E>::get(x[j + p.R]);
-                    y[j] = Elem<E>::put(xu * k.x - xw * k.y);
-                    y[j + p.R] = Elem<E>::put(xw * k.x + xu * k.y);
+                E u[V], w[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int i = e + j < p.R ? e + j : e;
+                    u[j] = x[i];
+                    w[j] = x[i + p.R];
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (e + j >= p.R) continue;
+                    const float2 k = a[e + j];
+                    const float xu = Elem<E>::get(u[j]), xw = Elem<E>::get(w[j]);
+                    y[e + j] = Elem<E>::put(fmaf(xu, k.x, -(xw * k.y)));
+                    y[e + j + p.R] = Elem<E>::put(fmaf(xw, k.x, xu * k.y));
                 }
             }
         } else {
-            const int e = c * V;
+            const int e = p.again && 2 * p.R >= V ? min(c * V, 2 * p.R - V) : c * V;
             if (e + V <= 2 * p.R) {
                 Vec<E> u = load_vec(x + e);
 #pragma unroll
                 for (int j = 0; j < V; j += 2) {
                     const float2 k = a[(e + j) >> 1];
                     const float xu = Elem<E>::get(u.v[j]), xw = Elem<E>::get(u.v[j + 1]);
-                    u.v[j] = Elem<E>::put(xu * k.x - xw * k.y);
-                    u.v[j + 1] = Elem<E>::put(xw * k.x + xu * k.y);
+                    u.v[j] = Elem<E>::put(fmaf(xu, k.x, -(xw * k.y)));
+                    u.v[j + 1] = Elem<E>::put(fmaf(xw, k.x, xu * k.y));
                 }
                 store_vec(y + e, u);
             } else {
-                for (int j = e; j < 2 * p.R; j += 2) {
-                    const float2 k = a[j >> 1];
-                    const float xu = Elem<E>::get(x[j]), xw = Elem<E>::get(x[j + 1]);
-                    y[j] = Elem<E>::put(xu * k.x - xw * k.y);
-                    y[j + 1] = Elem<E>::put(xw * k.x + xu * k.y);
+                E u[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) u[j] = x[e + j < 2 * p.R ? e + j : e];
+#pragma unroll
+                for (int j = 0; j < V; j += 2) {
+                    if (e + j >= 2 * p.R) continue;
+                    const float2 k = a[(e + j) >> 1];
+                    const float xu = Elem<E>::get(u[j]), xw = Elem<E>::get(u[j + 1]);
+                    y[e + j] = Elem<E>::put(fmaf(xu, k.x, -(xw * k.y)));
+                    y[e + j + 1] = Elem<E>::put(fmaf(xw, k.x, xu * k.y));
                 }
             }
         }
@@ -270,10 +297,12 @@ int mmfe_rotary_run(const mmfe_rotary* handle, const mmfe_rotary_args* a, void* 
     p.tokens = a->n_batch * a->n_tokens; p.N = (int)a->n_tokens; p.D = a->dim; p.R = h->R; p.sign = a->inverse ? -1.f : 1.f;
     const int V = a->dtype == MMFE_OUT_F32 ? 4 : 8;
     const bool copy_rest = !(a->q == a->q_out && a->k == a->k_out);      // in place, the elements without a pair stay where they are
+    p.again = !((a->heads_q > 0 && a->q == a->q_out) || (a->heads_k > 0 && a->k == a->k_out));
     p.chunks = ((h->halves ? h->R : 2 * h->R) + V - 1) / V + (copy_rest ? (a->dim - 2 * h->R + V - 1) / V : 0);
     const int64_t items = (int64_t)(a->heads_q + a->heads_k) * p.chunks;
     // A block takes as many tokens as give its threads 4 items each, within the LDS image of the angles (16 KB) and within what
-    // leaves a block for every CU: one new token per stream gets a block per token.
+    // leaves two blocks for every CU.  One token a block: 20000 tokens, 12 heads of 64: 21.6 us in place of 12.6; one new token of 8 streams in one block:
+    // 4.0 us, in 8 blocks 3.0; 8 items a thread: 20000 tokens, 12 heads of 128, float32: 49 us, with 4 42.
     int64_t T = (4 * kThreads + items - 1) / items;
     if (T > kMaxTokens) T = kMaxTokens;
     if (T > 2048 / h->R) T = 2048 / h->R;

@@ -314,3 +314,15 @@ def test_clip_graph(mm):
         graph.replay()
         n = mm.clip_grad_norm(want, 1.0)
         assert torch.equal(n, norm) and all(torch.equal(a, b) for a, b in zip(x, want))
+
+
+@pytest.mark.parametrize("case", [
+    (3, 301, 5, 2, 128, [1, 4], "axis", "halves", torch.float16),           # fewer pairs than a vector, a long rest
+    (3, 301, 5, 2, 64, [1, 2], "axis", "adjacent", torch.bfloat16),
+    (2, 130, 2, 2, 64, [16, 15], "shared", "halves", torch.bfloat16),       # a rest of two elements
+    (2, 130, 2, 1, 41, [5], "axis", "halves", torch.float32),
+    (1, 9, 1, 1, 6, [3], "axis", "adjacent", torch.float16),                # a head smaller than a vector
+    (2, 600, 16, 4, 128, [15, 21, 27], "shared", "halves", torch.float16),
+], ids=lambda c: "x".join(map(str, c[:5])))
+def test_rotary_sections_of_any_size(mm, case):
+    test_rotary(mm, case, True)
