@@ -145,7 +145,7 @@ template <bool BF, int DP, int SHAPE, bool CUT>
 __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const ForwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];               // [kRing k tiles][kRing v tiles]
     const Problem& p = a.p;
-    constexpr int kTileBytes = kStepKeys * DP * 2;
+    constexpr int kTileBytes = kStepKeys * kPitch<DP> * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int cuts = CUT ? a.cuts : 1, lot = blockIdx.x % (p.heads * cuts), cut = CUT ? lot / p.heads : 0;
     Doc d;
@@ -404,7 +404,7 @@ template <bool BF, int DP>
 __global__ void __launch_bounds__(64 * kSplitWaves, 1) split_kernel(const SplitArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // per wave: 2 x [k tile][v tile]
     const Problem& p = a.f.p;
-    constexpr int kTileBytes = kSplitTile * DP * 2;
+    constexpr int kTileBytes = kSplitTile * kPitch<DP> * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     // Chunk by chunk, the units of a chunk turned by the chunk's number: neighbouring blocks go to different XCDs, and a document's chunks
     // (long documents have many, short ones one) then spread over all of them, while the key heads of a chunk's keys, which lie
@@ -526,15 +526,15 @@ __global__ void __launch_bounds__(64 * kSplitWaves, 1) split_kernel(const SplitA
     // the waves' results meet in LDS: [wave][row][DP + 4] values, [wave][row] maximum and sum
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     block_sync();
-    constexpr int kPitch = DP + 4;
+    constexpr int kMeet = DP + 4;
     float* wo = reinterpret_cast<float*>(smem);
-    float2* wml = reinterpret_cast<float2*>(wo + kSplitWaves * 32 * kPitch);
+    float2* wml = reinterpret_cast<float2*>(wo + kSplitWaves * 32 * kMeet);
     if (col < n_rows) {
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4*>(wo + (wave * 32 + col) * kPitch + 32 * i + 8 * g + 4 * half) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+                *reinterpret_cast<float4*>(wo + (wave * 32 + col) * kMeet + 32 * i + 8 * g + 4 * half) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
         if (half == 0) wml[wave * 32 + col] = make_float2(m, l);
     }
     __syncthreads();
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(64 * kSplitWaves, 1) split_kernel(const SplitA
             const float2 s = wml[w * 32 + r];
             if (s.y == 0.f) continue;                                 // saw no key
             const float k = exp2_fast(s.x - top);
-            const float4 u = *reinterpret_cast<const float4*>(wo + (w * 32 + r) * kPitch + e);
+            const float4 u = *reinterpret_cast<const float4*>(wo + (w * 32 + r) * kMeet + e);
             total += k * s.y;
             v.x += k * u.x; v.y += k * u.y; v.z += k * u.z; v.w += k * u.w;
         }
@@ -616,7 +616,7 @@ typedef void (*forward_fn)(const ForwardArgs);
 typedef void (*split_fn)(const SplitArgs);
 template <bool BF, int SHAPE, bool CUT>
 forward_fn pick_dim(int dim) {
-    return dim <= 32 ? &forward_kernel<BF, 32, SHAPE, CUT> : dim <= 64 ? &forward_kernel<BF, 64, SHAPE, CUT> : &forward_kernel<BF, 128, SHAPE, CUT>;
+    return dim <= 32 ? &forward_kernel<BF, 32, SHAPE, CUT> : dim <= 64 ? &forward_kernel<BF, 64, SHAPE, CUT> : dim <= 96 ? &forward_kernel<BF, 96, SHAPE, CUT> : &forward_kernel<BF, 128, SHAPE, CUT>;
 }
 template <bool BF, bool CUT>
 forward_fn pick_forward(int dim, bool bias, bool cap) {
@@ -625,7 +625,7 @@ forward_fn pick_forward(int dim, bool bias, bool cap) {
 }
 template <bool BF>
 split_fn pick_split(int dim) {
-    return dim <= 32 ? &split_kernel<BF, 32> : dim <= 64 ? &split_kernel<BF, 64> : &split_kernel<BF, 128>;
+    return dim <= 32 ? &split_kernel<BF, 32> : dim <= 64 ? &split_kernel<BF, 64> : dim <= 96 ? &split_kernel<BF, 96> : &split_kernel<BF, 128>;
 }
 
 // How a call's keys are cut: chunks of split_kernel (n_splits > 0), or parts of forward_kernel's walks.
@@ -692,7 +692,8 @@ int walk_cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t par
     return n < 1 ? 1 : (int)n;
 }
 
-int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+int pitch(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 bool bad_rows(const char* name, const void* ptr, const int64_t* s) {
     // 16-byte pieces; a tile's rows are reached by 32-bit byte offsets
@@ -786,8 +787,7 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
         s.part = static_cast<float*>(workspace);
         s.part_ml = c.n_splits > 1 ? s.part + c.units * c.n_splits * 32 * a->dim : nullptr;
         const split_fn fn = bf ? pick_split<true>(a->dim) : pick_split<false>(a->dim);
-        const int dp = padded_dim(a->dim);
-        const size_t tiles = (size_t)kSplitWaves * 4 * kSplitTile * dp * 2, meet = (size_t)kSplitWaves * 32 * ((dp + 4) * 4 + 8);
+        const size_t tiles = (size_t)kSplitWaves * 4 * kSplitTile * pitch(a->dim) * 2, meet = (size_t)kSplitWaves * 32 * ((padded_dim(a->dim) + 4) * 4 + 8);
         const size_t lds = tiles > meet ? tiles : meet;
         int blocks = 1, cus = 256;
         rc = kernel_prepare(reinterpret_cast<const void*>(fn), 64 * kSplitWaves, lds, &blocks, &cus);
@@ -799,7 +799,7 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
     const bool bias = a->slopes != nullptr, cap = a->cap > 0.f;
     const forward_fn fn = c.cuts > 1 ? (bf ? pick_forward<true, true>(a->dim, bias, cap) : pick_forward<false, true>(a->dim, bias, cap))
                                      : (bf ? pick_forward<true, false>(a->dim, bias, cap) : pick_forward<false, false>(a->dim, bias, cap));
-    const size_t lds = 2 * (size_t)kRing * kStepKeys * padded_dim(a->dim) * 2;
+    const size_t lds = 2 * (size_t)kRing * kStepKeys * pitch(a->dim) * 2;
     int blocks = 1, cus = 256;
     rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);
     if (rc) return rc;

@@ -95,12 +95,12 @@ __device__ __forceinline__ float phi_of(float bound) {
 }
 
 // What both passes need of every row: delta and lse2 (blocks below q_blocks, 128 rows of one head each), and for float16 the tiles' largest
-// squared norms of g and, in the blocks behind, of v.  DP / 8 lanes share a row.
+// squared norms of g and, in the blocks behind, of v.  One lane has 8 elements of a row.
 template <bool BF, int DP>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const BackwardArgs a) {
     __shared__ float lds[kWaves];
     Problem p = a.p;
-    constexpr int kLanes = DP / 8;
+    constexpr int kLanes = kPitch<DP> / 8;
     const int e = (threadIdx.x & (kLanes - 1)) * 8;
     Doc d;
     float biggest = 0.f;
@@ -288,12 +288,13 @@ constexpr int kRing = 4;              // tiles in LDS: the one in use, the next 
 //
 // dk and dv of 128 keys, 32 per wave, over tiles of 64 rows.  Step u turns the scores of its rows (computed a step earlier) into p and
 // ds beside the products of the next rows, then adds them to dv and dk; its tiles stay until then, and it asks for those of step u + 3.
-// Head size 128 has one wave per SIMD (357 registers), the smaller ones two.
+// Head sizes past 64 have one wave per SIMD (128: 357 registers; 96: 283, and with two waves and what does not fit in memory, 4096 rows, 12 heads of
+// 72 take 428 us in place of 352), the smaller ones two.
 template <bool BF, int DP, bool CAP>
-__global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const BackwardArgs a) {
+__global__ void __launch_bounds__(kThreads, DP > 64 ? 1 : 2) keys_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][row statistics]
     const Problem& p = a.p;
-    constexpr int kTileBytes = kTile * DP * 2;
+    constexpr int kTileBytes = kTile * kPitch<DP> * 2;
     constexpr int kBuf = 2 * kTileBytes + kTile * 16;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int lot = blockIdx.x % (p.kv_heads * a.k_cuts), kvh = lot % p.kv_heads, cut = lot / p.kv_heads;
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [k tile][v tile]
     const Problem& p = a.p;
     constexpr int kKeys = 32;
-    constexpr int kTileBytes = kKeys * DP * 2;
+    constexpr int kTileBytes = kKeys * kPitch<DP> * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     Doc d;
     const int lot = blockIdx.x % (p.heads * a.q_cuts), cut = lot / p.heads;
@@ -782,7 +783,7 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     if (tk > 0) {
         p.tiles = b.k_tiles;
         const auto fn = &keys_kernel<BF, DP, CAP>;
-        const size_t lds = kRing * (2 * (size_t)kTile * DP * 2 + kTile * 16);
+        const size_t lds = kRing * (2 * (size_t)kTile * kPitch<DP> * 2 + kTile * 16);
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
         hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.k_cuts)), dim3(kThreads), lds, stream, b);
         if (b.k_cuts > 1) {
@@ -793,7 +794,7 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     if (tq > 0) {
         p.tiles = b.q_tiles;
         const auto fn = &rows_kernel<BF, DP, CAP>;
-        const size_t lds = kRing * 2 * (size_t)32 * DP * 2;
+        const size_t lds = kRing * 2 * (size_t)32 * kPitch<DP> * 2;
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
         hipLaunchKernelGGL(fn, dim3((uint32_t)(tq * p.heads * b.q_cuts)), dim3(kThreads), lds, stream, b);
         if (b.q_cuts > 1) {
@@ -807,7 +808,7 @@ int launch(BackwardArgs& b, hipStream_t stream) {
 template <bool BF, bool CAP>
 int launch_dim(BackwardArgs& b, hipStream_t stream) {
     const int dp = padded_dim(b.p.dim);
-    return dp == 32 ? launch<BF, 32, CAP>(b, stream) : dp == 64 ? launch<BF, 64, CAP>(b, stream) : launch<BF, 128, CAP>(b, stream);
+    return dp == 32 ? launch<BF, 32, CAP>(b, stream) : dp == 64 ? launch<BF, 64, CAP>(b, stream) : dp == 96 ? launch<BF, 96, CAP>(b, stream) : launch<BF, 128, CAP>(b, stream);
 }
 
 // places of the norms' tiles (see slot)
