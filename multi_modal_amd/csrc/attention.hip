@@ -637,8 +637,11 @@ split_fn pick_split(int dim) {
 //   - up to 512 keys, and up to 2048 where 256 units fill the CUs: no chunks; the row kernel, unless units share keys and its blocks do not all run
 //     at once (128 streams of 500 keys, one row, 16 heads on 4: 26.6 us, row kernel 61.4; 32 of them 17.3 and 18.3; 64 rows of 32 documents
 //     of 1000 keys, 12 heads of 64: 27, in chunks of 512 keys 75)
-//   - more rows than a unit takes, in more than 64 units: the row kernel, its walks cut (8000 keys, 16 heads on 4 of 128, 512 rows: 61 us, uncut 172, in
-//     chunks 120; 128 rows, 64 units: 39 in chunks, 173 uncut; 4 documents of 128 rows, 2000 keys, 12 heads on 4 of 64, 192 units: 24 cut, 33 in chunks)
+//   - more than 64 units, nearly as many as the row kernel's blocks or more: the row kernel, its walks cut (8000 keys, 16 heads on 4 of 128, 512 rows: 61 us,
+//     uncut 172, in chunks 120; 128 rows, 64 units: 39 in chunks, 173 uncut; 8 documents of 32 rows, 6000 keys, 16 heads on 4 of 128: 49 cut, 63 in
+//     chunks; of 9 rows, half as many units as blocks: 47 cut, 44 in chunks)
+//     Documents with lengths of their own may be much shorter than their room, so parts of more than 2048 keys are cut as long as that makes no
+//     more than four times the blocks: 16 documents of 32 rows over 1000 to 30001 keys in 32768, 16 heads on 4 of 128: 356 us without, 183 with
 //   - else chunks that make 512 blocks, two on each CU, of 256 keys at least, and of 1024 at most (documents shorter than their room leave chunks
 //     empty) unless that makes more than 2048: 16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 109 / 93 / 100 / 113 us with 512 /
 //     1024 / 2048 / 4096 keys; 32 streams of 2000 keys, one row, 4 key heads of 128: 39 / 34 / 33 with 256 / 512 / 1024.
@@ -649,13 +652,15 @@ struct Cut {
 };
 Cut cut_keys(const mmfe_attention_args* a) {
     Cut c;
-    c.cuts = std::min(12, walk_cuts(a, a->q_rows, a->heads, a->k_rows, a->dim > 64 ? 512 : 768));
-    if (a->packed || a->q_rows < 1 || a->n_docs < 1) return c;
     const int64_t keys = a->k_rows, row_tiles = (a->q_rows * (a->heads / a->kv_heads) + 31) / 32, units = a->n_docs * row_tiles * a->kv_heads;
-    const int64_t blocks = a->n_docs * ((a->q_rows + kRows - 1) / kRows) * a->heads;       // of the row kernel
+    const int64_t blocks = a->n_docs * ((a->q_rows + kRows - 1) / kRows) * a->heads;       // of the row kernel, of padded documents
+    const int want = a->dim > 64 ? 512 : 768;
+    c.cuts = std::min(12, walk_cuts(a, a->q_rows, a->heads, keys, want));
+    if (a->packed || a->q_rows < 1 || a->n_docs < 1) return c;
+    if (a->k_len != nullptr) c.cuts = (int)std::max<int64_t>(c.cuts, std::min<int64_t>(16, std::min(keys / 2048, 4 * want / blocks)));
     if (keys <= kShortKeys) return c;
     const bool whole = keys <= 512 || (keys <= 2048 && units >= 256);
-    if (whole ? units >= blocks || blocks <= 512 : units > blocks && units > 64) return c;
+    if (whole ? units >= blocks || blocks <= 512 : units > 64 && 5 * units >= 4 * blocks) return c;
     const int64_t all = keys * units;
     int64_t chunk = (all + 511) / 512, most = (all + 2047) / 2048;
     if (most < 1024) most = 1024;
@@ -775,7 +780,7 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
     f.lse = a->lse; f.lse_b = a->lse_stride[0]; f.lse_h = a->lse_stride[1];
     const Cut c = cut_keys(a);
     if ((c.n_splits > 1 || c.cuts > 1) && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
-    if (c.units * c.n_splits > 0x7fffffffll || c.units > 0x3ffffff) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
+    if (c.units * c.n_splits > 0x7fffffffll || c.units > 0x3ffffff || tiles * a->heads * c.cuts > 0x7fffffffll) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
     OnDevice on(device);
     if (on.rc) return on.rc;
     const bool bf = a->dtype == MMFE_OUT_BF16;
