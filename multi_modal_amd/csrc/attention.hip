@@ -137,7 +137,7 @@ __device__ __forceinline__ void hide(f32x16& x, int left) {
 // Keys of a step, and tiles of keys (and of values) in LDS.
 constexpr int kStepKeys = 32;
 constexpr int kRing = 4;
-constexpr float kLowest = -__FLT_MAX__;// maximum of keys that are seen and have scores of -infinity, which no keys at all have
+constexpr float kLowest = -__FLT_MAX__;      // maximum of keys that are seen and have scores of -infinity, which no keys at all have
 static_assert(kStepKeys * kRing >= kShortKeys, "a short document's keys are in LDS at once");
 
 // CUT: the walk is cut into parts (as an argument that any call could have, 3 % slower where it is not)
