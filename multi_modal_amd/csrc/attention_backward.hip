@@ -454,7 +454,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum a) {
 
 // dq of 128 rows, 32 per wave, over tiles of 32 keys; steps overlap as in keys_kernel.  Head size 64 is held to 168 registers for three waves
 // a SIMD (6 of them spilled): 8192 rows, 12 heads, 840 -> 954 TFLOP/s without a mask, 871 -> 830 under a causal one.
-template <bool BF, int DP, bool CAP>
+// CUT: the walk is cut into parts (as an argument that any call could have, 4 to 25 % slower where it is not).
+template <bool BF, int DP, bool CAP, bool CUT>
 __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [k tile][v tile]
     const Problem& p = a.p;
@@ -462,8 +463,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     constexpr int kTileBytes = kKeys * kPitch<DP> * 2;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     Doc d;
-    const int lot = blockIdx.x % (p.heads * a.q_cuts), cut = lot / p.heads;
-    if (!find_doc<true>(p, blockIdx.x / (p.heads * a.q_cuts), kRows, d)) return;
+    const int cuts = CUT ? a.q_cuts : 1, lot = blockIdx.x % (p.heads * cuts), cut = CUT ? lot / p.heads : 0;
+    if (!find_doc<true>(p, blockIdx.x / (p.heads * cuts), kRows, d)) return;
     const int head = head_of(p, lot % p.heads), kvh = head / p.group;
     const int row0 = d.tile * kRows, w0 = row0 + 32 * wave, row = w0 + col;
     const int nq = d.nq, nk = d.nk, off = nk - nq;
@@ -475,8 +476,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     const int wave_lim = w0 < nq ? limit(w0 + 31) : 0;
     const int full_lim = w0 < nq ? limit(w0) : 0;
     const int lim = row < nq ? limit(row) : 0;
-    const int all = block_lim > 0 ? (block_lim + kKeys - 1) / kKeys : 0, part = (all + a.q_cuts - 1) / a.q_cuts;
-    const int t0 = min(cut * part, all), n = min(t0 + part, all);     // this block's tiles
+    const int all = block_lim > 0 ? (block_lim + kKeys - 1) / kKeys : 0, part = CUT ? (all + cuts - 1) / cuts : all;
+    const int t0 = CUT ? min(cut * part, all) : 0, n = CUT ? min(t0 + part, all) : all;       // this block's tiles
 
     typedef Loader<DP, kKeys, kWaves> Load;
     Load lk, lv;
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     if (row >= d.rows) return;
     const float by = p.scale * __builtin_amdgcn_exp2f(-kShift<BF>) / phi * sh.factor();
     const bool some = lim > 1;                                        // a softmax over one key is constant
-    if (a.q_cuts == 1) {
+    if constexpr (!CUT) {
         store_rows<BF, DP>(const_cast<char*>(row_base(a.dq, d, d.q0 + row, head)), dq, p.dim, by, some);
         return;
     }
@@ -793,7 +794,7 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     }
     if (tq > 0) {
         p.tiles = b.q_tiles;
-        const auto fn = &rows_kernel<BF, DP, CAP>;
+        const auto fn = b.q_cuts > 1 ? &rows_kernel<BF, DP, CAP, true> : &rows_kernel<BF, DP, CAP, false>;
         const size_t lds = kRing * 2 * (size_t)32 * kPitch<DP> * 2;
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
         hipLaunchKernelGGL(fn, dim3((uint32_t)(tq * p.heads * b.q_cuts)), dim3(kThreads), lds, stream, b);
