@@ -280,6 +280,9 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[DP / 32], const char* t
 }
 
 constexpr int kRing = 4;              // tiles in LDS: the one in use, the next one's scores, two on their way
+template <int DP>
+constexpr int kKeysTile = DP == 96 ? 32 : 64;          // rows of keys_kernel's tiles
+constexpr int kStatBytes = 64 * 16;                    // of a tile's row statistics (one DMA)
 
 // Row statistics come as a third kind of operand: prepare_kernel leaves -lse and -delta of each row as three bfloat16 values that add
 // up to the float32, and a product with ones adds them to a row's scores and dp, over all keys at once.  Read as numbers they
@@ -288,14 +291,16 @@ constexpr int kRing = 4;              // tiles in LDS: the one in use, the next 
 //
 // dk and dv of 128 keys, 32 per wave, over tiles of 64 rows.  Step u turns the scores of its rows (computed a step earlier) into p and
 // ds beside the products of the next rows, then adds them to dv and dk; its tiles stay until then, and it asks for those of step u + 3.
-// Head sizes past 64 have one wave per SIMD (128: 357 registers; 96: 283, and with two waves and what does not fit in memory, 4096 rows, 12 heads of
-// 72 take 428 us in place of 352), the smaller ones two.
+// Head size 128 has one wave per SIMD (357 registers), 64 and less two.  At 96, with half the tile and without the overlap, two blocks fit a CU, and one's
+// products run beside the other's exponentials: 8192 rows, 12 heads on 4, 987 -> 636 us, causal 518 -> 337 (4096 rows, 12 heads of 72: 356 -> 209).
+// The same at 128 leaves 41 registers in memory: 744 -> 673 us for 8 heads of 8192 rows, but causal 403 -> 413 with the walks cut and 636 without.
 template <bool BF, int DP, bool CAP>
-__global__ void __launch_bounds__(kThreads, DP > 64 ? 1 : 2) keys_kernel(const BackwardArgs a) {
+__global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][row statistics]
     const Problem& p = a.p;
+    constexpr int kTile = kKeysTile<DP>;
     constexpr int kTileBytes = kTile * kPitch<DP> * 2;
-    constexpr int kBuf = 2 * kTileBytes + kTile * 16;
+    constexpr int kBuf = 2 * kTileBytes + kStatBytes;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int lot = blockIdx.x % (p.kv_heads * a.k_cuts), kvh = lot % p.kv_heads, cut = lot / p.kv_heads;
     Doc d;
@@ -360,50 +365,65 @@ __global__ void __launch_bounds__(kThreads, DP > 64 ? 1 : 2) keys_kernel(const B
     block_sync();
     arrived(kf);
     arrived(vf);
-    if (steps > 0) products(smem, 0, x, dp);
     Shape<CAP> sh;
     sh.set(p, head0 + g);
+    // p and ds of 32 rows, from their scores and dp - delta, into dv and dk
+    auto before = [&](const char* qt, int b, f32x16& x, f32x16& w) {
+        const int i0 = t * kTile + 32 * b;
+        f32x16 add;
+        if constexpr (CAP) {
+            const u32x4 st = statistics(qt, b);
+            add = mfma<true>(u32x4{st.x, st.y, 0u, 0u}, ones, f32x16{});
+        }
+        sh.template apply<true>(x, w, [&](int i) { return add[i]; }, (float)(i0 + 4 * half + off - key), 1.f);
+        if (i0 < wave_full || i0 + 32 > nq) {
+            const int lo = my_first - i0 - 4 * half, hi = nq - i0 - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = reg_row(i) >= lo && reg_row(i) < hi ? x[i] : -INFINITY;
+        }
+    };
+    auto behind = [&](const char* qt, int b, f32x16& x, f32x16& dp, const f32x16& w) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = exp2_fast(x[i]);
+            dp[i] *= x[i];
+            if constexpr (!BF) dp[i] *= phi;
+            if constexpr (CAP) dp[i] *= w[i];
+        }
+        accumulate<BF, DP>(dv, qt + kTileBytes, 32 * b, x, nk <= kShortKeys);
+        accumulate<BF, DP>(dk, qt, 32 * b, dp, nk <= kShortKeys);
+    };
+    auto live = [&](int b) {
+        const int i0 = t * kTile + 32 * b;
+        return i0 + 32 > wave_first && i0 < nq;
+    };
+    if constexpr (kTile == 64) {
+        if (steps > 0) products(smem, 0, x, dp);
+    }
     for (int step = 0; step < steps; ++step) {
-        if (step + kRing - 2 < steps) wait_but<2 * Load::kCount>();   // tile step + 1 is there; what step - 1 asked for may be on its way
+        // one step ahead, tile step + 1 is there, and what step - 1 asked for may be on its way; otherwise tile step, and two
+        if (step + kRing - 2 < steps) wait_but<(kTile == 64 ? 2 : 4) * Load::kCount>();
         else wait_all();
         block_sync();
         if (step + kRing - 1 < steps) stage();
         const char* qt = smem + (step % kRing) * kBuf;
-        const char* next = smem + ((step + 1) % kRing) * kBuf;
-        const char* gt = qt + kTileBytes;
+        f32x16 w;
+        if constexpr (kTile == 64) {
+            const char* next = smem + ((step + 1) % kRing) * kBuf;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int i0 = t * kTile + 32 * b;
-            const bool live = i0 + 32 > wave_first && i0 < nq;
-            f32x16 w;
-            if (live) {
-                f32x16 add;
-                if constexpr (CAP) {
-                    const u32x4 st = statistics(qt, b);
-                    add = mfma<true>(u32x4{st.x, st.y, 0u, 0u}, ones, f32x16{});
-                }
-                sh.template apply<true>(x, w, [&](int i) { return add[i]; }, (float)(i0 + 4 * half + off - key), 1.f);
-                if (i0 < wave_full || i0 + 32 > nq) {
-                    const int lo = my_first - i0 - 4 * half, hi = nq - i0 - 4 * half;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = reg_row(i) >= lo && reg_row(i) < hi ? x[i] : -INFINITY;
-                }
+            for (int b = 0; b < 2; ++b) {
+                const bool on = live(b);
+                if (on) before(qt, b, x, w);
+                f32x16 nx, nd;
+                products(b == 0 ? qt : next, 1 - b, nx, nd);
+                if (on) behind(qt, b, x, dp, w);
+                x = nx;
+                dp = nd;
             }
-            f32x16 nx, nd;
-            products(b == 0 ? qt : next, 1 - b, nx, nd);
-            if (live) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[i] = exp2_fast(x[i]);
-                    dp[i] *= x[i];
-                    if constexpr (!BF) dp[i] *= phi;
-                    if constexpr (CAP) dp[i] *= w[i];
-                }
-                accumulate<BF, DP>(dv, gt, 32 * b, x, nk <= kShortKeys);
-                accumulate<BF, DP>(dk, qt, 32 * b, dp, nk <= kShortKeys);
-            }
-            x = nx;
-            dp = nd;
+        } else if (live(0)) {
+            products(qt, 0, x, dp);
+            before(qt, 0, x, w);
+            behind(qt, 0, x, dp, w);
         }
         if (++t == t_end) {
             t = t_first;
@@ -784,7 +804,7 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     if (tk > 0) {
         p.tiles = b.k_tiles;
         const auto fn = &keys_kernel<BF, DP, CAP>;
-        const size_t lds = kRing * (2 * (size_t)kTile * kPitch<DP> * 2 + kTile * 16);
+        const size_t lds = kRing * (2 * (size_t)kKeysTile<DP> * kPitch<DP> * 2 + kStatBytes);
         if ((rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus)) != MMFE_OK) return rc;
         hipLaunchKernelGGL(fn, dim3((uint32_t)(tk * p.kv_heads * b.k_cuts)), dim3(kThreads), lds, stream, b);
         if (b.k_cuts > 1) {
@@ -824,7 +844,7 @@ bool is_whole(const mmfe_attention_args* a) {
 // parts of the two walks; a causal mask leaves a key min(rows, keys) rows
 int key_cuts(const mmfe_attention_args* a) {
     const int64_t seen = a->causal && a->prefix == nullptr && a->k_rows < a->q_rows ? a->k_rows : a->q_rows;
-    return walk_cuts(a, a->k_rows, a->kv_heads, seen * (a->heads / a->kv_heads), a->dim > 64 ? 512 : 768);
+    return walk_cuts(a, a->k_rows, a->kv_heads, seen * (a->heads / a->kv_heads), a->dim > 96 ? 512 : 768);
 }
 int row_cuts(const mmfe_attention_args* a) { return walk_cuts(a, a->q_rows, a->heads, a->k_rows, 768); }
 int64_t key_parts(const mmfe_attention_args* a) { return key_cuts(a) > 1 ? key_cuts(a) * in_all(a, a->k_rows) * a->kv_heads * a->dim : 0; }

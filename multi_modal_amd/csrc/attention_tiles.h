@@ -211,7 +211,7 @@ __device__ __forceinline__ const char* row_base(const Rows& r, const Doc& d, int
 // ---- LDS tiles ----
 
 // DP, the head size that the products run over, is 32, 64, 96 or 128; a row of 96 lies in the place of 128.  4096 rows, 12 heads of 72, bfloat16: forward
-// 124 us, gradients 352 + 137; as 128: 141, 419 + 176.
+// 124 us, gradients 209 + 137; as 128: 141, 419 + 176.
 template <int DP>
 constexpr int kPitch = DP == 96 ? 128 : DP;
 
