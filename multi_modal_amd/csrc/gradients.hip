@@ -152,17 +152,17 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const NormArgs p) {
 }
 
 // Norm from the partials, in every thread.
-__device__ __forceinline__ float total_norm(const double* partial, uint32_t n, int max_kind, double* lds) {
+__device__ __forceinline__ double total_norm(const double* partial, uint32_t n, int max_kind, double* lds) {
     double v = 0;
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) v = max_kind ? max_nan(v, partial[i]) : v + partial[i];
     v = block_reduce(v, max_kind, lds);
-    return (float)(max_kind ? v : sqrt(v));
+    return max_kind ? v : sqrt(v);
 }
 
 __global__ void __launch_bounds__(kThreads) total_kernel(const double* partial, uint32_t n, int max_kind, float* norm) {
     __shared__ double lds[kThreads / 64];
-    const float v = total_norm(partial, n, max_kind, lds);
-    if (threadIdx.x == 0) *norm = v;
+    const double v = total_norm(partial, n, max_kind, lds);
+    if (threadIdx.x == 0) *norm = (float)v;
 }
 
 template <typename E, typename F>
@@ -192,9 +192,10 @@ __device__ __forceinline__ void chunk_scale_to(const E* x, void* y, int64_t at, 
 
 __global__ void __launch_bounds__(kThreads) scale_kernel(const ScaleArgs p) {
     __shared__ double lds[kThreads / 64];
-    const float norm = total_norm(p.partial, p.n_partial, p.max_kind, lds);
-    if (p.store && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = norm;
-    float c = p.max_norm / (norm + 1e-6f);
+    const double norm = total_norm(p.partial, p.n_partial, p.max_kind, lds);
+    if (p.store && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = (float)norm;
+    // rounded once, and the product once; a norm that float32 does not hold counts as the infinity it is returned as
+    float c = isinf((float)norm) ? 0.f : (float)(p.max_norm / (norm + 1e-6));
     if (c > 1.f) c = 1.f;                                        // a NaN norm stays a NaN and reaches every gradient
     for (uint32_t k = blockIdx.x; k < p.n_chunks; k += gridDim.x) {
         const int t = find(p.first, p.n_tensors, k);

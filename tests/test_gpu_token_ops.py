@@ -326,3 +326,17 @@ def test_clip_graph(mm):
 ], ids=lambda c: "x".join(map(str, c[:5])))
 def test_rotary_sections_of_any_size(mm, case):
     test_rotary(mm, case, True)
+
+
+def test_clipping_rounds_twice_and_infinite_norms_give_zeros(mm):
+    """The factor is rounded once and the product once: 2 halves of 2^-23.  A norm past float32's range is infinite and leaves zeros."""
+    g = [torch.randn(3000, device="cuda", generator=torch.Generator("cuda").manual_seed(i)) * 10.0 ** (i - 3) for i in range(6)]
+    exact = math.sqrt(sum(float(t.double().square().sum()) for t in g))
+    factor = 0.5 / (exact + 1e-6)
+    want = [t.double() * factor for t in g]
+    norm = mm.clip_grad_norm(g, 0.5)
+    assert abs(float(norm) - exact) <= 2.0 ** -24 * exact
+    for a, b in zip(g, want):
+        assert ((a.double() - b).abs() <= 2.01 * 2.0 ** -24 * b.abs()).all()
+    big = torch.full((8,), 3e38, device="cuda")
+    assert mm.clip_grad_norm([big], 1.0).isinf() and (big == 0).all()
