@@ -558,3 +558,44 @@ def test_cut_walks_keep_nan_and_empty_rows(mm):
         assert fn(q, x, v).isnan().all()
         y, l = fn(q, x, v, causal=True, return_lse=True)
         assert y[0, at:].isnan().all() and l[0, 0, at:].isnan().all() and not y[0, :max(0, at - 63)].isnan().any()
+
+
+@pytest.mark.parametrize("rows, keys, heads, kv", [(1200, 1200, 2, 1), (3, 5000, 4, 2), (200, 3000, 2, 2)])
+def test_cut_walks_in_graphs(mm, rows, keys, heads, kv):
+    """Two graphs of calls whose walks are cut, each with its workspaces, replayed in turn and between eager calls on another stream."""
+    fn = mm.attention.attention
+
+    def make(seed):
+        gen = torch.Generator("cuda").manual_seed(seed)
+        t = [torch.randn(2, n, h, 64, device="cuda", generator=gen).to(HF) for n, h in ((rows, heads), (keys, kv), (keys, kv), (rows, heads))]
+        return t + [torch.tensor([keys, keys // 2], dtype=torch.int32, device="cuda")]
+
+    def step(q, k, v, g, lens):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        o = fn(q, k, v, kv_lengths=lens, causal=True)
+        return (o.detach(),) + torch.autograd.grad(o, [q, k, v], g)
+    sets = [make(0), make(1)]
+    for s in sets:
+        step(*s)
+    graphs = []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = step(*s)
+        graphs.append((g, got))
+    side = torch.cuda.Stream()
+    for i in range(3):
+        for s, fresh in zip(sets, (make(10 + i), make(20 + i))):
+            for a, b in zip(s, fresh):
+                a.copy_(b)
+            s[4][1] = keys // 2 - i
+        graphs[0][0].replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step(*sets[1])
+        graphs[1][0].replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for (_, got), s in zip(graphs, sets):
+            assert all(torch.equal(a, b) for a, b in zip(got, step(*s)))
+        assert all(torch.equal(a, b) for a, b in zip(other, graphs[1][1]))
+        torch.cuda.synchronize()
