@@ -647,8 +647,9 @@ split_fn pick_split(int dim) {
 //   - more than 64 units, nearly as many as the row kernel's blocks or more: the row kernel, its walks cut (8000 keys, 16 heads on 4 of 128, 512 rows: 61 us,
 //     uncut 172, in chunks 120; 128 rows, 64 units: 39 in chunks, 173 uncut; 8 documents of 32 rows, 6000 keys, 16 heads on 4 of 128: 49 cut, 63 in
 //     chunks; of 9 rows, half as many units as blocks: 47 cut, 44 in chunks)
-//     Documents with lengths of their own may be much shorter than their room, so parts of more than 2048 keys are cut as long as that makes no
-//     more than four times the blocks: 16 documents of 32 rows over 1000 to 30001 keys in 32768, 16 heads on 4 of 128: 356 us without, 183 with
+//     Several documents with lengths of their own may be much shorter than their room: up to 128 rows of each are then cut into parts of 2048 keys as
+//     long as that makes no more than four times the blocks (16 documents of 32 rows over 1000 to 30001 keys in 32768, 16 heads on 4 of 128: 356 us
+//     without, 183 with; 8192 rows of one, 16 heads: 370 without, 415 with)
 //   - else chunks that make 512 blocks, two on each CU, of 256 keys at least, and of 1024 at most (documents shorter than their room leave chunks
 //     empty) unless that makes more than 2048: 16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 109 / 93 / 100 / 113 us with 512 /
 //     1024 / 2048 / 4096 keys; 32 streams of 2000 keys, one row, 4 key heads of 128: 39 / 34 / 33 with 256 / 512 / 1024.
@@ -664,7 +665,7 @@ Cut cut_keys(const mmfe_attention_args* a) {
     const int want = a->dim > 64 ? 512 : 768;
     c.cuts = std::min(12, walk_cuts(a, a->q_rows, a->heads, keys, want));
     if (a->packed || a->q_rows < 1 || a->n_docs < 1) return c;
-    if (a->k_len != nullptr) c.cuts = (int)std::max<int64_t>(c.cuts, std::min<int64_t>(16, std::min(keys / 2048, 4 * want / blocks)));
+    if (a->k_len != nullptr && a->n_docs > 1 && a->q_rows <= kRows) c.cuts = (int)std::max<int64_t>(c.cuts, std::min<int64_t>(16, std::min(keys / 2048, 4 * want / blocks)));
     if (keys <= kShortKeys) return c;
     const bool whole = keys <= 512 || (keys <= 2048 && units >= 256);
     if (whole ? units >= blocks || blocks <= 512 : units > 64 && 5 * units >= 4 * blocks) return c;
