@@ -94,6 +94,7 @@ __device__ __forceinline__ float phi_of(float bound) {
     return ldexpf(1.f, 6 - e);
 }
 
+// Memory bound: 17 thousand rows of 12 heads of 64, 4 tensors' rows read: 16 us.
 // What both passes need of every row: delta and lse2 (blocks below q_blocks, 128 rows of one head each), and for float16 the tiles' largest
 // squared norms of g and, in the blocks behind, of v.  One lane has 8 elements of a row.
 template <bool BF, int DP>
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const
     store_part<DP>(a.part_v + at, dv, p.dim, back, any);
 }
 
-// Sums of the parts of one or two gradients, 4 elements a thread.
+// Sums of the parts of one or two gradients, 4 elements a thread; memory bound (17 thousand keys, 4 key heads of 64 in two parts: 15 us).
 struct Sum {
     const float* part[2];
     Rows to[2];
