@@ -72,17 +72,25 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t, or a copy of it, contiguous and on a 16-byte boundary."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _Call:
-    """One checked call: what does not depend on the outputs."""
+    """One checked call: what does not depend on its tensors.  `counts` are q_len, k_len, q_off, k_off, prefix and slopes; `strides`
+    those of q, k and v as the forward pass reads them."""
 
-    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "q_len", "k_len", "q_off", "k_off", "prefix", "slopes", "device", "q_stride", "k_stride", "v_stride", "backward_bytes")
+    __slots__ = ("packed", "causal", "n_docs", "scale", "cap", "counts", "device", "strides", "backward_bytes")
 
-    def args(self, q, k, v, out, rest, lse) -> bytes:
+    def args(self, q, k, v, out, rest, lse, counts, strides) -> bytes:
         H, n = q.shape[-2], q.shape[-3]
         return N.pack_attention(
             _ARGS_SIZE, OUT_CODES[q.dtype], self.n_docs, H, k.shape[-2], q.shape[-1], self.packed, self.causal, self.scale, self.cap, n, k.shape[-3],
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(self.q_len), _ptr(self.k_len), _ptr(self.q_off), _ptr(self.k_off), _ptr(self.prefix),
-            _ptr(self.slopes), _ptr(out), _ptr(rest), _ptr(lse), *self.q_stride, *self.k_stride, *self.v_stride, *_packed_strides(q), H * n, n)
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), *map(_ptr, counts), _ptr(out), _ptr(rest), _ptr(lse), *strides, *_packed_strides(q), H * n, n)
 
     def forward(self, q, k, v, want_lse: bool, gradients: bool = False):
         device = q.device
@@ -91,16 +99,20 @@ class _Call:
         if want_lse:
             shape = (q.shape[-2], q.shape[-3])
             lse = torch.empty(shape if self.packed else (q.shape[0],) + shape, dtype=torch.float32, device=device)
-        args = self.args(q, k, v, out, None, lse)
+        args = self.args(q, k, v, out, None, lse, self.counts, self.strides)
         if gradients:
             self.backward_bytes = N.attention_workspace(args, backward=True)
             if self.backward_bytes:            # 0: the backward pass reads neither out nor its rest
                 rest = torch.empty(q.shape, dtype=q.dtype, device=device)
-                args = self.args(q, k, v, out, rest, lse)
+                args = self.args(q, k, v, out, rest, lse, self.counts, self.strides)
         need = N.attention_workspace(args) if k.shape[-3] > 512 else 0
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         N.attention_forward(args, _ptr(work), self.device, raw_stream(self.device))
         return out, rest, lse
+
+
+def _form(tensors) -> list:
+    return [None if t is None else (t.shape, t.dtype, t.get_device(), t.stride()) for t in tensors]
 
 
 class _AttentionFn(torch.autograd.Function):
@@ -109,21 +121,35 @@ class _AttentionFn(torch.autograd.Function):
         out, rest, lse = call.forward(q, k, v, True, True)
         ctx.call = call
         # the counts too: autograd then notices when one of them has been changed before the backward pass
-        ctx.save_for_backward(q, k, v, out if call.backward_bytes else None, rest, lse, call.q_len, call.k_len, call.q_off, call.k_off, call.prefix, call.slopes)
+        saved = (q, k, v, out if call.backward_bytes else None, rest, lse, *call.counts)
+        ctx.form = _form(saved)
+        ctx.save_for_backward(*saved)
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, _):
-        q, k, v, out, rest, lse = ctx.saved_tensors[:6]
-        call = ctx.call
+        # Saved-tensor hooks (torch.autograd.graph.save_on_cpu, checkpoints) return equal values in any layout: every address below is taken
+        # from what was unpacked, and the forward pass's strides serve only where they are still the tensors' own.
+        saved, call = ctx.saved_tensors, ctx.call
+        q, k, v, out, rest, lse, *counts = saved
+        strides, form = call.strides, _form(saved)
+        if form != ctx.form:
+            for new, old in zip(form, ctx.form):
+                if (new and new[:3]) != (old and old[:3]):
+                    raise RuntimeError(f"attention: a saved-tensor hook returned {new} in place of {old} (shape, type, device, strides)")
+            lse, *counts = (None if t is None else t.contiguous() for t in (lse, *counts))
+        if form != ctx.form or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 or (out is not None and (out.data_ptr() | rest.data_ptr()) % 16):
+            (q, q_stride), (k, k_stride), (v, v_stride) = _rows(q), _rows(k), _rows(v)
+            strides = q_stride + k_stride + v_stride
+            out, rest = _dense(out), _dense(rest)
         g, g_stride = _rows(grad_out)
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         kv_stride = _packed_strides(gk)
         grads = N.pack_attention_grads(_GRADS_SIZE, 0, g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), *g_stride, *_packed_strides(gq), *kv_stride, *kv_stride)
         work = torch.empty(call.backward_bytes, dtype=torch.uint8, device=q.device) if call.backward_bytes else None
-        N.attention_backward(call.args(q, k, v, out, rest, lse), grads, _ptr(work), call.device, raw_stream(call.device))
+        N.attention_backward(call.args(q, k, v, out, rest, lse, counts, strides), grads, _ptr(work), call.device, raw_stream(call.device))
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None
 
@@ -193,25 +219,24 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
         device = q.device
     call.device = device.index
     call.packed, call.causal, call.n_docs = packed, bool(causal), m
-    call.q_len = call.k_len = call.q_off = call.k_off = None
+    q_len = k_len = q_off = k_off = None
     if packed:
-        call.q_off = _counts(offsets, "offsets", m + 1, device, n, rising=True)
-        call.k_off = call.q_off if kv_offsets is None else _counts(kv_offsets, "kv_offsets", m + 1, device, s, rising=True)
+        q_off = _counts(offsets, "offsets", m + 1, device, n, rising=True)
+        k_off = q_off if kv_offsets is None else _counts(kv_offsets, "kv_offsets", m + 1, device, s, rising=True)
     else:
-        call.q_len = _counts(lengths, "lengths", m, device, n)
-        call.k_len = call.q_len if kv_lengths is lengths and s == n else _counts(kv_lengths, "kv_lengths", m, device, s)
-    call.prefix = _counts(prefix, "prefix", m, device)
-    call.slopes = None
+        q_len = _counts(lengths, "lengths", m, device, n)
+        k_len = q_len if kv_lengths is lengths and s == n else _counts(kv_lengths, "kv_lengths", m, device, s)
+    prefix = _counts(prefix, "prefix", m, device)
     if slopes is not None:
         t = torch.as_tensor(slopes)
         if tuple(t.shape) != (H,):
             raise ValueError(f"slopes must hold one entry per query head ({H}), got {tuple(t.shape)}")
         if t.requires_grad:
             raise ValueError("slopes have no gradient: detach them")
-        call.slopes = t.to(device=device, dtype=torch.float32).contiguous()
-    q, call.q_stride = _rows(q)
-    k, call.k_stride = _rows(k)
-    v, call.v_stride = _rows(v)
+        slopes = t.to(device=device, dtype=torch.float32).contiguous()
+    call.counts = (q_len, k_len, q_off, k_off, prefix, slopes)
+    (q, q_stride), (k, k_stride), (v, v_stride) = _rows(q), _rows(k), _rows(v)
+    call.strides = q_stride + k_stride + v_stride
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _AttentionFn.apply(q, k, v, call)
     else:

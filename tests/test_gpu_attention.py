@@ -599,3 +599,51 @@ def test_cut_walks_in_graphs(mm, rows, keys, heads, kv):
             assert all(torch.equal(a, b) for a, b in zip(got, step(*s)))
         assert all(torch.equal(a, b) for a, b in zip(other, graphs[1][1]))
         torch.cuda.synchronize()
+
+
+def turned(t):
+    return t.transpose(0, -1).contiguous().transpose(0, -1)
+
+
+@pytest.mark.parametrize("B, n, s, H, K, packed", [(2, 193, 193, 4, 4, False), (2, 300, 300, 4, 2, False), (1, 1100, 1300, 2, 1, False), (2, 20, 3000, 4, 2, False),
+                                                   (1, 260, 260, 4, 2, True), (1, 1500, 1500, 2, 2, True)])
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_gradients_under_saved_tensor_hooks(mm, dtype, B, n, s, H, K, packed):
+    """Views of one packed projection whose saved tensors come back in other layouts (host copies, clones, recomputation), with counts that are
+    changed in between: the bits of the plain run."""
+    from torch.autograd.graph import save_on_cpu, saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+    fn = mm.attention.attention
+    gen = torch.Generator().manual_seed(n + s)
+    room = max(n, s)
+    qkv = torch.randn(B, room, H + 2 * K, 64, generator=gen).to(dtype).cuda()
+    q, k, v = qkv[:, :n, :H], qkv[:, :s, H:H + K], qkv[:, :s, H + K:]
+    g = torch.randn(B, n, H, 64, generator=gen).to(dtype).cuda()
+    if packed:
+        q, k, v, g = q[0], k[0], v[0], g[0]
+        cuts = [0, n // 3, n - 5]
+    else:
+        cuts = [n] * B
+        cuts[-1] = n - 7
+
+    def run(counts, prefix, hooks=None, again=False):
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        call = lambda *x: fn(*x, causal=True, prefix=prefix, **(dict(offsets=counts) if packed else dict(lengths=counts)))
+        if hooks is None:
+            o = checkpoint(call, *x, use_reentrant=False) if again else call(*x)
+        else:
+            with hooks:
+                o = call(*x)
+            counts.fill_(0)
+            prefix.fill_(0)
+        return (o.detach(),) + torch.autograd.grad(o, x, g)
+
+    def fresh():
+        return torch.tensor(cuts, dtype=torch.int32, device="cuda"), torch.tensor([3] * (2 if packed else B), dtype=torch.int32, device="cuda")
+    want = run(*fresh())
+    keep = lambda t: t.detach().clone(memory_format=torch.preserve_format)
+    for hooks in (save_on_cpu(pin_memory=True), save_on_cpu(), saved_tensors_hooks(keep, lambda t: t.contiguous().clone()), saved_tensors_hooks(keep, turned),
+                  saved_tensors_hooks(keep, lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t))):
+        got = run(*fresh(), hooks)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(run(*fresh(), again=True), want))

@@ -241,3 +241,75 @@ def test_folded_views():
     x = torch.zeros(2, 5, 12, 8)
     assert not any(map(_folded, (x, x[:, :, 2:5], x[:, ::2], x.transpose(1, 2), x[:0], x[:, :1], x[..., :3])))
     assert _folded(x[:, :1].expand(2, 5, 12, 8)) and _folded(x.view(-1).as_strided((1, 9, 2, 8), (0, 8, 8, 1)))
+
+
+# What a saved-tensor hook may make of a tensor: equal values in another layout.
+RELAID = {
+    "same": lambda t: t,
+    "packed": lambda t: torch.empty(t.size(), dtype=t.dtype).copy_(t),                     # what offloading to the host does
+    "clone": lambda t: t.clone(),
+    "gaps": lambda t: torch.empty(t.shape[:-1] + (t.shape[-1] + 8,), dtype=t.dtype)[..., :t.shape[-1]].copy_(t),
+    "turned": lambda t: t.transpose(0, -1).contiguous().transpose(0, -1),                  # no unit stride inside the heads
+}
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("kv", [2, 4])
+@pytest.mark.parametrize("relay", RELAID)
+def test_attention_backward_addresses_what_was_unpacked(N, monkeypatch, relay, kv, packed):
+    """Pointers and strides of the backward call belong together, whatever layout a saved-tensor hook returns; counts are the saved ones."""
+    from multi_modal_amd import attention as A
+    seen, calls = {}, []
+
+    def unpack(t):
+        t = RELAID[relay](t)
+        seen[t.data_ptr()] = t
+        return t
+    monkeypatch.setattr(A, "require_gpu", lambda: None)
+    monkeypatch.setattr(A, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda self: self)
+    monkeypatch.setattr(A.N, "attention_forward", lambda args, work, device, stream: None)
+    monkeypatch.setattr(A.N, "attention_backward", lambda args, grads, work, device, stream: calls.append(
+        (N.AttentionArgs.from_buffer_copy(args), N.AttentionGrads.from_buffer_copy(grads))))
+    qkv = torch.zeros(2, 300, 3, 4, 64, dtype=torch.float16)
+    q, k, v = (t.detach() for t in qkv.unbind(2))
+    k, v = k[:, :, :kv], v[:, :, :kv]
+    counts = torch.tensor([0, 100, 290] if packed else [300, 20], dtype=torch.int32)
+    if packed:
+        q, k, v = q[0], k[0], v[0]
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    prefix = torch.tensor([3, 4], dtype=torch.int32)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.preserve_format) if t.dtype == torch.int32 else t.detach(), unpack):
+        out = A.attention(q, k, v, causal=True, prefix=prefix, **(dict(offsets=counts) if packed else dict(lengths=counts)))
+    prefix.fill_(7)                                    # after the forward pass: a hook has its copy, and autograd notices nothing
+    torch.autograd.grad(out, [q, k, v], torch.zeros_like(out))
+    (args, grads), = calls
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        at, strides = getattr(args, name), tuple(getattr(args, name + "_stride"))
+        if relay == "turned":                          # the kernels cannot read it where it is
+            assert at not in seen and strides == A._packed_strides(t), (name, strides)
+        else:
+            assert seen[at].shape == t.shape and strides == A._rows(seen[at])[1], (name, strides, seen[at].stride())
+    dense = A._packed_strides(q)
+    assert tuple(args.out_stride) == dense
+    for at, of in ((args.out, q.shape), (args.out_rest, q.shape), (args.lse, (4, 300) if packed else (2, 4, 300))):
+        assert not at or at not in seen or (seen[at].shape == torch.Size(of) and seen[at].is_contiguous())
+    for at, want in ((args.prefix, [3, 4]), (args.q_off if packed else args.q_len, counts.tolist())):
+        assert (ctypes.c_int32 * len(want)).from_address(at)[:] == want
+
+
+def test_attention_backward_refuses_other_tensors(N, monkeypatch):
+    """A hook that returns another shape or type than it was given would make the kernels read past it."""
+    from multi_modal_amd import attention as A
+    monkeypatch.setattr(A, "require_gpu", lambda: None)
+    monkeypatch.setattr(A, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda self: self)
+    monkeypatch.setattr(A.N, "attention_forward", lambda *a: None)
+    monkeypatch.setattr(A.N, "attention_backward", lambda *a: pytest.fail("launched"))
+    for change in (lambda t: t.float() if t.dtype == torch.float16 else t, lambda t: t[:1] if t.dim() == 4 else t, lambda t: t[..., :1] if t.dtype == torch.float32 else t,
+                   lambda t: t[:1] if t.dtype == torch.int32 else t, lambda t: t.long() if t.dtype == torch.int32 else t):
+        q = torch.zeros(2, 300, 4, 64, dtype=torch.float16, requires_grad=True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), change):
+            out = A.attention(q, q, q, lengths=torch.tensor([5, 300], dtype=torch.int32))
+        with pytest.raises(RuntimeError, match="saved-tensor hook"):
+            torch.autograd.grad(out, [q], torch.zeros_like(out))
