@@ -50,23 +50,26 @@ struct ForwardArgs {
     float2* part_ml;
 };
 
-// How scores leave the linear form (bits); anything but kPlain takes them to log2 units before the maximum.
-enum { kPlain = 0, kBias = 1, kCap = 2 };
+// How scores leave the linear form (bits); kBias and kCap take them to log2 units before the maximum.  kCap is kExpCap's form, kWide kAnyCap's.
+enum { kPlain = 0, kBias = 1, kCap = 2, kWide = 4 };
 
 template <int SHAPE>
 struct Shape {
     float c, slope, cap_in, cap_out;
+    AnyCap any;
     __device__ __forceinline__ Shape(const Problem& p, int head) {
         c = p.scale * kLog2e;
         slope = SHAPE & kBias ? __uint_as_float(uniform(__float_as_uint(p.slopes[head] * kLog2e))) : 0.f;
         cap_in = SHAPE & kCap ? 2.f * kLog2e * p.scale / p.cap : 0.f;
         cap_out = SHAPE & kCap ? 2.f * p.cap * kLog2e : 0.f;
+        if constexpr (SHAPE & kWide) any.set(p);
     }
     // x: products of 32 keys; at: distance from the lane's row back to its first key (row + off - j0 - 4 * half); side 1: all keys stand at
     // or before all rows of the wave, -1: all behind them, 0: some of each.  Returns what the scores lack: on one side, -slope * |at - r|
     // is a number of the row's plus a number that all lanes share, and only the shared one is added here (one instruction a score, not three).
     // A capped score is cap tanh(z) = cap - 2 cap / (e^(2 z) + 1).
     __device__ __forceinline__ float apply(f32x16& x, float at, int side) const {
+        if constexpr (SHAPE & kWide) any.apply<false>(x, nullptr);
         if constexpr (SHAPE & kCap)
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = fmaf(-cap_out, __builtin_amdgcn_rcpf(exp2_fast(x[i] * cap_in) + 1.f), 0.5f * cap_out);
@@ -90,7 +93,7 @@ struct Shape {
         return 0.f;
     }
     // factor from the units the maximum is kept in to log2 units
-    __device__ __forceinline__ float unit() const { return SHAPE == kPlain ? c : 1.f; }
+    __device__ __forceinline__ float unit() const { return SHAPE & (kBias | kCap) ? 1.f : c; }
 };
 
 // Softmax state of a lane's row, and what 32 keys do to it.
@@ -462,10 +465,10 @@ __global__ void __launch_bounds__(64 * kSplitWaves, 1) split_kernel(const SplitA
             if (ok && 16 * s + 8 * half < p.dim) qf[s] = *reinterpret_cast<const u32x4*>(q + 32 * s + 16 * half);
         }
     }
-    const bool shaped = p.cap > 0.f || p.slopes != nullptr;
-    const float c = shaped ? 1.f : p.scale * kLog2e;
+    const float c = p.slopes ? 1.f : p.scale * kLog2e;
     const float slope = p.slopes && col < n_rows ? p.slopes[mine.head] * kLog2e : 0.f;
-    const float cap_in = p.cap > 0.f ? p.scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
+    AnyCap cap{};
+    if (p.cap > 0.f) cap.set(p);
     if (wave < n_tiles) stage(wave, 0);
 
     f32x16 o[DP / 32];
@@ -487,14 +490,11 @@ __global__ void __launch_bounds__(64 * kSplitWaves, 1) split_kernel(const SplitA
         f32x16 x{};
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) x = mfma<BF>(read_rows<DP>(kt, 0, s), qf[s], x);
-        if (shaped) {
+        if (p.cap > 0.f) cap.apply<false>(x, nullptr);
+        if (p.slopes) {
             const float at = (float)(mine.token + off - j0 - 4 * half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float v = p.cap > 0.f ? cap_out * tanh_fast(x[i] * cap_in) : x[i] * (p.scale * kLog2e);
-                if (p.slopes) v -= slope * fabsf(at - (float)reg_row(i));
-                x[i] = v;
-            }
+            for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], p.scale * kLog2e, -slope * fabsf(at - (float)reg_row(i)));
         }
         if (j0 + kSplitTile > full_lim || j0 + kSplitTile > s1) {
             const int left = min(lim, s1) - j0 - 4 * half;
@@ -630,9 +630,10 @@ forward_fn pick_dim(int dim) {
     return dim <= 32 ? &forward_kernel<BF, 32, SHAPE, CUT> : dim <= 64 ? &forward_kernel<BF, 64, SHAPE, CUT> : dim <= 96 ? &forward_kernel<BF, 96, SHAPE, CUT> : &forward_kernel<BF, 128, SHAPE, CUT>;
 }
 template <bool BF, bool CUT>
-forward_fn pick_forward(int dim, bool bias, bool cap) {
-    if (bias) return cap ? pick_dim<BF, kBias | kCap, CUT>(dim) : pick_dim<BF, kBias, CUT>(dim);
-    return cap ? pick_dim<BF, kCap, CUT>(dim) : pick_dim<BF, kPlain, CUT>(dim);
+forward_fn pick_forward(int dim, bool bias, float cap) {
+    if (cap > kUsualCap) return bias ? pick_dim<BF, kBias | kWide, CUT>(dim) : pick_dim<BF, kWide, CUT>(dim);
+    if (bias) return cap > 0.f ? pick_dim<BF, kBias | kCap, CUT>(dim) : pick_dim<BF, kBias, CUT>(dim);
+    return cap > 0.f ? pick_dim<BF, kCap, CUT>(dim) : pick_dim<BF, kPlain, CUT>(dim);
 }
 template <bool BF>
 split_fn pick_split(int dim) {
@@ -813,9 +814,9 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
         if (c.n_splits > 1) hipLaunchKernelGGL(bf ? &join_kernel<true> : &join_kernel<false>, dim3((uint32_t)(c.units * 32)), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(hip_stream), s);
         return launched("attention");
     }
-    const bool bias = a->slopes != nullptr, cap = a->cap > 0.f;
-    const forward_fn fn = c.cuts > 1 ? (bf ? pick_forward<true, true>(a->dim, bias, cap) : pick_forward<false, true>(a->dim, bias, cap))
-                                     : (bf ? pick_forward<true, false>(a->dim, bias, cap) : pick_forward<false, false>(a->dim, bias, cap));
+    const bool bias = a->slopes != nullptr;
+    const forward_fn fn = c.cuts > 1 ? (bf ? pick_forward<true, true>(a->dim, bias, a->cap) : pick_forward<false, true>(a->dim, bias, a->cap))
+                                     : (bf ? pick_forward<true, false>(a->dim, bias, a->cap) : pick_forward<false, false>(a->dim, bias, a->cap));
     const size_t lds = 2 * (size_t)kRing * kStepKeys * pitch(a->dim) * 2;
     int blocks = 1, cus = 256;
     rc = kernel_prepare(reinterpret_cast<const void*>(fn), kThreads, lds, &blocks, &cus);

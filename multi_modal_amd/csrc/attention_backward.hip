@@ -80,9 +80,11 @@ __device__ __forceinline__ u32x2 thirds(float v) {
     return u32x2{(a & 0xffffu) | b << 16, c & 0xffffu};
 }
 
+// What a score's form lacks to log2 p beside the row's lse (see Shape).
+__device__ __forceinline__ float lacks(const Problem& p) { return p.cap > 0.f && p.cap <= kUsualCap ? p.cap * kLog2e : 0.f; }
 // What keys_kernel adds to a row's products: in log2 units beside a capped score, in the products' own otherwise.  -1e30: p = 0
 __device__ __forceinline__ float row_add(const Problem& p, float lse2) {
-    const float add = p.cap > 0.f ? p.cap * kLog2e - lse2 : -lse2 / (p.scale * kLog2e);
+    const float add = p.cap > 0.f ? lacks(p) - lse2 : -lse2 / (p.scale * kLog2e);
     return add < -1e30f ? -1e30f : add;                // a NaN stays one
 }
 
@@ -188,30 +190,33 @@ __device__ __forceinline__ float find_phi(const BackwardArgs& a, const Doc& d, i
     }
 }
 
-// Scores in log2 units from the products, and the factor that a capped score's gradient has.  A capped score is
+// Scores in log2 units from the products, and the factor that a capped score's gradient has.  In kExpCap's form a score is
 // cap tanh(z) = cap (1 - 2 r) with r = 1 / (e^(2 z) + 1), and 1 - tanh^2 = 4 (r - r^2): one exponential and one reciprocal; the 4
 // is left to the gradients' final factor.
-template <bool CAP>
+template <int CAP>
 struct Shape {
     bool bias;
     float c, slope, cap_in, cap_out;
+    AnyCap any;
     __device__ __forceinline__ void set(const Problem& p, int head) {
         bias = p.slopes != nullptr;
         c = p.scale * kLog2e;
         slope = bias ? p.slopes[head] * kLog2e : 0.f;
-        cap_in = CAP ? 2.f * kLog2e * p.scale / p.cap : 0.f;
-        cap_out = 2.f * p.cap * kLog2e;
+        cap_in = CAP == kExpCap ? 2.f * kLog2e * p.scale / p.cap : 0.f;
+        cap_out = CAP == kExpCap ? 2.f * p.cap * kLog2e : 0.f;
+        if constexpr (CAP == kAnyCap) any.set(p);
     }
     // x -> score + add, w -> the factor.  at: distance of register row 0, step: its sign per row.  FOLDED: the products hold `add` already
     template <bool FOLDED, typename ADD>
     __device__ __forceinline__ void apply(f32x16& x, f32x16& w, ADD add, float at, float step) const {
+        if constexpr (CAP == kAnyCap) any.apply<true>(x, &w);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            if constexpr (CAP) {
+            if constexpr (CAP == kExpCap) {
                 const float r = __builtin_amdgcn_rcpf(exp2_fast(x[i] * cap_in) + 1.f);
                 x[i] = fmaf(-cap_out, r, add(i));
                 w[i] = fmaf(-r, r, r);
-            } else if constexpr (FOLDED) x[i] *= c;
+            } else if constexpr (FOLDED && !CAP) x[i] *= c;
             else x[i] = fmaf(x[i], c, add(i));
         }
         if (bias) {
@@ -295,7 +300,7 @@ constexpr int kStatBytes = 64 * 16;                    // of a tile's row statis
 // Head size 128 has one wave per SIMD (357 registers), 64 and less two.  At 96, with half the tile and without the overlap, two blocks fit a CU, and one's
 // products run beside the other's exponentials: 8192 rows, 12 heads on 4, 987 -> 636 us, causal 518 -> 337 (4096 rows, 12 heads of 72: 356 -> 209).
 // The same at 128 leaves 41 registers in memory: 744 -> 673 us for 8 heads of 8192 rows, but causal 403 -> 413 with the walks cut and 636 without.
-template <bool BF, int DP, bool CAP>
+template <bool BF, int DP, int CAP>
 __global__ void __launch_bounds__(kThreads, DP == 128 ? 1 : 2) keys_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [q tile][g tile][row statistics]
     const Problem& p = a.p;
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const Sum a) {
 // dq of 128 rows, 32 per wave, over tiles of 32 keys; steps overlap as in keys_kernel.  Head size 64 is held to 168 registers for three waves
 // a SIMD (6 of them spilled): 8192 rows, 12 heads, 840 -> 954 TFLOP/s without a mask, 871 -> 830 under a causal one.
 // CUT: the walk is cut into parts (as an argument that any call could have, 4 to 25 % slower where it is not).
-template <bool BF, int DP, bool CAP, bool CUT>
+template <bool BF, int DP, int CAP, bool CUT>
 __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const BackwardArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // kRing x [k tile][v tile]
     const Problem& p = a.p;
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
     load_rows<DP>(gf, row_base(a.g, d, d.q0 + r, head), p.dim, nq > 0);
     const int64_t at = d.batch * a.lse_b + head * a.lse_h + d.q0 + r;
     const float phi = find_phi<BF>(a, d, kvh, reinterpret_cast<float*>(smem));
-    float add = nq > 0 ? (CAP ? p.cap * kLog2e : 0.f) - a.lse2[at] : 0.f;       // what the scores' log2 form lacks to log2 p
+    float add = nq > 0 ? lacks(p) - a.lse2[at] : 0.f;                         // what the scores' log2 form lacks to log2 p
     float delta = nq > 0 ? -a.delta[at] * phi : 0.f;
     Shape<CAP> sh;
     sh.set(p, head);
@@ -590,7 +595,7 @@ constexpr int kWholeRows = 256;
 template <int DP, int WAVES>
 constexpr int kWholeLoad = WAVES * 512 / DP;           // rows that one DMA of each wave brings
 
-template <bool BF, int DP, bool CAP, int WAVES>
+template <bool BF, int DP, int CAP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) whole_kernel(const BackwardArgs a, int padded_rows) {
     extern __shared__ __attribute__((aligned(16))) char smem[];       // k, v, q, g of padded_rows rows each, statistics of the rows, WAVES floats
     const Problem& p = a.p;
@@ -675,7 +680,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) whole_kernel(const BackwardArgs
     if (w0 < p.q_rows) {
         const int lim = any && mine < nq ? limit(mine) : 0, wave_lim = any && w0 < nq ? limit(w0 + 31) : 0, full_lim = any && w0 < nq ? limit(w0) : 0;
         const float l2 = lse == -INFINITY ? INFINITY : lse * kLog2e - kShift<BF>;
-        const float add = (CAP ? p.cap * kLog2e : 0.f) - l2;
+        const float add = lacks(p) - l2;
         f32x16 dq[DP / 32];
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) dq[e] = f32x16{};
@@ -775,7 +780,7 @@ void launch_sum(const Sum& s, hipStream_t stream) {
     hipLaunchKernelGGL(sum_kernel<BF>, dim3((uint32_t)(need < 8192 ? need : 8192)), dim3(kThreads), 0, stream, s);
 }
 
-template <bool BF, int DP, bool CAP, int WAVES>
+template <bool BF, int DP, int CAP, int WAVES>
 int launch_whole(BackwardArgs& b, hipStream_t stream) {
     Problem& p = b.p;
     constexpr int kLoad = kWholeLoad<DP, WAVES>;
@@ -789,7 +794,7 @@ int launch_whole(BackwardArgs& b, hipStream_t stream) {
     return launched("attention backward");
 }
 
-template <bool BF, int DP, bool CAP>
+template <bool BF, int DP, int CAP>
 int launch(BackwardArgs& b, hipStream_t stream) {
     Problem& p = b.p;
     int rc = MMFE_OK, blocks = 1, cus = 256;
@@ -827,10 +832,15 @@ int launch(BackwardArgs& b, hipStream_t stream) {
     return launched("attention backward");
 }
 
-template <bool BF, bool CAP>
+template <bool BF, int CAP>
 int launch_dim(BackwardArgs& b, hipStream_t stream) {
     const int dp = padded_dim(b.p.dim);
     return dp == 32 ? launch<BF, 32, CAP>(b, stream) : dp == 64 ? launch<BF, 64, CAP>(b, stream) : dp == 96 ? launch<BF, 96, CAP>(b, stream) : launch<BF, 128, CAP>(b, stream);
+}
+
+template <bool BF>
+int launch_cap(BackwardArgs& b, hipStream_t stream) {
+    return b.p.cap > kUsualCap ? launch_dim<BF, kAnyCap>(b, stream) : b.p.cap > 0.f ? launch_dim<BF, kExpCap>(b, stream) : launch_dim<BF, kUncapped>(b, stream);
 }
 
 // places of the norms' tiles (see slot)
@@ -900,9 +910,7 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     OnDevice on(device);
     if (on.rc) return on.rc;
     hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
-    const bool cap = a->cap > 0.f;
-    if (a->dtype == MMFE_OUT_BF16) return cap ? launch_dim<true, true>(b, stream) : launch_dim<true, false>(b, stream);
-    return cap ? launch_dim<false, true>(b, stream) : launch_dim<false, false>(b, stream);
+    return a->dtype == MMFE_OUT_BF16 ? launch_cap<true>(b, stream) : launch_cap<false>(b, stream);
 }
 
 }  // extern "C"

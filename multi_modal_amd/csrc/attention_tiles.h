@@ -378,8 +378,57 @@ __device__ __forceinline__ void store4(char* to, char* rest, float a, float b, f
         *reinterpret_cast<u32x2*>(rest) = u32x2{pack2<BF>(a - widen<BF>(w.x, 0), b - widen<BF>(w.x, 1)), pack2<BF>(c - widen<BF>(w.y, 0), d - widen<BF>(w.y, 1))};
 }
 
-// tanh(z) from one exponential: 1 - 2 / (e^(2 z) + 1); absolute error a few 2^-24, exact limits
-__device__ __forceinline__ float tanh_fast(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_fast(2.f * kLog2e * z) + 1.f); }
+// tanh(z) / z for |z| <= 1/2, u = (z / 2)^2: minimax in z^2 with the constant term held at 1 (fitted in float64), off by 2^-26 relative; the coefficients hold
+// the powers of 4.
+__device__ __forceinline__ float tanh_ratio(float u) {
+    return fmaf(fmaf(fmaf(fmaf(0.01724148727953434f * 256.f, u, -0.05304549261927605f * 64.f), u, 0.13325878977775574f * 16.f), u, -0.333331435918808f * 4.f), u, 1.f);
+}
+
+// How scores are capped (0: not).  1 - 2 / (e^(2 z) + 1) takes an exponential and a reciprocal, and its error is that of a number of size cap: 1.2e-7 cap,
+// which up to kUsualCap stays below what the float32 products behind scores of that size are off by.  Any other cap takes kAnyCap, whose error is relative to the
+// score (the exponential's form: 1.2e-3 at 1e4, 0.09 at 1e6).  It is a kernel of its own because it branches, which parts the products from the vector
+// instructions beside them: 2 x 4096 rows, 12 heads on 4 of 64, bfloat16, causal, forward and backward 162 + 353 us, 130 + 345 with the exponential.  (split_kernel,
+// which waits for memory, has kAnyCap only: 16 streams of 20 000 keys, 16 heads on 4 of 128: 136 us, 144 with the exponential.)
+enum { kUncapped = 0, kExpCap = 1, kAnyCap = 2 };
+constexpr float kUsualCap = 64.f;
+
+// kAnyCap: the products x become those that an uncapped score of the same value has, cap / scale tanh(z) with z = scale x / cap.
+// For |z| <= 1/2 that is x tanh(z) / z; beyond, cap / scale (1 - 2 r) with r = 1 / (e^(2 z) + 1), where the score is at least 0.46 cap.  Where all of a wave's
+// 1024 products are of the first kind neither exponential nor reciprocal is taken.
+struct AnyCap {
+    float half, twice, most;          // scale / (2 cap), 2 log2(e) scale / cap, cap / scale
+    __device__ __forceinline__ void set(const Problem& p) {
+        half = 0.5f * p.scale / p.cap;
+        twice = 2.f * kLog2e * p.scale / p.cap;
+        most = fminf(p.cap / p.scale, 0.25f * __FLT_MAX__);
+    }
+    // w (WEIGHTS): (1 - tanh^2 z) / 4, which is r - r^2
+    template <bool WEIGHTS>
+    __device__ __forceinline__ void apply(f32x16& x, f32x16* w) const {
+        float m = 0.f, k = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(x[i])), fabsf(x[i + 1]));
+            k = __builtin_elementwise_maximum(__builtin_elementwise_maximum(k, fabsf(x[i + 2])), fabsf(x[i + 3]));
+        }
+        if (__all(__builtin_elementwise_maximum(m, k) * half <= 0.25f)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float h = x[i] * half, t = tanh_ratio(h * h);
+                if constexpr (WEIGHTS) (*w)[i] = fmaf(-(h * t), h * t, 0.25f);
+                x[i] *= t;
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float h = x[i] * half, t = tanh_ratio(h * h), r = __builtin_amdgcn_rcpf(exp2_fast(x[i] * twice) + 1.f);
+            const bool small = fabsf(h) <= 0.25f;
+            if constexpr (WEIGHTS) (*w)[i] = small ? fmaf(-(h * t), h * t, 0.25f) : fmaf(-r, r, r);
+            x[i] = small ? x[i] * t : fmaf(-2.f * most, r, most);
+        }
+    }
+};
 
 // Row i of the result registers (see above).
 __device__ __forceinline__ constexpr int reg_row(int i) { return 8 * (i >> 2) + (i & 3); }

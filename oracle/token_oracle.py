@@ -4,9 +4,14 @@ import math
 import torch
 
 
-def attention_head(q, k, v, scale, cap=0.0, slope=0.0, causal=False, prefix=0, g=None):
+def attention_head(q, k, v, scale, cap=0.0, slope=0.0, causal=False, prefix=0, g=None, relative=False):
     """One head of one document: q (n, D), k and v (m, D), all float64.  Returns a dict with o, lse, and with g the gradients dq, dk, dv
-    by their formulas; next to each result what its tolerance is made of (see attention_tolerances)."""
+    by their formulas; next to each result what its tolerance is made of (see attention_tolerances).
+
+    relative: a capped score's error is bounded by the score and not by the cap.  With z = s / cap and steps of u = 2^-24: up to |z| = 1/2 the series in z^2 and its
+    products are off by at most 1 step for z, 2 for the square (which count z^2 / 3 times at most), 1 for each of 3 products; beyond, 1 - 2 / (e^(2 z) + 1) has the
+    exponential's 2 steps and its argument's 2 |z|, taken by r (1 - r) <= 1/4, the reciprocal's 2 and the sum's 1, taken by r <= 1, twice, and 1 of the result:
+    2 (1/4 (2 + 2 |z|) + 3) + 1, where |z| r (1 - r) <= 0.23, is at most 9 steps of cap, and |s| >= 0.46 cap: 20 steps of |s| hold both."""
     n, m = q.shape[0], k.shape[0]
     raw = scale * (q @ k.T)
     t = torch.tanh(raw / cap) if cap else None
@@ -27,7 +32,8 @@ def attention_head(q, k, v, scale, cap=0.0, slope=0.0, causal=False, prefix=0, g
     # rounding errors of a score in float32: the products' sum, the multiplications behind it, tanh, the distance
     D = q.shape[1]
     u = 2.0 ** -24
-    es = u * ((D + 4) * scale * (q.abs() @ k.T.abs()) + 4 * torch.where(see, s.abs(), torch.zeros_like(s)) + 16 * cap)
+    capped = (cap * t).abs() if cap else 0.0
+    es = u * ((D + 4) * scale * (q.abs() @ k.T.abs()) + 4 * torch.where(see, s.abs(), torch.zeros_like(s)) + (20 * capped if relative else 16 * cap))
     es = torch.where(see, es, torch.zeros_like(es))
     es = es + (es.amax(1, keepdim=True) if m else 0.0)              # of the score, and of the row's normaliser
     r["p"], r["es"], r["see"] = p, es, see
@@ -71,7 +77,7 @@ def attention_tolerances(r, q, k, v, g, scale, eps, tiny):
     return tol
 
 
-def attention(q, k, v, docs, scale=None, cap=0.0, slopes=None, causal=False, prefix=None, g=None, eps=0.0, tiny=0.0):
+def attention(q, k, v, docs, scale=None, cap=0.0, slopes=None, causal=False, prefix=None, g=None, eps=0.0, tiny=0.0, relative=False):
     """q (T, H, D), k and v (S, K, D); docs: (first row, rows, first key, keys) of each document.  Returns ({o, lse, dq, dk, dv}, the same of
     tolerances), zeros (lse -inf) in rows that no document holds."""
     T, H, D = q.shape
@@ -89,7 +95,7 @@ def attention(q, k, v, docs, scale=None, cap=0.0, slopes=None, causal=False, pre
             c = h // (H // K)
             a = (q[q0:q0 + n, h].double(), k[k0:k0 + m, c].double(), v[k0:k0 + m, c].double())
             gg = None if g is None else g[q0:q0 + n, h].double()
-            r = attention_head(*a, scale, cap, 0.0 if slopes is None else float(slopes[h]), causal, 0 if prefix is None else int(prefix[d]), gg)
+            r = attention_head(*a, scale, cap, 0.0 if slopes is None else float(slopes[h]), causal, 0 if prefix is None else int(prefix[d]), gg, relative)
             t = attention_tolerances(r, *a, gg, scale, eps, tiny)
             z["o"][q0:q0 + n, h], w["o"][q0:q0 + n, h] = r["o"], t["o"]
             z["lse"][h, q0:q0 + n] = r["lse"]

@@ -647,3 +647,39 @@ def test_gradients_under_saved_tensor_hooks(mm, dtype, B, n, s, H, K, packed):
         got = run(*fresh(), hooks)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(torch.equal(a, b) for a, b in zip(run(*fresh(), again=True), want))
+
+
+CAPPED = [
+    # as PADDED: one block a head, two passes, cut walks, chunks of keys, every head size
+    ([193, 30], 193, None, 193, 2, 2, 64, HF, False, False, False),
+    ([100], 100, None, 100, 2, 2, 32, BF, True, False, True),
+    ([300, 31], 300, None, 300, 4, 2, 64, BF, True, True, False),
+    ([260], 260, None, 260, 2, 1, 128, HF, True, False, True),
+    ([1100], 1100, None, 1100, 1, 1, 72, HF, False, False, False),
+    ([1, 1], 1, [4000, 700], 4000, 4, 1, 64, HF, True, False, False),
+    ([3], 3, [3000], 3000, 4, 2, 128, BF, True, False, True),
+]
+
+
+@pytest.mark.parametrize("cap, size", [(5.0, 4.0), (50.0, 20.0), (50.0, 1.0), (1e3, 1.0), (1e4, 1.0), (1e4, 60.0), (1e6, 1.0), (1e30, 1.0), (3e38, 1.0)])
+@pytest.mark.parametrize("case", CAPPED, ids=lambda c: f"{c[0]}x{c[3]}x{c[6]}")
+def test_capped_scores_of_any_cap(mm, O, case, cap, size):
+    """The error of a capped score is bounded by the score, however large the cap; scores of a few units (size 1) and across half the cap."""
+    class Relative:
+        attention = staticmethod(lambda *a, **k: O.attention(*a, relative=True, **k))
+    lens, N, kv, S, H, K, D, dtype, causal, prefix, bias = case
+    B = len(lens)
+    gen = torch.Generator().manual_seed(N + S + D)
+    q = (size * torch.randn(B, N, H, D, generator=gen)).to(dtype).cuda()
+    k, v = (torch.randn(B, S, K, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    g = torch.randn(B, N, H, D, generator=gen).to(dtype).cuda()
+    m = kv or lens
+    host, opts = {}, dict(causal=causal, cap=cap, lengths=lens, kv_lengths=m)
+    if prefix:
+        host["prefix"] = opts["prefix"] = [x // 2 for x in m]
+    if bias:
+        host["slopes"] = opts["slopes"] = slopes_of(H)
+    for b in range(B):
+        for t, n in ((q, lens[b]), (g, lens[b]), (k, m[b]), (v, m[b])):
+            t[b, n:] = math.nan
+    check(mm, Relative, q, k, v, docs_padded(lens, m, N, S), opts, g=g, flat=flat4, lse_flat=lse4, host=host)
