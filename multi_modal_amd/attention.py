@@ -14,7 +14,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, once_differentiable, raw_stream, require_gpu
+from .plans import OUT_CODES, once_differentiable, raw_stream, refuse_forward_mode, require_gpu
 
 _ARGS_SIZE = ctypes.sizeof(N.AttentionArgs)
 _GRADS_SIZE = ctypes.sizeof(N.AttentionGrads)
@@ -172,7 +172,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
 
     `lengths`, `offsets` and `prefix` may be integer tensors on the GPU (not read back; entries out of range are clamped) or on the
     host (checked).  return_lse=True also returns the float32 log-sum-exp of each row's scores, (B, H, N) or (H, T), without gradient.
-    Tensors on the CPU are copied over and the result is copied back."""
+    Second derivatives and forward-mode derivatives are refused.  Tensors on the CPU are copied over and the result is copied back."""
     dtype = q.dtype
     if dtype not in _DTYPES or k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"attention takes float16 or bfloat16 tensors of one type, got {q.dtype}, {k.dtype}, {v.dtype}")
@@ -213,6 +213,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
         m = qs[0]
         if kv_lengths is None and s == n:
             kv_lengths = lengths
+    refuse_forward_mode("attention", q, k, v)
     if not q.is_cuda:
         require_gpu()
         q, k, v = q.cuda(), k.cuda(), v.cuda()

@@ -11,6 +11,7 @@ from collections import OrderedDict
 from typing import Callable, Dict, Hashable, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable as _once_differentiable
 
 from . import _native as N
@@ -54,12 +55,19 @@ def mark_written(tensors) -> None:
         torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
+def refuse_forward_mode(what: str, *tensors) -> None:
+    """A dual tensor (torch.autograd.forward_ad) does not say requires_grad; a kernel would read its value and drop its tangent."""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def once_differentiable(backward):
     """torch.autograd.function.once_differentiable where a second derivative is being recorded; the plain function, which takes 10 us
     less, where none is."""
     recorded = _once_differentiable(backward)
 
     def run(ctx, *grads):
+        refuse_forward_mode("this gradient", *grads)
         return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 

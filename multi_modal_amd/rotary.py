@@ -16,7 +16,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, mark_written, once_differentiable, raw_stream, require_gpu
+from .plans import OUT_CODES, mark_written, once_differentiable, raw_stream, refuse_forward_mode, require_gpu
 
 _ARGS_SIZE = ctypes.sizeof(N.RotaryArgs)
 
@@ -60,7 +60,7 @@ class Rotary:
         """q: (B, N, H, D); k: (B, N, K, D) of the same type, or None; float32, float16 or bfloat16, any strides (views of a packed
         projection are read where they are).  positions: (axes, N), the same for every batch entry, or (axes, B, N); integers of any
         sign and size.  Returns new contiguous tensors (q', k'), or q' alone when k is None; float32 arithmetic, rounded once, angles
-        in float64.  Differentiable in q and k.
+        in float64.  Differentiable in q and k (once, in reverse mode).
         inplace=True writes the result over q and k (no gradients; the two must not share elements) and returns them.
         Tensors on the CPU are copied over and the results copied back."""
         origin = q.device
@@ -83,6 +83,7 @@ class Rotary:
         if tuple(positions.shape) not in ((A, n), (A, B, n)):
             raise ValueError(f"positions must be ({A}, {n}) or ({A}, {B}, {n}), got {tuple(positions.shape)}")
         given = (q,) if k is None else (q, k)
+        refuse_forward_mode("Rotary", *given)
         if inplace:
             if torch.is_grad_enabled() and any(t.requires_grad for t in given):
                 raise RuntimeError("inplace=True has no gradient: use it under torch.no_grad()")

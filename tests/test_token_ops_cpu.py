@@ -313,3 +313,33 @@ def test_attention_backward_refuses_other_tensors(N, monkeypatch):
             out = A.attention(q, q, q, lengths=torch.tensor([5, 300], dtype=torch.int32))
         with pytest.raises(RuntimeError, match="saved-tensor hook"):
             torch.autograd.grad(out, [q], torch.zeros_like(out))
+
+
+def test_forward_mode_is_refused(N, monkeypatch):
+    """A dual tensor's tangent must not be dropped in silence."""
+    import torch.autograd.forward_ad as fwd
+    from multi_modal_amd import attention as A, rotary as R
+    for m in (A, R):
+        monkeypatch.setattr(m, "require_gpu", lambda: None)
+        monkeypatch.setattr(m, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda self, *a: self)
+    monkeypatch.setattr(A.N, "attention_forward", lambda *a: None)
+    monkeypatch.setattr(R.N, "RotaryHandle", lambda *a: type("H", (), {"run": lambda *a: None, "close": lambda self: None})())
+    q, pos = torch.zeros(1, 3, 2, 8, dtype=torch.float16), torch.zeros(1, 3, dtype=torch.int32)
+    rot = R.Rotary([2], device=0)
+    rot.device = -1                                    # the CPU's number
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        for args in ((dual, q, q), (q, dual, q), (q, q, dual)):
+            with pytest.raises(NotImplementedError, match="attention"):
+                A.attention(*args)
+        for args in ((dual, None), (q, dual), (dual, q)):
+            with pytest.raises(NotImplementedError, match="Rotary"):
+                rot(*args, pos)
+        leaf = q.clone().requires_grad_()
+        for out in (A.attention(leaf, leaf, leaf), rot(leaf, None, pos)):
+            with pytest.raises(NotImplementedError, match="gradient"):
+                torch.autograd.grad(out, [leaf], dual)
+        assert A.attention(q, q, q).shape == q.shape and rot(q, q, pos)[1].shape == q.shape       # tensors without a tangent
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda x: A.attention(x, q, q), (q,), (q,))
