@@ -357,7 +357,8 @@ int mmfe_attention_backward(const mmfe_attention_args* args, const mmfe_attentio
  * classification/vggsound/vanilla_single.py:75-80).  norm = (sum of all squares)^(1/2) (MMFE_NORM_2) or the largest magnitude
  * (MMFE_NORM_MAX) over all tensors, summed in float64 in a fixed order; with out != NULL every tensor times
  * min(1, max_norm / (norm + 1e-6)) goes to out[i], as out_dtype[i]; out[i] may be x[i] with the same type (in place: nothing is
- * written when the factor is 1).  A NaN norm makes every output NaN; an infinite one makes finite values zero.
+ * written when the factor is 1).  A NaN norm makes every output NaN, and so does an infinite one under an infinite
+ * max_norm; an infinite norm under a finite max_norm makes finite values zero.
  *   x, numel, dtype, out, out_dtype   HOST arrays of n_tensors entries, read before the call returns; x[i] / out[i] are device
  *                                     pointers of numel[i] contiguous elements (MMFE_OUT_* types), aligned to their elements
  *   partials                          device, mmfe_grad_partials(n_tensors) doubles, the call's own until it has run

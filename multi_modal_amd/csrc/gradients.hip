@@ -194,8 +194,10 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const ScaleArgs p) {
     __shared__ double lds[kThreads / 64];
     const double norm = total_norm(p.partial, p.n_partial, p.max_kind, lds);
     if (p.store && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = (float)norm;
-    // rounded once, and the product once; a norm that float32 does not hold counts as the infinity it is returned as
-    float c = isinf((float)norm) ? 0.f : (float)(p.max_norm / (norm + 1e-6));
+    // rounded once, and the product once; a norm that float32 does not hold counts as the infinity it is returned as: a factor of 0, or NaN where the
+    // limit is infinite too
+    const float held = (float)norm;
+    float c = isinf(held) ? p.max_norm / held : (float)(p.max_norm / (norm + 1e-6));
     if (c > 1.f) c = 1.f;                                        // a NaN norm stays a NaN and reaches every gradient
     for (uint32_t k = blockIdx.x; k < p.n_chunks; k += gridDim.x) {
         const int t = find(p.first, p.n_tensors, k);

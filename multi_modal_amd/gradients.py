@@ -104,8 +104,9 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: f
 def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                    error_if_nonfinite: bool = False, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the gradients of `parameters` (or the tensors themselves, where they are no parameters) by
-    min(1, max_norm / (norm + 1e-6)), in place, and returns their norm, as torch.nn.utils.clip_grad_norm_ does; a NaN norm makes
-    every gradient NaN.  With `out` (one contiguous tensor per gradient, same number of elements, any of the three types) the
+    min(1, max_norm / (norm + 1e-6)), in place, and returns their norm, as torch.nn.utils.clip_grad_norm_ does: a NaN norm makes
+    every gradient NaN, an infinite one finite gradients zero (NaN where max_norm is infinite too).  With `out` (one contiguous tensor
+    per gradient, same number of elements, any of the three types) the
     scaled gradients go there and the gradients stay as they are.  The tensors must not share memory.
     error_if_nonfinite=True waits for the norm and raises before anything is scaled."""
     kind = _kind(norm_type)

@@ -340,3 +340,25 @@ def test_clipping_rounds_twice_and_infinite_norms_give_zeros(mm):
         assert ((a.double() - b).abs() <= 2.01 * 2.0 ** -24 * b.abs()).all()
     big = torch.full((8,), 3e38, device="cuda")
     assert mm.clip_grad_norm([big], 1.0).isinf() and (big == 0).all()
+
+
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+def test_infinite_limits(mm, kind):
+    """max_norm = inf measures the norm and leaves the gradients alone, unless the norm is infinite: NaN then, as torch's own has it."""
+    for value, scaled in ((2.0, 1.0), (math.inf, math.nan), (math.nan, math.nan)):
+        x = [torch.ones(5000, device="cuda"), torch.ones(70, device="cuda").to(torch.bfloat16)]
+        x[1][3] = value
+        want = [torch.nn.Parameter(t.float()) for t in x]
+        for p, t in zip(want, x):
+            p.grad = t.float().clone()
+        norm = torch.nn.utils.clip_grad_norm_(want, math.inf, kind)
+        outs = [torch.zeros(t.shape, device="cuda") for t in x]
+        got = mm.clip_grad_norm(x, math.inf, kind, out=outs)
+        assert torch.allclose(got, norm, rtol=2.0 ** -20, atol=0, equal_nan=True)
+        mm.clip_grad_norm(x, math.inf, kind)
+        for t, o, p in zip(x, outs, want):
+            assert torch.equal(t.float().nan_to_num(7.0), p.grad.nan_to_num(7.0)) and torch.equal(o.nan_to_num(7.0), p.grad.nan_to_num(7.0))
+            assert torch.equal(t[:3].float().nan_to_num(7.0), torch.full((3,), scaled, device="cuda").nan_to_num(7.0))
+    if kind == 2.0:                                    # finite in float64, infinite in float32
+        big = torch.full((1000,), 3e38, device="cuda")
+        assert mm.clip_grad_norm([big], math.inf).isinf() and big.isnan().all()
