@@ -33,15 +33,26 @@ def grid_positions(*sizes: int, device=None) -> torch.Tensor:
     return torch.stack([a.reshape(-1) for a in axes])
 
 
+def _gpu_index(device: Union[None, int, str, torch.device]) -> Optional[int]:
+    """Index of a GPU, None for the current one."""
+    if device is None:
+        return None
+    d = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+    if d.type != "cuda":
+        raise ValueError(f"the frequency table lives on a GPU, not on {d}")
+    return d.index
+
+
 class Rotary:
     """Rotary(sections): sections[a] = element pairs of a head that axis a turns (1 to 4 axes, 2 * sum(sections) <= head size; the
     elements behind them pass through).
 
     ladder "shared": pair i of all R = sum(sections) turns with base ** (-i / R); "axis": the j-th pair of axis a with
     base ** (-j / sections[a]).  pairing "halves": elements (i, i + R) form a pair; "adjacent": elements (2 i, 2 i + 1).
-    The frequency table lives on `device` (default: the current one); the object may be shared between threads and streams."""
+    The frequency table lives on the GPU `device` (an index, "cuda", "cuda:1", a torch.device; default: the current one); the object may be shared between threads and streams."""
 
-    def __init__(self, sections: Sequence[int], base: float = 10000.0, ladder: str = "axis", pairing: str = "halves", device: Optional[int] = None):
+    def __init__(self, sections: Sequence[int], base: float = 10000.0, ladder: str = "axis", pairing: str = "halves",
+                 device: Union[None, int, str, torch.device] = None):
         self.sections = tuple(int(s) for s in sections)
         if ladder not in _LADDERS or pairing not in _PAIRINGS:
             raise ValueError("ladder is 'shared' or 'axis', pairing is 'halves' or 'adjacent'")
@@ -49,10 +60,11 @@ class Rotary:
             raise ValueError(f"sections: 1 to 4 axes with 1 to 512 pairs together, got {self.sections}")
         if not 0.0 < float(base) < float("inf"):
             raise ValueError("base must be a positive number")
+        index = _gpu_index(device)
         require_gpu()
         self.base, self.ladder, self.pairing = float(base), ladder, pairing
         self._pairs2 = 2 * sum(self.sections)
-        self.device = torch.cuda.current_device() if device is None else torch.device("cuda", device).index if isinstance(device, int) else torch.device(device).index
+        self.device = torch.cuda.current_device() if index is None else index
         self._h = N.RotaryHandle(self.sections, _LADDERS[ladder], _PAIRINGS[pairing], self.base, self.device)
 
     def __call__(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,

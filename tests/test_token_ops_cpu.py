@@ -343,3 +343,16 @@ def test_forward_mode_is_refused(N, monkeypatch):
         assert A.attention(q, q, q).shape == q.shape and rot(q, q, pos)[1].shape == q.shape       # tensors without a tangent
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda x: A.attention(x, q, q), (q,), (q,))
+
+
+def test_rotary_devices(N, monkeypatch):
+    """Devices by index, name and object; a missing index is the current GPU, and what is no GPU is refused."""
+    from multi_modal_amd import rotary as R
+    for device in ("cpu", "cpu:0", torch.device("cpu"), torch.device("meta")):
+        with pytest.raises(ValueError, match="GPU"):
+            R.Rotary([4], device=device)
+    monkeypatch.setattr(R, "require_gpu", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(R.N, "RotaryHandle", lambda *a: a)
+    for device, index in ((None, 3), ("cuda", 3), (torch.device("cuda"), 3), (0, 0), (2, 2), ("cuda:1", 1), (torch.device("cuda", 1), 1)):
+        assert R.Rotary([4], device=device)._h[4] == index == R.Rotary([4], device=device).device
