@@ -34,14 +34,21 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
         s = (0, n if m[0] > 1 else 0, h if m[1] > 1 else 0)
     if e == 1 and t.data_ptr() % 16 == 0 and (s[0] | s[1] | s[2]) % 8 == 0 and s[1] <= 1 << 24:
         return t, s
-    t = t.contiguous()
-    return _rows(t if t.data_ptr() % 16 == 0 else t.clone())
+    return _dense(t), _packed_strides(t)
 
 
 def _packed_strides(t: torch.Tensor) -> Tuple[int, int, int]:
     """Strides of a contiguous tensor of t's shape."""
     h, d = t.shape[-2], t.shape[-1]
     return (t.shape[-3] * h * d if t.dim() == 4 else 0, h * d, d)
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t, or a copy of it, contiguous and on a 16-byte boundary."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _counts(x, name: str, n: int, device, limit: Optional[int] = None, rising: bool = False) -> Optional[torch.Tensor]:
@@ -70,14 +77,6 @@ def _counts(x, name: str, n: int, device, limit: Optional[int] = None, rising: b
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
-
-
-def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """t, or a copy of it, contiguous and on a 16-byte boundary."""
-    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class _Call:

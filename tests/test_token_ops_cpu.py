@@ -356,3 +356,15 @@ def test_rotary_devices(N, monkeypatch):
     monkeypatch.setattr(R.N, "RotaryHandle", lambda *a: a)
     for device, index in ((None, 3), ("cuda", 3), (torch.device("cuda"), 3), (0, 0), (2, 2), ("cuda:1", 1), (torch.device("cuda", 1), 1)):
         assert R.Rotary([4], device=device)._h[4] == index == R.Rotary([4], device=device).device
+
+
+def test_attention_rows_of_empty_and_strided_tensors():
+    """Every layout ends in one that the kernels read: a tensor without elements counts as contiguous whatever its strides."""
+    from multi_modal_amd import attention as A
+    x = torch.arange(2 * 10 * 3 * 32, dtype=torch.float16).view(2, 10, 3, 32)
+    for t in (x[..., ::2][:, :0], x[:, :0, :, :12], x[:0, ..., 1:9], x[:0, :, ::2, ::4], x[0, :0, :, ::4], torch.zeros(2, 0, 3, 12, dtype=torch.float16)[..., :8],
+              x, x[..., ::2], x[..., 1:17], x[..., 8:16], x.transpose(1, 2), x[0], x[0, :, :, 4:12], x[:, :1, :, 2:10], x.transpose(1, 3)[..., 0:1].expand(-1, -1, -1, 8)):
+        r, strides = A._rows(t)
+        assert torch.equal(r, t) and r.shape == t.shape
+        used = [(s, g) for s, g, n in zip(r.stride()[:-1], strides[-(r.dim() - 1):], r.shape) if n > 1 and r.numel()]
+        assert all(s == g for s, g in used) and all(s % 8 == 0 for s in strides) and r.data_ptr() % 16 == 0 and (r.stride(-1) == 1 or not r.numel())
