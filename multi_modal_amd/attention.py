@@ -8,7 +8,6 @@ what a stream has kept.
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -19,6 +18,8 @@ from .plans import OUT_CODES, once_differentiable, raw_stream, refuse_forward_mo
 _ARGS_SIZE = ctypes.sizeof(N.AttentionArgs)
 _GRADS_SIZE = ctypes.sizeof(N.AttentionGrads)
 _DTYPES = (torch.float16, torch.bfloat16)
+_LARGEST = torch.finfo(torch.float32).max
+_SCALES = (2.0 ** -90, 2.0 ** 126)
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
@@ -193,8 +194,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths=None
     call = _Call()
     call.cap = float(cap)
     call.scale = D ** -0.5 if scale is None else float(scale)
-    if not (0.0 <= call.cap < math.inf) or not (0.0 < call.scale < math.inf):
-        raise ValueError("cap must be >= 0 and scale > 0, both finite")
+    # as the float32 that the kernels take: a cap that rounds to zero would be none, and below the least scale a row without keys would get weights
+    if not (0.0 <= call.cap <= _LARGEST and (call.cap == 0.0 or ctypes.c_float(call.cap).value > 0.0)) or not _SCALES[0] <= call.scale <= _SCALES[1]:
+        raise ValueError("cap must be 0 or a positive float32, and scale lie between 2^-90 and 2^126")
     if prefix is not None and not causal:
         raise ValueError("prefix belongs to causal=True")
     if packed and (lengths is not None or kv_lengths is not None):

@@ -731,7 +731,8 @@ int make_problem(const mmfe_attention_args* a, Problem& p) {
     if (a->heads < 1 || a->kv_heads < 1 || a->heads > 4096 || a->heads % a->kv_heads != 0) { set_error("attention: %d query heads cannot share %d key heads", a->heads, a->kv_heads); return MMFE_EINVAL; }
     if (a->q_rows > (1 << 30) || a->k_rows > (1 << 30) || a->n_docs > (1 << 24)) { set_error("attention: too many rows"); return MMFE_EINVAL; }
     if (a->slopes != nullptr && (a->q_rows > (1 << 24) || a->k_rows > (1 << 24))) { set_error("attention: distances are float32: at most 2^24 rows with slopes"); return MMFE_EINVAL; }
-    if (!(a->scale > 0.f) || !std::isfinite(a->scale) || !(a->cap >= 0.f) || !std::isfinite(a->cap)) { set_error("attention: scale > 0 and cap >= 0 must be finite"); return MMFE_EINVAL; }
+    // the least scale takes the gradients' mark of rows without keys, -1e30 in the products' units, to -1200 in log2 units: p = 0
+    if (!(a->scale >= 0x1p-90f) || a->scale > 0x1p126f || !(a->cap >= 0.f) || !std::isfinite(a->cap)) { set_error("attention: scale must lie between 2^-90 and 2^126, cap >= 0 be finite"); return MMFE_EINVAL; }
     if (a->cap > 0.f && !std::isfinite(4.f * a->scale / a->cap)) { set_error("attention: cap is too small against scale"); return MMFE_EINVAL; }
     if (a->packed && (a->q_off == nullptr || a->k_off == nullptr)) { set_error("attention: packed documents need offsets"); return MMFE_EINVAL; }
     if (a->prefix != nullptr && !a->causal) { set_error("attention: a prefix belongs to a causal mask"); return MMFE_EINVAL; }

@@ -368,3 +368,22 @@ def test_attention_rows_of_empty_and_strided_tensors():
         assert torch.equal(r, t) and r.shape == t.shape
         used = [(s, g) for s, g, n in zip(r.stride()[:-1], strides[-(r.dim() - 1):], r.shape) if n > 1 and r.numel()]
         assert all(s == g for s, g in used) and all(s % 8 == 0 for s in strides) and r.data_ptr() % 16 == 0 and (r.stride(-1) == 1 or not r.numel())
+
+
+def test_attention_scales_and_caps_past_float32(N):
+    """Numbers that float32 does not hold, or holds as zero, are refused rather than rounded to another meaning."""
+    from multi_modal_amd.attention import attention as fn
+    q = torch.zeros(2, 10, 4, 64, dtype=torch.bfloat16)
+    for kw in (dict(cap=1e300), dict(cap=1e-60), dict(scale=1e300), dict(scale=1e-60), dict(scale=1e-28), dict(scale=3e38), dict(cap=math.nan)):
+        with pytest.raises(ValueError, match="scale"):
+            fn(q, q, q, **kw)
+    lib, A = N.load_library(), 1 << 20
+
+    def forward(scale, cap):
+        s = N.AttentionArgs(struct_size=ctypes.sizeof(N.AttentionArgs), dtype=2, n_docs=2, heads=4, kv_heads=4, dim=64, scale=scale, cap=cap, q_rows=10, k_rows=10,
+                            q=A, k=A, v=A, out=A)
+        return lib.mmfe_attention_forward(ctypes.byref(s), None, 99, None)
+    good = forward(0.1, 0.0)
+    assert good not in (0, -1)
+    assert forward(2.0 ** -90, 0.0) == forward(2.0 ** 126, 0.0) == forward(0.1, 3e38) == forward(0.1, 1e-30) == good
+    assert forward(2.0 ** -91, 0.0) == forward(2.0 ** 127, 0.0) == forward(-0.1, 0.0) == forward(math.nan, 0.0) == forward(0.1, math.inf) == -1
