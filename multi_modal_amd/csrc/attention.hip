@@ -787,14 +787,14 @@ int mmfe_attention_forward(const mmfe_attention_args* a, void* workspace, int de
     if (tiles == 0) return MMFE_OK;
     if (a->out == nullptr) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride)) return MMFE_EINVAL;
-    if (tiles * a->heads > 0x7fffffffll) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
     f.out = Rows{a->out, a->out_stride[0], a->out_stride[1], a->out_stride[2]};
     f.rest = static_cast<char*>(a->out_rest);
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     f.lse = a->lse; f.lse_b = a->lse_stride[0]; f.lse_h = a->lse_stride[1];
     const Cut c = cut_keys(a);
     if ((c.n_splits > 1 || c.cuts > 1) && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
-    if (c.units * c.n_splits > 0x7fffffffll || c.units > 0x3ffffff || tiles * a->heads * c.cuts > 0x7fffffffll) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
+    // (keys are cut into several chunks below 2048 units only, so that the joining launch is always small)
+    if (c.n_splits > 0 ? too_many_blocks(c.units * c.n_splits, 64 * kSplitWaves) : too_many_blocks(tiles * a->heads * c.cuts, kThreads)) { set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL; }
     OnDevice on(device);
     if (on.rc) return on.rc;
     const bool bf = a->dtype == MMFE_OUT_BF16;

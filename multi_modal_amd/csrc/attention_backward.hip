@@ -893,7 +893,9 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride) || bad_rows("grad_out", g->grad_out, g->grad_out_stride) || bad_rows("grad_q", g->grad_q, g->grad_q_stride) ||
         bad_rows("grad_k", g->grad_k, g->grad_k_stride) || bad_rows("grad_v", g->grad_v, g->grad_v_stride)) return MMFE_EINVAL;
-    if (count_tiles(b.p, a->q_rows, kRows) * a->heads * row_cuts(a) + count_tiles(b.p, a->k_rows, kRows) * a->heads * key_cuts(a) > 0x7fffffffll) {
+    const int64_t tq = count_tiles(b.p, a->q_rows, kRows), tk = count_tiles(b.p, a->k_rows, kRows);
+    if (whole ? too_many_blocks((int64_t)a->n_docs * a->heads, 512)
+              : too_many_blocks(tq * a->heads + tk * a->kv_heads, kThreads) || too_many_blocks(tq * a->heads * row_cuts(a), kThreads) || too_many_blocks(tk * a->kv_heads * key_cuts(a), kThreads)) {
         set_error("attention: too many rows and heads in one call"); return MMFE_EINVAL;
     }
     auto rows = [](const void* ptr, const int64_t* s) { return Rows{ptr, s[0], s[1], s[2]}; };

@@ -237,6 +237,9 @@ struct OnDevice {
     OnDevice& operator=(const OnDevice&) = delete;
 };
 
+// Whether a launch of so many blocks is past what HIP takes: 2^32 - 1 threads.
+inline bool too_many_blocks(int64_t blocks, int threads) { return blocks > 0xffffffffll / threads; }
+
 // Launch-geometry helpers (thread-safe, cached per kernel and device).
 //   kernel_prepare: raises the kernel's dynamic-LDS limit to the CU's 160 KB on the current device (once) and
 //   returns how many blocks of `threads` threads with `lds` bytes of dynamic LDS are resident per CU, and the CU count.

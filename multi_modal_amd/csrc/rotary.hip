@@ -310,6 +310,7 @@ int mmfe_rotary_run(const mmfe_rotary* handle, const mmfe_rotary_args* a, void* 
     if (T < 1) T = 1;
     p.T = (int)T;
     p.dN = fast_div((uint32_t)p.N); p.dR = fast_div((uint32_t)p.R); p.dItems = fast_div((uint32_t)items); p.dChunks = fast_div((uint32_t)p.chunks);
+    if (too_many_blocks((p.tokens + p.T - 1) / p.T, kThreads)) { set_error("rotary: too many tokens in one call"); return MMFE_EINVAL; }
     OnDevice on(h->device);
     if (on.rc) return on.rc;
     const size_t lds = kMaxTokens * 4 * 8 + (size_t)p.T * p.R * 8;

@@ -387,3 +387,30 @@ def test_attention_scales_and_caps_past_float32(N):
     assert good not in (0, -1)
     assert forward(2.0 ** -90, 0.0) == forward(2.0 ** 126, 0.0) == forward(0.1, 3e38) == forward(0.1, 1e-30) == good
     assert forward(2.0 ** -91, 0.0) == forward(2.0 ** 127, 0.0) == forward(-0.1, 0.0) == forward(math.nan, 0.0) == forward(0.1, math.inf) == -1
+
+
+def test_attention_grids_past_the_launch_limit(N):
+    """More blocks than a launch takes (2^32 - 1 threads) are refused before anything is launched; device 99 is what a good call is refused for."""
+    lib, A = N.load_library(), 1 << 20
+
+    def args(**kw):
+        a = dict(struct_size=ctypes.sizeof(N.AttentionArgs), dtype=2, n_docs=2, heads=4, kv_heads=4, dim=64, scale=0.1, cap=0.0, q_rows=10, k_rows=10, q=A, k=A, v=A, out=A, lse=A)
+        a.update(kw)
+        s = N.AttentionArgs(**a)
+        s.lse_stride = (ctypes.c_int64 * 2)(a["heads"] * a["q_rows"], a["q_rows"])
+        return s
+
+    def both(**kw):
+        g = N.AttentionGrads(struct_size=ctypes.sizeof(N.AttentionGrads), grad_out=A, grad_q=A, grad_k=A, grad_v=A)
+        return (lib.mmfe_attention_forward(ctypes.byref(args(**kw)), A, 99, None),
+                lib.mmfe_attention_backward(ctypes.byref(args(**kw)), ctypes.byref(g), A, 99, None))
+    good = both()[0]
+    assert both() == (good, good) and good not in (0, -1)
+    assert both(n_docs=2 ** 20, heads=16, kv_heads=16) == (-1, -1)                    # 2^24 blocks of 256
+    assert both(n_docs=2 ** 20, heads=15, kv_heads=15, dim=72) == (good, -1)          # the preparing launch of the gradients has 2 x 15 x 2^20
+    assert both(n_docs=2 ** 19, heads=15, kv_heads=15) == (good, good)
+    assert both(n_docs=2 ** 19, heads=16, kv_heads=16) == (good, -1)                  # short documents: 2^23 blocks of 512
+    assert both(n_docs=2 ** 17, heads=8, kv_heads=8, q_rows=1, k_rows=4000) == (good, -1)
+    assert both(n_docs=2 ** 21, heads=64, kv_heads=8, q_rows=1, k_rows=4000)[0] == good   # one chunk a key head: 2^24 blocks of 128
+    assert both(n_docs=2 ** 22, heads=64, kv_heads=8, q_rows=1, k_rows=4000)[0] == -1
+    assert both(packed=1, q_off=A, k_off=A, n_docs=2 ** 23, heads=2, kv_heads=2) == (-1, -1)
