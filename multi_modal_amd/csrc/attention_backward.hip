@@ -891,6 +891,8 @@ int mmfe_attention_backward(const mmfe_attention_args* a, const mmfe_attention_g
     if (any_k && (g->grad_k == nullptr || g->grad_v == nullptr)) { set_error("attention: NULL data pointer"); return MMFE_EINVAL; }
     if ((any_q || any_k) && !whole && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) { set_error("attention: this call needs a 16-byte aligned workspace"); return MMFE_EINVAL; }
     if ((reinterpret_cast<uintptr_t>(a->out_rest) & 15) != 0) { set_error("attention: out_rest: 16-byte aligned"); return MMFE_EINVAL; }
+    // the workspace's statistics are addressed as lse is
+    if (any_q && ((a->heads > 1 && a->lse_stride[1] != a->q_rows) || (!a->packed && a->n_docs > 1 && a->lse_stride[0] != a->heads * a->q_rows))) { set_error("attention: lse must be dense"); return MMFE_EINVAL; }
     if (bad_rows("out", a->out, a->out_stride) || bad_rows("grad_out", g->grad_out, g->grad_out_stride) || bad_rows("grad_q", g->grad_q, g->grad_q_stride) ||
         bad_rows("grad_k", g->grad_k, g->grad_k_stride) || bad_rows("grad_v", g->grad_v, g->grad_v_stride)) return MMFE_EINVAL;
     const int64_t tq = count_tiles(b.p, a->q_rows, kRows), tk = count_tiles(b.p, a->k_rows, kRows);

@@ -414,3 +414,22 @@ def test_attention_grids_past_the_launch_limit(N):
     assert both(n_docs=2 ** 21, heads=64, kv_heads=8, q_rows=1, k_rows=4000)[0] == good   # one chunk a key head: 2^24 blocks of 128
     assert both(n_docs=2 ** 22, heads=64, kv_heads=8, q_rows=1, k_rows=4000)[0] == -1
     assert both(packed=1, q_off=A, k_off=A, n_docs=2 ** 23, heads=2, kv_heads=2) == (-1, -1)
+
+
+def test_attention_backward_takes_a_dense_lse_only(N):
+    """Statistics of the rows lie in the workspace as lse does: strides of a larger array would lead out of it."""
+    lib, A = N.load_library(), 1 << 20
+
+    def backward(stride, **kw):
+        a = dict(struct_size=ctypes.sizeof(N.AttentionArgs), dtype=2, n_docs=2, heads=4, kv_heads=2, dim=64, scale=0.1, cap=0.0, q_rows=10, k_rows=10, q=A, k=A, v=A, out=A, lse=A)
+        a.update(kw)
+        s = N.AttentionArgs(**a)
+        s.lse_stride = (ctypes.c_int64 * 2)(*stride)
+        g = N.AttentionGrads(struct_size=ctypes.sizeof(N.AttentionGrads), grad_out=A, grad_q=A, grad_k=A, grad_v=A)
+        return lib.mmfe_attention_backward(ctypes.byref(s), ctypes.byref(g), A, 99, None)
+    good = backward((40, 10))
+    assert good not in (0, -1)
+    assert backward((80, 10)) == backward((40, 20)) == backward((10, 20)) == backward((40, -10)) == backward((80, 10), kv_heads=4) == -1
+    packed = dict(packed=1, q_off=A, k_off=A)
+    assert backward((0, 10), **packed) == backward((7, 10), **packed) == backward((7, 10), n_docs=1) == backward((10, 3), heads=1, kv_heads=1) == good
+    assert backward((0, 12), **packed) == -1
