@@ -14,7 +14,7 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, mark_written, raw_stream, require_gpu
+from .plans import OUT_CODES, folded, mark_written, raw_stream, require_gpu
 
 _KINDS = {2.0: N.NORM_2, math.inf: N.NORM_MAX}
 
@@ -137,10 +137,12 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
         norm = _run(grads, codes, grads, codes, kind, max_norm, device)
         mark_written(grads)
         return norm
-    # views with gaps: their values pass through a packed copy
-    for t in grads:
-        if any(s == 0 and m > 1 for s, m in zip(t.stride(), t.shape)):
-            raise ValueError("clip_grad_norm cannot write an expanded gradient")
+    # views with gaps: their values pass through a packed copy, so the library does not see what they share
+    if any(map(folded, grads)):
+        raise ValueError("clip_grad_norm cannot write a gradient whose elements share memory (an expanded view)")
+    starts = [t.data_ptr() for t in grads if t.numel()]
+    if len(set(starts)) < len(starts):
+        raise ValueError("clip_grad_norm: two of the gradients share memory (the same gradient given twice?)")
     packed = [t if _dense(t) else t.contiguous() for t in grads]
     norm = _run(packed, codes, packed, codes, kind, max_norm, device)
     mark_written(packed)

@@ -55,6 +55,18 @@ def mark_written(tensors) -> None:
         torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
+def folded(t: torch.Tensor) -> bool:
+    """Whether two of t's elements may be one in memory (expanded and overlapping views)."""
+    if t.is_contiguous() or t.numel() == 0:
+        return False
+    reach = 1
+    for s, m in sorted((s, m) for s, m in zip(t.stride(), t.shape) if m > 1):
+        if s < reach:
+            return True
+        reach += s * (m - 1)
+    return False
+
+
 def refuse_forward_mode(what: str, *tensors) -> None:
     """A dual tensor (torch.autograd.forward_ad) does not say requires_grad; a kernel would read its value and drop its tangent."""
     if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):

@@ -16,7 +16,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _native as N
-from .plans import OUT_CODES, mark_written, once_differentiable, raw_stream, refuse_forward_mode, require_gpu
+from .plans import OUT_CODES, folded as _folded, mark_written, once_differentiable, raw_stream, refuse_forward_mode, require_gpu
 
 _ARGS_SIZE = ctypes.sizeof(N.RotaryArgs)
 
@@ -147,18 +147,6 @@ class Rotary:
 
     def close(self) -> None:
         self._h.close()
-
-
-def _folded(t: torch.Tensor) -> bool:
-    """Whether two of t's elements may be one in memory (expanded and overlapping views)."""
-    if t.is_contiguous() or t.numel() == 0:
-        return False
-    reach = 1
-    for s, m in sorted((s, m) for s, m in zip(t.stride(), t.shape) if m > 1):
-        if s < reach:
-            return True
-        reach += s * (m - 1)
-    return False
 
 
 def _share(a: torch.Tensor, b: torch.Tensor) -> bool:

@@ -362,3 +362,20 @@ def test_infinite_limits(mm, kind):
     if kind == 2.0:                                    # finite in float64, infinite in float32
         big = torch.full((1000,), 3e38, device="cuda")
         assert mm.clip_grad_norm([big], math.inf).isinf() and big.isnan().all()
+
+
+def test_clip_views_that_share_memory(mm):
+    """Views with gaps go through copies: the same view twice, and views that overlap themselves, are refused as dense ones are; neighbours are not."""
+    buf = torch.randn(12, 40, device="cuda")
+    keep = buf.clone()
+    a = buf[:, :7]
+    flat = buf.view(-1)
+    for grads in ([a, a], [a, buf[:, 9:12], a], [buf[:, :7], buf[:, :5]], [flat.as_strided((5, 8), (4, 1)), buf[6:, :3]], [a[:1].expand(3, 7), buf[:, 9:12]]):
+        with pytest.raises(ValueError, match="share memory"):
+            mm.clip_grad_norm(grads, 0.1)
+        assert torch.equal(buf, keep)
+    _, ref = clip_ref([buf[:, :7], buf[:, 7:20]], 0.1, 2.0)
+    mm.clip_grad_norm([buf[:, :7], buf[:0, :3], buf[:, 7:20], buf[:0, 1:4]], 0.1)
+    check_clipped(buf[:, :7], ref[0], torch.float32)
+    check_clipped(buf[:, 7:20], ref[1], torch.float32)
+    assert torch.equal(buf[:, 20:], keep[:, 20:])
