@@ -125,6 +125,7 @@ class _AttentionFn(torch.autograd.Function):
         ctx.form = _form(saved)
         ctx.save_for_backward(*saved)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)       # or every backward pass fills a gradient of lse's shape with zeros that nothing reads
         return out, lse
 
     @staticmethod
@@ -134,6 +135,8 @@ class _AttentionFn(torch.autograd.Function):
         # from what was unpacked, and the forward pass's strides serve only where they are still the tensors' own.
         saved, call = ctx.saved_tensors, ctx.call
         q, k, v, out, rest, lse, *counts = saved
+        if grad_out is None:                   # an operation behind this one returned no gradient
+            return tuple(torch.zeros_like(t) if needed else None for t, needed in zip((q, k, v), ctx.needs_input_grad)) + (None,)
         strides, form = call.strides, _form(saved)
         if form != ctx.form:
             for new, old in zip(form, ctx.form):

@@ -433,3 +433,37 @@ def test_attention_backward_takes_a_dense_lse_only(N):
     packed = dict(packed=1, q_off=A, k_off=A)
     assert backward((0, 10), **packed) == backward((7, 10), **packed) == backward((7, 10), n_docs=1) == backward((10, 3), heads=1, kv_heads=1) == good
     assert backward((0, 12), **packed) == -1
+
+
+def test_attention_backward_fills_no_gradient_of_lse(N, monkeypatch):
+    """lse has no gradient: nothing is allocated and zeroed for one; an undefined gradient of the output still gives zeros."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from multi_modal_amd import attention as A
+    monkeypatch.setattr(A, "require_gpu", lambda: None)
+    monkeypatch.setattr(A, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda self: self)
+    monkeypatch.setattr(A.N, "attention_forward", lambda *a: None)
+    monkeypatch.setattr(A.N, "attention_backward", lambda *a: None)
+    seen = []
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    q = torch.zeros(2, 30, 4, 64, dtype=torch.float16, requires_grad=True)
+    out, lse = A.attention(q, q, q, return_lse=True)
+    assert not lse.requires_grad
+    with Record():
+        torch.autograd.grad(out, [q], torch.ones_like(out))
+    assert not any("zero" in name for name in seen) and any("empty" in name for name in seen), seen
+
+    class Nothing(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+    (g,) = torch.autograd.grad(Nothing.apply(A.attention(q, q, q)), [q], torch.ones_like(out), allow_unused=True)
+    assert (g == 0).all()
