@@ -683,3 +683,44 @@ def test_capped_scores_of_any_cap(mm, O, case, cap, size):
         for t, n in ((q, lens[b]), (g, lens[b]), (k, m[b]), (v, m[b])):
             t[b, n:] = math.nan
     check(mm, Relative, q, k, v, docs_padded(lens, m, N, S), opts, g=g, flat=flat4, lse_flat=lse4, host=host)
+
+
+def test_cut_walks_with_rows_that_see_nothing(mm, O):
+    """1000 of 1200 rows over 700 of 1200 keys of one head, causal, walks cut: the rows that see keys, next to 300 that see none."""
+    gen = torch.Generator().manual_seed(21)
+    q, k, v, g = (torch.randn(1, 1200, 1, 64, generator=gen).to(HF).cuda() for _ in range(4))
+    check(mm, O, q, k, v, docs_padded([1000], [700], 1200, 1200), dict(causal=True, lengths=[1000], kv_lengths=[700]), g=g, flat=flat4, lse_flat=lse4)
+
+
+@pytest.mark.parametrize("rows, H, K, D, causal", [(2000, 2, 1, 64, False), (2000, 2, 2, 64, True), (1300, 4, 2, 128, True), (1100, 2, 1, 96, False), (1500, 1, 1, 32, True)])
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_long_documents_in_the_mean(mm, O, dtype, rows, H, K, D, causal):
+    """The bounds of single elements add up worst cases over the keys, and would let a lost tile of 32 keys pass among 2000.  Roundings are independent:
+    a result's mean square error is the sum of its terms' squares, (u p v)^2 over the keys for o, (u p g)^2 over the rows for dv, (u scale ds k)^2 and
+    (u scale ds q)^2 for dq and dk, and (u x)^2 for its own rounding, u half a step of the type, at which a rounding's mean square is at most a third of u^2."""
+    gen = torch.Generator().manual_seed(rows + D)
+    q, g = (torch.randn(1, rows, H, D, generator=gen).to(dtype).cuda() for _ in "qg")
+    k, v = (torch.randn(1, rows, K, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = mm.attention.attention(*x, causal=causal)
+    dq, dk, dv = torch.autograd.grad(o, x, g)
+    u, scale = torch.finfo(dtype).eps / 2, D ** -0.5
+    ref = {n: torch.zeros(rows, h, D, dtype=torch.float64, device="cuda") for n, h in (("o", H), ("dq", H), ("dk", K), ("dv", K))}
+    var = {n: torch.zeros_like(t) for n, t in ref.items()}
+    for h in range(H):
+        c = h // (H // K)
+        a = [t.double() for t in (q[0, :, h], k[0, :, c], v[0, :, c], g[0, :, h])]
+        r = O.attention_head(*a[:3], scale, causal=causal, g=a[3])
+        p2, ds2 = r["p"].square(), (scale * r["ds"]).square()
+        ref["o"][:, h], ref["dq"][:, h] = r["o"], r["dq"]
+        ref["dk"][:, c] += r["dk"]
+        ref["dv"][:, c] += r["dv"]
+        var["o"][:, h] = p2 @ a[2].square()
+        var["dq"][:, h] = ds2 @ a[1].square()
+        var["dk"][:, c] += ds2.T @ a[0].square()
+        var["dv"][:, c] += p2.T @ a[3].square()
+    for name, got in (("o", o), ("dq", dq), ("dk", dk), ("dv", dv)):
+        # in blocks of 100 rows, so that the few large ones do not cover the others
+        err, bound = ((t.flatten(1).mean(1).split(100)) for t in ((got.detach()[0].double() - ref[name]).square(), u * u * (var[name] + ref[name].square())))
+        for i, (e, b) in enumerate(zip(err, bound)):
+            assert float(e.mean()) <= float(b.mean()), (name, i, float((e.mean() / b.mean()).sqrt()))
