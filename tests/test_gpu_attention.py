@@ -724,3 +724,53 @@ def test_long_documents_in_the_mean(mm, O, dtype, rows, H, K, D, causal):
         err, bound = ((t.flatten(1).mean(1).split(100)) for t in ((got.detach()[0].double() - ref[name]).square(), u * u * (var[name] + ref[name].square())))
         for i, (e, b) in enumerate(zip(err, bound)):
             assert float(e.mean()) <= float(b.mean()), (name, i, float((e.mean() / b.mean()).sqrt()))
+
+
+CROSS = [
+    # rows of each document, keys of each, rows before and behind, keys before and behind, H, K, D, dtype, causal, prefix, bias, cap
+    ([5, 200, 0, 64, 129], [300, 10, 7, 0, 129], (3, 9), (0, 40), 4, 2, 64, BF, True, True, False, 0.0),
+    ([1, 1, 3, 1], [5000, 0, 1300, 31], (0, 0), (0, 0), 8, 2, 128, HF, True, False, True, 0.0),        # new tokens over packed keys, walks cut
+    ([1500, 20], [40, 900], (0, 1), (130, 0), 2, 1, 72, BF, False, False, True, 9.0),
+    ([3, 0, 7] * 30, [0, 5, 150] * 30, (2, 0), (0, 3), 2, 2, 32, HF, True, True, False, 100.0),        # more than 64 documents
+    ([130, 1] * 40, [1, 257] * 40, (0, 0), (0, 0), 3, 1, 96, BF, False, False, False, 0.0),
+]
+
+
+@pytest.mark.parametrize("case", CROSS, ids=lambda c: f"{len(c[0])}x{c[4]}x{c[6]}")
+def test_packed_rows_with_keys_of_their_own(mm, O, case):
+    lens, kv, (lead, tail), (klead, ktail), H, K, D, dtype, causal, prefix, bias, cap = case
+    off, koff = [lead], [klead]
+    for n, m in zip(lens, kv):
+        off.append(off[-1] + n)
+        koff.append(koff[-1] + m)
+    T, S = off[-1] + tail, koff[-1] + ktail
+    gen = torch.Generator().manual_seed(T + S)
+    q, g = (torch.randn(T, H, D, generator=gen).to(dtype).cuda() for _ in "qg")
+    k, v = (torch.randn(S, K, D, generator=gen).to(dtype).cuda() for _ in "kv")
+    for ts, o in (((q, g), off), ((k, v), koff)):
+        for t in ts:
+            t[:o[0]] = math.nan
+            t[o[-1]:] = math.inf
+    host, opts = {}, dict(causal=causal, cap=cap, offsets=off, kv_offsets=torch.tensor(koff, device="cuda"))
+    if prefix:
+        host["prefix"] = opts["prefix"] = [n // 3 + 5 for n in kv]                # past the keys of some documents
+    if bias:
+        host["slopes"] = opts["slopes"] = slopes_of(H)
+    docs = [(off[d], lens[d], koff[d], kv[d]) for d in range(len(lens))]
+    check(mm, O, q, k, v, docs, opts, g=g, host=host)
+
+
+def test_broadcast_rows_and_gradients(mm):
+    """Tensors and gradients that repeat one row (stride 0) give the bits of their written-out copies."""
+    fn = mm.attention.attention
+    gen = torch.Generator().manual_seed(31)
+    for n, s, H, K in ((70, 70, 2, 2), (300, 300, 4, 2), (1200, 1300, 1, 1), (3, 3000, 4, 1)):
+        q, k, v = (torch.randn(1, 1, h, 64, generator=gen).to(HF).cuda() for h in (H, K, K))
+        g = torch.randn(64, generator=gen).to(HF).cuda()
+        views = [q.expand(2, n, -1, -1), k.expand(2, s, -1, -1), v.expand(2, s, -1, -1), g.expand(2, n, H, 64)]
+
+        def run(q, k, v, g):
+            x = [t.detach().requires_grad_() for t in (q, k, v)]
+            o = fn(*x, causal=True)
+            return (o.detach(),) + torch.autograd.grad(o, x, g)
+        assert all(torch.equal(a, b) for a, b in zip(run(*views), run(*(t.contiguous() for t in views))))
