@@ -311,8 +311,8 @@ int mmfe_rotary_run(const mmfe_rotary* handle, const mmfe_rotary_args* args, voi
  *   packed = 0   n_docs batch entries of q_rows x k_rows; q_len / k_len (device, n_docs entries, clamped to [0, rows]) or NULL = all
  *   packed = 1   document d holds rows q_off[d] .. q_off[d + 1] - 1 of q_rows and keys k_off[d] .. of k_rows (device, n_docs + 1
  *                nondecreasing entries each, clamped to the rows); batch strides are ignored and must be 0
- * 2^-90 <= scale <= 2^126, cap >= 0 and finite.  float16 / bfloat16, head size a multiple of 8 up to 128; strides in elements, multiples of 8, unit stride inside the heads,
- * 16-byte aligned.  Scores, softmax and sums are float32; the softmax's values are rounded to the 16-bit type for the product with v.
+ * float16 / bfloat16, head size a multiple of 8 up to 128; strides in elements, multiples of 8, unit stride inside the heads,
+ * 16-byte aligned; 2^-90 <= scale <= 2^126, cap finite.  Scores, softmax and sums are float32; the softmax's values are rounded to the 16-bit type for the product with v.
  * Values of rows outside a document never enter it; inside one, a NaN or infinity of a key that a causal mask hides may reach rows
  * up to 63 before it.  Asynchronous on hip_stream, allocates nothing. */
 typedef struct mmfe_attention_args {

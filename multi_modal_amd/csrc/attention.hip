@@ -658,7 +658,9 @@ split_fn pick_split(int dim) {
 //   - else chunks that make 512 blocks, two on each CU, of 256 keys at least, and of 1024 at most (documents shorter than their room leave chunks
 //     empty) unless that makes more than 2048: 16 streams of 1000 to 30001 keys in 32768, 4 key heads of 128: 109 / 93 / 100 / 113 us with 512 /
 //     1024 / 2048 / 4096 keys; 32 streams of 2000 keys, one row, 4 key heads of 128: 39 / 34 / 33 with 256 / 512 / 1024.
-// Over all of it a call takes 3 % longer on average than with the best of these choices for it.
+// Over 486 shapes of 1 to 32 documents, 1 to 2048 rows and 500 to 32000 keys (profiles/token_ops_cuts.csv) a call takes 4.6 % longer on average than with the
+// best of these choices for it (documents as long as their room 3.7 %, of uneven lengths 6.2 %), half of them at most 1.3 %; the worst are 8 documents of 512 rows and
+// 1000 to 30001 keys in 32000, 16 heads on 4 of 64, in two parts: 500 us, in six 302.
 struct Cut {
     int row_tiles = 0, chunk = 0, n_splits = 0, cuts = 1;
     int64_t units = 0;
@@ -698,8 +700,8 @@ int64_t in_all(const mmfe_attention_args* a, int64_t rows) { return a->packed ? 
 // is known here; the long ones are taken to have three times as many partners.  Forward and backward, causal, head size 64: 4000 rows, 4 query
 // heads on one key head: 548 us uncut, 126 so; 64 rows over 8000 keys, 6 heads: 234 and 62; 32 documents of 400, 12 heads on 4, which 512 blocks
 // serve: 132, and 151 if cut.  Forward alone: 4000 rows, 2 key heads of 128 and 4 query heads: 104 and 46; one recording of 4000 among 12 of 50, 6 heads: 86
-// and 40.  Over 200 shapes of 1 to 32 documents of 64 to 8000 rows each pass takes 1 to 4 % longer on average than with the best choice
-// for it; the worst is 8 packed recordings of 1000 rows, 6 heads, taken for longer ones: forward and backward 125 us, uncut 107.
+// and 40.  Over 87 shapes of 1 to 32 documents of 64 to 8000 rows (profiles/token_ops_cuts.csv) forward and backward take 3.1 % longer on average than with the best
+// number of parts for the keys' walks, 1.2 % for the rows'; the worst are 2 documents of 300 rows and 3000 keys, 16 heads on 4 of 128: 214 us, uncut 178.
 int walk_cuts(const mmfe_attention_args* a, int64_t rows, int heads, int64_t partners, int64_t want) {
     if (a->n_docs < 1 || rows < 1) return 1;
     const int64_t tiles = (rows + kRows - 1) / kRows, blocks = (a->packed ? tiles : tiles * a->n_docs) * heads;

@@ -587,8 +587,8 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 3 : 2) rows_kernel(const 
 // does all of a head's gradients, with q, k, v and g in LDS, a wave for every 32 rows and then for the 32 keys of the same numbers.  Eight
 // waves and one block per CU; documents of up to 128 take four, and two blocks share a CU.  The tensors are read from memory once, delta is
 // the sum of p dp over the keys, taken in a first walk over them, and neither o nor what its rounding lost is read, or has to be stored by the
-// forward pass.  Bound by the vector instructions around the three exponentials of each score, with the products beside them only in part.
-// 64 clips of 193 rows, 12 heads of 64, float16: 87 us (in four waves with two groups of rows each, two blocks a CU and q and g brought after
+// forward pass.  Neither pipe is full (vector instructions 47 % of a CU's cycles, products 24 %): one block a CU brings its tensors, waits, and computes with nothing beside
+// it, and 193 rows take the products of 224.  64 clips of 193 rows, 12 heads of 64, float16: 84 to 88 us (in four waves with two groups of rows each, two blocks a CU and q and g brought after
 // k and v, 92; by the two passes above and the launch before them, whose blocks wait for their first tiles most of the time, 105), and the
 // forward pass 29 in place of 34 us.
 constexpr int kWholeRows = 256;
